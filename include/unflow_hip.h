@@ -36,7 +36,7 @@ extern "C" {
 /* ABI version of this header (bumped on any signature change).  The library returns the value it was BUILT with; a C user
  * compares `unflow_abi_version() == UNFLOW_ABI_VERSION` (tools/capi_bench.cpp), the Python binding reads this very line
  * (unopticalflow_amd/_lib.py). */
-#define UNFLOW_ABI_VERSION 12
+#define UNFLOW_ABI_VERSION 13
 int unflow_abi_version(void);
 
 /* ---- kernel-exact timing (bench.py's roofline legs; nothing in the reference corresponds) ----
@@ -414,6 +414,42 @@ int unflow_img_pyramid(const float* img, float* half, float* quarter, int planes
 int unflow_prepare_triplets(const uint8_t* src, const long long* offsets, const int* dims,
                             const uint8_t* flip, float* dst, int B, int H, int W, int swap_rb,
                             void* stream);
+
+/* ---- training operators (ABI 13): a classification loss over many classes and an orthogonalising optimiser step.  Nothing in the reference
+ * corresponds.  They take fp32, bf16 and fp16 tensors, 2-byte types aligned to 2 bytes, row-major. */
+#define UNFLOW_DTYPE_FP32 0
+#define UNFLOW_DTYPE_BF16 1
+#define UNFLOW_DTYPE_FP16 2
+
+/* Softmax cross entropy of z = scale * hidden weight^T without holding z:
+ *   hidden [N, D] (rows ldh elements apart), weight [V, D] (rows ldw apart), target int64 [N];
+ *   loss_i = log sum_v exp(z_iv) - z_i,target(i);  0 where target(i) == ignore_index;  NaN where it is otherwise outside [0, V)
+ *   reduction 0: loss [N] holds every loss_i; 1: loss [1] = their sum / the number of rows that are not ignored (at least 1); 2: their sum
+ *   lse [N] is left for the backward pass.
+ * The backward pass takes the upstream gradient gout ([N] for reduction 0, else [1]) and writes dhidden [N, D] and / or dweight [V, D] (dense,
+ * in the inputs' type; NULL: not wanted), working through the classes in pieces.  Sums are fp32, in fixed order (bitwise reproducible).
+ * Workspace: unflow_linear_ce_workspace() says how much each pass needs, 256-byte aligned; its contents mean nothing between calls. */
+#define UNFLOW_LCE_MAX_ROWS (1 << 20)      /* N; split longer batches */
+#define UNFLOW_LCE_MAX_DIM (1 << 20)       /* D, ldh, ldw */
+int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_dhidden, int need_dweight,
+                               long long* forward_bytes, long long* backward_bytes);
+int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V, int D, int dtype, float scale,
+                         long long ignore_index, int reduction, float* loss, float* lse, void* workspace, long long workspace_bytes, void* stream);
+int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* lse, const float* gout, int N, int V, int D, int dtype,
+                         float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, void* workspace, long long workspace_bytes, void* stream);
+
+/* Newton-Schulz orthogonalisation of `count` matrices of any shapes (HOST array of descriptors; everything is enqueued, nothing of it is kept):
+ *   X = x / (|x|_F + eps);  `steps` times  X <- a X + (b S + c S S) X,  S = X X^T  (on the transpose of a matrix with more rows than columns)
+ * and out = X (unflow_orthogonalize), or with momentum as the optimiser step (unflow_muon_step; x = gradient, out = parameter)
+ *   momentum += (1 - mu)(x - momentum);  u = nesterov ? x + mu (momentum - x) : momentum
+ *   out = out (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X(u)
+ * Matrices are dense row-major [rows, cols]; momentum is fp32 whatever the type.  Coefficients whose polynomial leaves [0, 16] are refused. */
+#define UNFLOW_MATRIX_MAX_SIDE (1 << 18)
+typedef struct { const void* x; void* out; float* momentum; int rows, cols; } unflow_matrix;
+int unflow_orthogonalize_workspace(const unflow_matrix* matrices, int count, int dtype, long long* bytes);
+int unflow_orthogonalize(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace, long long workspace_bytes, void* stream);
+int unflow_muon_step(const unflow_matrix* matrices, int count, int dtype, float lr, float momentum, float weight_decay, int nesterov, int steps, float a, float b, float c, float eps,
+                     void* workspace, long long workspace_bytes, void* stream);
 
 /* ---- host helper of the evaluation path (KITTI 16-bit flow PNGs, core/evaluation/flowlib.py:107-127) ----
  * rows: height x (1 + stride) host bytes (filter byte + filtered scanline per row), decoded in place.

@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(PKG, 'libunflow_hip.so')
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
+_F = ctypes.c_float
 
 # name -> argument types (all return int)
 SIGNATURES = {
@@ -100,6 +102,12 @@ SIGNATURES = {
     'unflow_bias_leaky_bwd2_bf16': [_P, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P],
     'unflow_img_pyramid': [_P, _P, _P, _I, _I, _I, _P],
     'unflow_prepare_triplets': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    'unflow_linear_ce_workspace': [_P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _P, _P],
+    'unflow_linear_ce_fwd': [_P, _L, _P, _L, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P],
+    'unflow_linear_ce_bwd': [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P],
+    'unflow_orthogonalize_workspace': [_P, _I, _I, _P],
+    'unflow_orthogonalize': [_P, _I, _I, _I, _F, _F, _F, _F, _P, _L, _P],
+    'unflow_muon_step': [_P, _I, _I, _F, _F, _F, _I, _I, _F, _F, _F, _F, _P, _L, _P],
     'unflow_png_unfilter': [_P, _I, _I, _I],
 }
 
@@ -124,7 +132,7 @@ class UnflowLibraryError(RuntimeError):
 # The ABI this file's SIGNATURES table was written for.  Bump it together with UNFLOW_ABI_VERSION of include/unflow_hip.h whenever an
 # entry point changes: load() wants library == header == this number, so a header bump + rebuild with a stale ctypes table is caught
 # (reading the number from the header alone only detects a stale .so).
-BINDING_ABI = 12
+BINDING_ABI = 13
 
 
 def _abi_version():

@@ -22,16 +22,19 @@ LIB_TUNING = os.path.join(PKG, 'libunflow_hip_tuning.so')
 HOST_LIB = os.path.join(PKG, 'libunflow_host.so')
 TORCH_LIB = os.path.join(PKG, 'libunflow_torch.so')
 SOURCES = ('corr.hip', 'warp.hip', 'warp_corr.hip', 'ssim.hip', 'photo.hip', 'elementwise.hip', 'elementwise_bf16.hip',
-           'prepare.hip', 'optim.hip', 'png_host.cpp')
+           'prepare.hip', 'optim.hip', 'train/linear_ce.hip', 'train/muon.hip', 'png_host.cpp')
 HOST_SOURCES = ('png_host.cpp',)
 # -ffp-contract=off: mask / SSIM arithmetic must follow the reference op by op; the kernels call
 # fmaf() explicitly where a fused multiply-add is wanted.
 FLAGS = ('-O3', '--offload-arch=gfx950', '-fPIC', '-std=c++17', '-ffp-contract=off',
          '-fno-slp-vectorize')   # SLP packs the 2-px FMAs into v_pk_fma_f32 + a v_mov per pair: slower than plain v_fmac
+# The training operators of csrc/train are built without packed fp32 instructions: what their epilogues would gain is nothing next to the
+# matrix products, and some forms of these instructions have given wrong results now and then.
+TRAIN_FLAGS = ('-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops')
 
 
 def _headers():
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
+    deps = [os.path.join(d, f) for d in (CSRC, os.path.join(CSRC, 'train')) for f in os.listdir(d) if f.endswith('.h')]
     bodies = os.path.join(CSRC, 'bodies')                          # kernel bodies that a single-scale and a multi-scale kernel both include
     deps += [os.path.join(bodies, f) for f in sorted(os.listdir(bodies)) if f.endswith('.inc')] if os.path.isdir(bodies) else []
     deps.append(os.path.join(os.path.dirname(PKG), 'include', 'unflow_hip.h'))
@@ -47,7 +50,8 @@ def _newer(target, deps):
 
 
 def _compile(hipcc, src, obj, extra, verbose):
-    cmd = [hipcc, *FLAGS, *extra, '-c', src, '-o', obj]
+    flags = FLAGS + (TRAIN_FLAGS if os.path.basename(os.path.dirname(src)) == 'train' else ())
+    cmd = [hipcc, *flags, *extra, '-c', src, '-o', obj]
     if verbose:
         print(' '.join(cmd), flush=True)
     subprocess.run(cmd, check=True)
@@ -69,7 +73,7 @@ def build(force=False, verbose=True, tuning=False):
     jobs, objs = [], []
     for name in srcs:
         src = os.path.join(CSRC, name)
-        obj = os.path.join(objdir, os.path.splitext(name)[0] + '.o')
+        obj = os.path.join(objdir, os.path.splitext(os.path.basename(name))[0] + '.o')
         objs.append(obj)
         if force or _newer(obj, [src] + hdrs):
             jobs.append((src, obj))

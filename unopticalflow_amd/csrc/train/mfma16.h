@@ -1,0 +1,215 @@
+// C[m][n] = sum_k A[m][k] B[n][k] on the 16-bit matrix instructions: the product every operator of this folder is made of.
+//
+// Operands.  Both are row-major with k contiguous, 16-byte aligned, a leading dimension that is a multiple of 8 elements, and hold one of
+//   ONE plane   bf16 or fp16 numbers as they are
+//   TWO planes  numbers of 22 bits: x = hi + lo, hi = fp16(x), lo = fp16(x - hi).  The planes lie interleaved, 32 k at a time: elements
+//               [64 b, 64 b + 32) of a row are hi of k = 32 b .. 32 b + 31, the next 32 are lo of the same k.
+// A product of TWO-plane operands is hi hi + hi lo + lo hi (lo lo is below 2^-22 of it): three fp16 matrix products give what fp32 ones give,
+// at 2.5 PFLOP/s / 3 against 157 TFLOP/s of v_mfma_f32_16x16x4_f32.  Sums are fp32 in the accumulators in either case.  Values are scaled by a
+// power of two that the caller chooses, so that hi never overflows and lo keeps its bits down to 2^-17 of the largest value.
+//
+// A tile is staged 128 bytes of every row at a time (64 k of ONE plane, 32 k of TWO): the interleaving makes both the same copy.  LDS-DMA,
+// 16 bytes per lane; what lies outside the operand (rows past the end, k past the end) is an offset outside the buffer descriptor, which reads
+// as zero.  A row's eight 16-byte pieces are stored in the order piece ^ (row / 2 mod 8): the 16 lanes of an operand read (16 rows, one piece)
+// then touch each of the 64 banks once.
+#pragma once
+#include "../common.h"
+
+namespace {
+
+typedef unsigned short u16;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum Planes { ONE = 1, TWO = 2 };
+enum Element { BF16 = 0, FP16 = 1 };
+
+__host__ __device__ static inline long long round_up(long long a, long long b) { return (a + b - 1) / b * b; }
+
+// elements of a packed row that holds k numbers
+__host__ __device__ static inline long long packed_width(int planes, long long k) { return planes == TWO ? 2 * round_up(k, 32) : round_up(k, 8); }
+// place of number k in a packed row (its lo plane is 32 further); k, k + 1, .. of an aligned group of 32 are adjacent
+__device__ __forceinline__ long long packed_at(int planes, long long k) { return planes == TWO ? (k >> 5) * 64 + (k & 31) : k; }
+
+template <int EL> __device__ __forceinline__ u16 to_bits(float v) {
+    if constexpr (EL == BF16) return __builtin_bit_cast(u16, (__bf16)v);
+    else return __builtin_bit_cast(u16, (_Float16)v);
+}
+template <int EL> __device__ __forceinline__ float from_bits(u16 v) {
+    if constexpr (EL == BF16) return (float)__builtin_bit_cast(__bf16, v);
+    else return (float)__builtin_bit_cast(_Float16, v);
+}
+
+// one number into a packed row (p: the row's start)
+template <int PL, int EL> __device__ __forceinline__ void pack1(u16* p, long long k, float v) {
+    p += packed_at(PL, k);
+    const u16 hi = to_bits<EL>(v);
+    p[0] = hi;
+    if constexpr (PL == TWO) p[32] = to_bits<EL>(v - from_bits<EL>(hi));
+}
+// four numbers k .. k + 3 (k a multiple of 4)
+template <int PL, int EL> __device__ __forceinline__ void pack4(u16* p, long long k, f32x4 v) {
+    p += packed_at(PL, k);
+    u16 h[4], l[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        h[r] = to_bits<EL>(v[r]);
+        l[r] = to_bits<EL>(v[r] - from_bits<EL>(h[r]));
+    }
+    *reinterpret_cast<u32x2*>(p) = u32x2{h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16};
+    if constexpr (PL == TWO) *reinterpret_cast<u32x2*>(p + 32) = u32x2{l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16};
+}
+template <int PL, int EL> __device__ __forceinline__ f32x4 unpack4(const u16* p, long long k) {
+    p += packed_at(PL, k);
+    const u32x2 h = *reinterpret_cast<const u32x2*>(p);
+    f32x4 v{from_bits<EL>((u16)h[0]), from_bits<EL>((u16)(h[0] >> 16)), from_bits<EL>((u16)h[1]), from_bits<EL>((u16)(h[1] >> 16))};
+    if constexpr (PL == TWO) {
+        const u32x2 l = *reinterpret_cast<const u32x2*>(p + 32);
+        v += f32x4{from_bits<EL>((u16)l[0]), from_bits<EL>((u16)(l[0] >> 16)), from_bits<EL>((u16)l[1]), from_bits<EL>((u16)(l[1] >> 16))};
+    }
+    return v;
+}
+
+template <int EL> __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (EL == BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+struct Operand {
+    const u16* p;          // element (0, 0)
+    long long ld;          // elements from row to row
+    int rows;
+};
+
+constexpr int kStageBytes = 128;                      // of every row
+constexpr unsigned kOutside = 0x80000000u;            // an offset outside every descriptor
+
+// A workgroup of WM x WN waves owns a BM x BN tile; a wave owns (BM / WM) x (BN / WN) of it.  acc[i][j] belongs to the wave's rows
+// 16 i .. and columns 16 j ..; a lane holds row m = 16 i + (lane & 15) and the four columns n = 16 j + 4 (lane >> 4) ..  (the operands go to
+// the instruction in the order B, A, so that the four values a lane holds are neighbours in a row of C).
+template <int BM_, int BN_, int WM_, int WN_, int PL_, int EL_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PL = PL_, EL = EL_;
+    static constexpr int WAVES = WM * WN, THREADS = WAVES * 64, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
+    static constexpr int STAGE = (BM + BN) * kStageBytes;
+    static constexpr int LDS = 2 * STAGE;
+    static constexpr int QA = BM / 8 / WAVES, QB = BN / 8 / WAVES;            // 1 KB copies (8 rows) of a wave per stage
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0, "a wave copies whole groups of 8 rows");
+
+    f32x4 acc[MI][NI];
+
+    __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+    __device__ __forceinline__ static int row(int i) { return (wave() / WN) * TM + i * 16 + ((int)threadIdx.x & 15); }
+    __device__ __forceinline__ static int col(int j) { return (wave() % WN) * TN + j * 16 + (((int)threadIdx.x & 63) >> 4) * 4; }
+
+    // k0, k1: the part of the packed width that is summed (k0 a multiple of 64); m0, n0: the tile's corner.  Every wave of the workgroup calls
+    // this with the same arguments; LDS bytes are free for other use after the barrier that ends it.
+    __device__ __forceinline__ void run(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
+        const int w = wave(), lane = (int)threadIdx.x & 63;
+        const int piece = (lane & 7) ^ (((4 * (w & 1)) + (lane >> 4)) & 7);          // of the row 8 q + lane / 8, q = w + WAVES i
+        const int k_piece = piece * 8;
+        const int ra = A.rows - m0, rb = B.rows - n0;
+        // (a tile spans at most 256 rows of at most 2^21 numbers: its bytes stay below 2^31)
+        const auto da = __builtin_amdgcn_make_buffer_rsrc((void*)(A.p + (long long)m0 * A.ld), 0, 0x7fffffff, 0x00020000);
+        const auto db = __builtin_amdgcn_make_buffer_rsrc((void*)(B.p + (long long)n0 * B.ld), 0, 0x7fffffff, 0x00020000);
+        unsigned oa[QA], ob[QB];
+#pragma unroll
+        for (int i = 0; i < QA; ++i) {
+            const int r = 8 * (w + WAVES * i) + (lane >> 3);
+            oa[i] = r < ra ? (unsigned)((r * A.ld + k0 + k_piece) * 2) : kOutside;
+        }
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            const int r = 8 * (w + WAVES * i) + (lane >> 3);
+            ob[i] = r < rb ? (unsigned)((r * B.ld + k0 + k_piece) * 2) : kOutside;
+        }
+        auto fetch = [&](int t) {
+            char* to = lds + (t & 1) * STAGE;
+            const bool in = k0 + t * 64 + k_piece < k1;
+            const unsigned adv = (unsigned)t * kStageBytes;
+#pragma unroll
+            for (int i = 0; i < QA; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_ptr)(to + (w + WAVES * i) * 1024), 16, (int)(in ? oa[i] + adv : kOutside), 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < QB; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_ptr)(to + BM * kStageBytes + (w + WAVES * i) * 1024), 16, (int)(in ? ob[i] + adv : kOutside), 0, 0, 0);
+        };
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        // operand reads: row 16 i + (lane & 15) of the wave's part, piece 4 s + (lane >> 4) for s = 0, 1 (the two halves of 64 k; hi and lo)
+        const int swz = ((lane & 15) >> 1) & 7, pc = lane >> 4;
+        const int base_a = ((w / WN) * TM + (lane & 15)) * kStageBytes, base_b = BM * kStageBytes + ((w % WN) * TN + (lane & 15)) * kStageBytes;
+        const int p0 = ((pc) ^ swz) * 16, p1 = ((pc + 4) ^ swz) * 16;
+
+        const int stages = (k1 - k0 + 63) / 64;
+        if (stages > 0) fetch(0);
+        for (int t = 0; t < stages; ++t) {
+            UNFLOW_WAIT_VMCNT0();                     // this wave's part of stage t is in LDS,
+            __builtin_amdgcn_s_barrier();             // everyone's is, and nobody reads stage t - 1 any more
+            if (t + 1 < stages) fetch(t + 1);
+            const char* s = lds + (t & 1) * STAGE;
+            uint4 a[MI], b[NI], c[NI];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) b[j] = *reinterpret_cast<const uint4*>(s + base_b + j * 16 * kStageBytes + p0);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const uint4*>(s + base_a + i * 16 * kStageBytes + p0);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(b[j], a[i], acc[i][j]);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) c[j] = *reinterpret_cast<const uint4*>(s + base_b + j * 16 * kStageBytes + p1);
+            if constexpr (PL == TWO) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(c[j], a[i], acc[i][j]);       // a hi, b lo
+            }
+#pragma unroll
+            for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const uint4*>(s + base_a + i * 16 * kStageBytes + p1);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(PL == TWO ? b[j] : c[j], a[i], acc[i][j]);
+        }
+        __syncthreads();
+    }
+};
+
+// Order of the tiles of an mt x nt grid: workgroups of one XCD take neighbouring tiles, and these go down groups of 8 tile rows before the next
+// tile column, so that what runs at one time shares operand rows in the XCD's L2.
+__device__ __forceinline__ void tile_of(int id, int mt, int nt, int& tm, int& tn) {
+    const int group = 8 * nt, g = id / group, first = g * 8;
+    const int size = mt - first < 8 ? mt - first : 8, in = id - g * group;
+    tm = first + in % size;
+    tn = in / size;
+}
+
+// ---- packing an operand
+template <class T> __device__ __forceinline__ float load1(const T* p);
+template <> __device__ __forceinline__ float load1<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float load1<__bf16>(const __bf16* p) { return (float)*p; }
+template <> __device__ __forceinline__ float load1<_Float16>(const _Float16* p) { return (float)*p; }
+
+template <class T> __device__ __forceinline__ void store4(T* p, f32x4 v, int n) {            // n = 1 .. 4 of the four values
+    if (n == 4 && ((size_t)p & (4 * sizeof(T) - 1)) == 0) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p) = v;
+        else {
+            u16 h[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) h[r] = __builtin_bit_cast(u16, (T)v[r]);
+            *reinterpret_cast<u32x2*>(p) = u32x2{h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16};
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < n) p[r] = (T)v[r];
+    }
+}
+
+}  // namespace

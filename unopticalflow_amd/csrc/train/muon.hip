@@ -1,0 +1,540 @@
+// Orthogonalisation by Newton-Schulz products, and the optimiser step made of it (Muon), over a list of matrices of any shapes at once.
+//
+//   X_0 = G / (|G|_F + eps)          (G^T where G has more rows than columns: m <= n from here on)
+//   S = X X^T,  Q = a I + b S + c S S,  X <- Q X,       `steps` times
+//   step: M += (1 - mu)(G - M),  U = G + mu (M - G) (nesterov) or M,  P = P (1 - lr wd) - lr sqrt(max(1, rows / cols)) X(U)
+//
+// S and Q are symmetric: their tiles above the diagonal are not computed but written as the mirror of those below, so a step costs
+// m^2 n + m^3 + 2 m^2 n operations instead of 4 m^2 n + 2 m^3.  The products bound large matrices; a list of small ones is bound by launches,
+// so every phase is one launch over the tiles of all matrices (a wave finds its matrix in a table of running tile counts), 3 launches a step.
+//
+// Numbers (mfma16.h): every type is iterated on as two fp16 planes (22 bits, products and sums as in fp32).  One plane would take a third of
+// the products, and its 2^-12 looks small beside the 2^-9 of a bf16 result, but the iteration multiplies small singular values by a^5 = 485 and
+// what rounding spreads over their directions with them: a bf16 matrix of low rank comes out several percent off that way.  The Frobenius norm is summed in 64 bits.  |X|, |S|, |Q| are bounded by the polynomial over [0, 1], which gives the powers of two that
+// the planes are scaled by.  A matrix whose norm is far below eps comes out as nearly zero, as the definition has it, but without relative
+// accuracy.
+#include "pack.h"
+#include <cmath>
+#include <cstring>
+
+namespace {
+
+constexpr int kFp32 = 0, kBf16 = 1, kFp16 = 2;                     // UNFLOW_DTYPE_*
+constexpr int kChunk = 16384;                                      // numbers a workgroup of the norm takes
+
+struct Problem {
+    const void* x;               // gradient / input
+    void* out;                   // parameter / output
+    float* momentum;
+    long long X, XT0, XT1, S, Q; // byte offsets into the workspace
+    long long shares_at;         // byte offset of the partial sums of S
+    int rows, cols, m, n;
+    int part0, parts;            // its sums of squares
+    int shares;                  // S is summed over n in this many parts
+    float boost;                 // sqrt(max(1, rows / cols))
+};
+static_assert(sizeof(Problem) % 4 == 0, "copied by words");
+
+// running counts of the work items of all problems, one row per phase
+enum { kNorm, kPack, kSquare, kJoin, kPoly, kApply, kPhases };
+
+struct Exponents { int x, s, q; };                                 // planes hold X 2^x, S 2^s, Q 2^q
+
+// host structures into the workspace through kernel arguments: nothing is copied by the runtime, so a captured call holds no host memory
+constexpr int kPiece = 896;
+struct Words { unsigned w[kPiece]; };
+__global__ __launch_bounds__(256) void write_table_kernel(Words src, int count, unsigned* __restrict__ dst) {
+    for (int i = threadIdx.x; i < count; i += 256) dst[i] = src.w[i];
+}
+
+// the problem that work item `id` of a phase belongs to, and the item's number within it
+__device__ __forceinline__ int problem_of(const int* __restrict__ ends, int count, int id, int& local) {
+    const int lane = (int)threadIdx.x & 63;
+    int at = 0;
+    for (int base = 0; base < count; base += 64) {
+        const int e = base + lane < count ? ends[base + lane] : 0x7fffffff;
+        const int before = __popcll(__ballot(e <= id));
+        at += before;
+        if (before < 64) break;
+    }
+    at = __builtin_amdgcn_readfirstlane(at);
+    local = id - (at > 0 ? ends[at - 1] : 0);
+    return at;
+}
+
+__device__ __forceinline__ float direction(float g, float m, float mu, int nesterov) { return nesterov ? g + mu * (m - g) : m; }
+
+// ---- sum of squares of a chunk (after the momentum's update)
+template <class T, bool STEP>
+__global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, float mu, int nesterov, double* __restrict__ parts) {
+    int chunk;
+    const Problem p = table[problem_of(ends, count, (int)blockIdx.x, chunk)];
+    const long long total = (long long)p.rows * p.cols, e0 = (long long)chunk * kChunk;
+    const T* x = (const T*)p.x;
+    double sum = 0.;
+    for (int k = 0; k < kChunk / 1024; ++k) {
+        const long long e = e0 + k * 1024 + threadIdx.x * 4;
+        const long long left = total - e;
+        if (left <= 0) break;
+        const int n = left < 4 ? (int)left : 4;
+        f32x4 v = load4(x + e, n);
+        if constexpr (STEP) {
+            f32x4 m = load4(p.momentum + e, n);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                m[r] = m[r] + (1.f - mu) * (v[r] - m[r]);
+                v[r] = direction(v[r], m[r], mu, nesterov);
+            }
+            store4<float>(p.momentum + e, m, n);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r >= n) v[r] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += (double)v[r] * (double)v[r];
+    }
+    __shared__ double red[256];
+    red[threadIdx.x] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) parts[p.part0 + chunk] = red[0];
+}
+
+// ---- X_0 and its transpose, as planes: a 64 x 64 tile of the matrix per workgroup, both ways
+template <class T, bool STEP>
+__global__ __launch_bounds__(256) void start_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const double* __restrict__ parts, float mu, int nesterov, float eps,
+                                                    Exponents ex, char* __restrict__ ws) {
+    __shared__ float tile[64][65];
+    __shared__ double red[256];
+    int id;
+    const Problem p = table[problem_of(ends, count, (int)blockIdx.x, id)];
+    double sum = 0.;
+    for (int i = threadIdx.x; i < p.parts; i += 256) sum += parts[p.part0 + i];
+    red[threadIdx.x] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    // 2^x / (norm + eps), in two factors: the norm may be far from 1 (the division in 64 bits keeps matrices of huge or tiny numbers exact)
+    const double factor = ldexp(1.0 / (sqrt(red[0]) + (double)eps), ex.x);
+    const int across = ceil_div(p.cols, 64), r0 = id / across * 64, c0 = id % across * 64;
+    const bool wide = p.rows <= p.cols;
+    u16* straight = (u16*)(ws + (wide ? p.X : p.XT0));               // [rows][packed cols]
+    u16* turned = (u16*)(ws + (wide ? p.XT0 : p.X));                 // [cols][packed rows]
+    const long long lds_ = packed_width(TWO, p.cols), ldt = packed_width(TWO, p.rows);
+    const int wide_c = (int)(lds_ / 2), wide_r = (int)(ldt / 2);
+    const int x = (threadIdx.x & 15) * 4, y = threadIdx.x >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + y + 16 * i, c = c0 + x;
+        f32x4 v{0.f, 0.f, 0.f, 0.f};
+        if (r < p.rows && c < p.cols) {
+            const int n = p.cols - c < 4 ? p.cols - c : 4;
+            const long long e = (long long)r * p.cols + c;
+            v = load4((const T*)p.x + e, n);
+            if constexpr (STEP) {
+                const f32x4 m = load4(p.momentum + e, n);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = k < n ? direction(v[k], m[k], mu, nesterov) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (float)((double)v[k] * factor);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tile[y + 16 * i][x + k] = v[k];
+        if (r < p.rows && c < wide_c) pack4<TWO, FP16>(straight + r * lds_, c, v);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = c0 + y + 16 * i, r = r0 + x;
+        if (c < p.cols && r < wide_r) {
+            f32x4 v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = tile[x + k][y + 16 * i];
+            pack4<TWO, FP16>(turned + c * ldt, r, v);
+        }
+    }
+}
+
+// tile `id` of the lower triangle, row by row
+__device__ __forceinline__ void triangle_of(int id, int& tm, int& tn) {
+    tm = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > id) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
+    tn = id - tm * (tm + 1) / 2;
+}
+
+// four numbers of a row of a symmetric matrix [m][packed m], and (off the diagonal tiles) their mirror
+__device__ __forceinline__ void symmetric_store(u16* p, long long ld, int m, int wide, int row, int col, f32x4 v, bool mirror) {
+    if (row < m && col < wide) pack4<TWO, FP16>(p + row * ld, col, v);
+    if (mirror && row < wide) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (col + r < m) pack1<TWO, FP16>(p + (col + r) * ld, row, v[r]);
+    }
+}
+
+// ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves its accumulators for join_kernel
+template <class TileT>
+__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, Exponents ex, char* __restrict__ ws) {
+    UNFLOW_DYNAMIC_LDS(char, lds);
+    int id, tm, tn;
+    const Problem p = table[problem_of(ends, count, xcd_remap((int)blockIdx.x, (int)gridDim.x), id)];
+    triangle_of(id / p.shares, tm, tn);
+    const int share = id % p.shares;
+    const long long ld = packed_width(TWO, p.n), lds_ = packed_width(TWO, p.m);
+    const int stages = ceil_div((int)ld, 64), per = ceil_div(stages, p.shares);
+    const int k0 = share * per * 64, k1 = (share + 1) * per * 64 < (int)ld ? (share + 1) * per * 64 : (int)ld;
+    const Operand X{(const u16*)(ws + p.X), ld, p.m};
+    TileT T;
+    T.run(X, X, k0, k1, tm * TileT::BM, tn * TileT::BN, lds);
+    if (p.shares > 1) {
+        f32x4* to = (f32x4*)(ws + p.shares_at) + (long long)id * (TileT::MI * TileT::NI * TileT::THREADS) + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < TileT::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j) to[(i * TileT::NI + j) * TileT::THREADS] = T.acc[i][j];
+        return;
+    }
+    const float f = ldexpf(1.f, ex.s - 2 * ex.x);
+    const int wide = (int)(lds_ / 2);
+#pragma unroll
+    for (int i = 0; i < TileT::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TileT::NI; ++j)
+            symmetric_store((u16*)(ws + p.S), lds_, p.m, wide, tm * TileT::BM + TileT::row(i), tn * TileT::BN + TileT::col(j), T.acc[i][j] * f, tm != tn);
+}
+template <class TileT>
+__global__ __launch_bounds__(TileT::THREADS) void join_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, Exponents ex, char* __restrict__ ws) {
+    constexpr int EACH = TileT::MI * TileT::NI * TileT::THREADS;
+    int id, tm, tn;
+    const Problem p = table[problem_of(ends, count, (int)blockIdx.x, id)];
+    triangle_of(id, tm, tn);
+    const f32x4* from = (const f32x4*)(ws + p.shares_at) + (long long)id * p.shares * EACH + threadIdx.x;
+    const float f = ldexpf(1.f, ex.s - 2 * ex.x);
+    const long long lds_ = packed_width(TWO, p.m);
+    const int wide = (int)(lds_ / 2);
+#pragma unroll
+    for (int i = 0; i < TileT::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TileT::NI; ++j) {
+            f32x4 v = from[(i * TileT::NI + j) * TileT::THREADS];
+            for (int s = 1; s < p.shares; ++s) v += from[(long long)s * EACH + (i * TileT::NI + j) * TileT::THREADS];
+            symmetric_store((u16*)(ws + p.S), lds_, p.m, wide, tm * TileT::BM + TileT::row(i), tn * TileT::BN + TileT::col(j), v * f, tm != tn);
+        }
+}
+
+// ---- Q = a I + b S + c S S: lower tiles
+template <class TileT>
+__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, float a, float b, float c, Exponents ex,
+                                                                                             char* __restrict__ ws) {
+    UNFLOW_DYNAMIC_LDS(char, lds);
+    int id, tm, tn;
+    const Problem p = table[problem_of(ends, count, xcd_remap((int)blockIdx.x, (int)gridDim.x), id)];
+    triangle_of(id, tm, tn);
+    const long long ld = packed_width(TWO, p.m);
+    const u16* s = (const u16*)(ws + p.S);
+    const Operand S{s, ld, p.m};
+    TileT T;
+    T.run(S, S, 0, (int)ld, tm * TileT::BM, tn * TileT::BN, lds);
+    const float fb = ldexpf(b, ex.q - ex.s), fc = ldexpf(c, ex.q - 2 * ex.s), fa = ldexpf(a, ex.q);
+    const int wide = (int)(ld / 2);
+#pragma unroll
+    for (int i = 0; i < TileT::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TileT::NI; ++j) {
+            const int row = tm * TileT::BM + TileT::row(i), col = tn * TileT::BN + TileT::col(j);
+            f32x4 v{0.f, 0.f, 0.f, 0.f};
+            if (row < p.m && col < wide) {
+                v = unpack4<TWO, FP16>(s + row * ld, col);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = fmaf(fc, T.acc[i][j][r], fb * v[r]) + (row == col + r ? fa : 0.f);
+            }
+            symmetric_store((u16*)(ws + p.Q), ld, p.m, wide, row, col, v, tm != tn);
+        }
+}
+
+// ---- X <- Q X.  LAST: the output, or the parameter's update
+struct Update { float keep, lr; };                                   // 1 - lr wd, lr
+template <class TileT, bool LAST, bool STEP, class T>
+__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int odd, Exponents ex, Update up,
+                                                                                              char* __restrict__ ws) {
+    UNFLOW_DYNAMIC_LDS(char, lds);
+    int id, tm, tn;
+    const Problem p = table[problem_of(ends, count, xcd_remap((int)blockIdx.x, (int)gridDim.x), id)];
+    tile_of(id, ceil_div(p.m, TileT::BM), ceil_div(p.n, TileT::BN), tm, tn);
+    const long long ldm = packed_width(TWO, p.m), ldn = packed_width(TWO, p.n);
+    const Operand Q{(const u16*)(ws + p.Q), ldm, p.m}, XT{(const u16*)(ws + (odd ? p.XT1 : p.XT0)), ldm, p.n};
+    TileT T_;
+    T_.run(Q, XT, 0, (int)ldm, tm * TileT::BM, tn * TileT::BN, lds);
+    const float f = ldexpf(1.f, LAST ? -(ex.q + ex.x) : -ex.q);
+    const int wide_m = (int)(ldm / 2), wide_n = (int)(ldn / 2);
+    u16 *X = (u16*)(ws + p.X), *next = (u16*)(ws + (odd ? p.XT0 : p.XT1));
+    const bool tall = p.rows > p.cols;
+    const float lr = up.lr * p.boost;
+#pragma unroll
+    for (int i = 0; i < TileT::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TileT::NI; ++j) {
+            const int row = tm * TileT::BM + TileT::row(i), col = tn * TileT::BN + TileT::col(j);
+            f32x4 v = T_.acc[i][j] * f;
+            if constexpr (LAST) {
+                if (row >= p.m || col >= p.n) continue;
+                const int n = p.n - col < 4 ? p.n - col : 4;
+                T* out = (T*)p.out;
+                if (!tall) {
+                    out += (long long)row * p.cols + col;
+                    if constexpr (STEP) v = load4(out, n) * up.keep - v * lr;
+                    store4<T>(out, v, n);
+                } else {
+                    out += (long long)col * p.cols + row;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r < n) {
+                            T* o = out + (long long)r * p.cols;
+                            *o = (T)(STEP ? (float)*o * up.keep - v[r] * lr : v[r]);
+                        }
+                }
+            } else {
+                if (row < p.m && col < wide_n) pack4<TWO, FP16>(X + row * ldn, col, v);
+                if (row < wide_m) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (col + r < p.n) pack1<TWO, FP16>(next + (col + r) * ldm, row, v[r]);
+                }
+            }
+        }
+}
+
+// ---- the host side
+using T256t = Tile<256, 256, 2, 4, TWO, FP16>;
+using T128t = Tile<128, 128, 2, 2, TWO, FP16>;
+using T64t = Tile<64, 64, 2, 2, TWO, FP16>;
+
+static const int kSizes[3] = {256, 128, 64};
+
+// One tile size per phase and call: the one with the least time of a model in which the chip's 256 CUs take a tile each, a tile of size t costs
+// t^2 / e(t) for every k, and the phase lasts as long as one tile at least.  e: what part of the 256-tile's rate the smaller ones reach.
+static int best_size(const long long counts[3]) {
+    const double cost[3] = {65536., 16384. / 0.75, 4096. / 0.45};
+    int best = 0;
+    double least = 0.;
+    for (int i = 0; i < 3; ++i) {
+        const double t = cost[i] * (counts[i] > 256 ? counts[i] / 256. : 1.);
+        if (i == 0 || t < least) { best = i; least = t; }
+    }
+    return best;
+}
+
+// Bounds of |X|, |S|, |Q| (spectral norms: every singular value of X_0 is in [0, 1]) over all steps, as powers of two that keep the planes
+// below 2^15 with a quarter to spare.  false: the iteration leaves [0, 16] and is of no use.
+static bool exponents_of(int steps, float a, float b, float c, Exponents& ex) {
+    double mx = 1., ms = 1., mq = 1.;
+    for (int i = 0; i <= 512; ++i) {
+        double s = i / 512.;
+        for (int k = 0; k < steps; ++k) {
+            const double t = s * s, q = fabs(a + b * t + c * t * t);
+            mq = mq > q ? mq : q;
+            s *= q;
+            if (!(s <= 16.)) return false;
+            mx = mx > s ? mx : s;
+        }
+    }
+    ms = mx * mx;
+    if (!(mq <= 4096.)) return false;
+    auto exponent = [](double v) { int e = 15; while (v * 1.25 > 1.) { v *= 0.5; --e; } return e; };
+    ex = Exponents{exponent(mx), exponent(ms), exponent(mq)};
+    return true;
+}
+
+constexpr long long kGroupBytes = 4ll << 30;                         // matrices are taken together as long as their planes fit in this
+
+struct Group {
+    int first, count;
+    int size_s, size_x;                                              // indices into kSizes
+    int total[kPhases];
+    long long table, ends, parts, bytes;
+};
+
+static long long plane_bytes(long long m, long long n) {
+    return round_up(2 * packed_width(TWO, n) * m, 256) + 2 * round_up(2 * packed_width(TWO, m) * n, 256) + 2 * round_up(2 * packed_width(TWO, m) * m, 256);
+}
+static long long lower(long long m, int size) { const long long t = (m + size - 1) / size; return t * (t + 1) / 2; }
+static long long full(long long m, long long n, int size) { return ((m + size - 1) / size) * ((n + size - 1) / size); }
+
+// lays out matrices [first, first + count): problems and running counts on the host, offsets into the workspace
+static Group lay_out(const unflow_matrix* a, int first, int count, Problem* problems, int* ends) {
+    Group g{};
+    g.first = first;
+    g.count = count;
+    long long at = 0;
+    auto take = [&](long long bytes) { const long long p = at; at += round_up(bytes, 256); return p; };
+    g.table = take((long long)sizeof(Problem) * count);
+    g.ends = take(4ll * kPhases * count);
+    long long cs[3] = {}, cx[3] = {}, chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        const long long r = a[first + i].rows, c = a[first + i].cols, m = r < c ? r : c, n = r < c ? c : r;
+        for (int k = 0; k < 3; ++k) { cs[k] += lower(m, kSizes[k]); cx[k] += full(m, n, kSizes[k]); }
+        chunks += (r * c + kChunk - 1) / kChunk;
+    }
+    g.size_s = best_size(cs);
+    g.size_x = best_size(cx);
+    g.parts = take(8 * chunks);
+    const int size = kSizes[g.size_s];
+    // S sums over the long side; where its tiles do not fill the chip the sum is cut into shares of at least 4 stages
+    const long long want = 256 / cs[g.size_s];
+    int part0 = 0, run[kPhases] = {};
+    for (int i = 0; i < count; ++i) {
+        const unflow_matrix& q = a[first + i];
+        Problem p{};
+        p.x = q.x; p.out = q.out; p.momentum = q.momentum;
+        p.rows = q.rows; p.cols = q.cols;
+        p.m = q.rows < q.cols ? q.rows : q.cols;
+        p.n = q.rows < q.cols ? q.cols : q.rows;
+        p.boost = q.rows > q.cols ? sqrtf((float)q.rows / (float)q.cols) : 1.f;
+        p.X = take(2 * packed_width(TWO, p.n) * p.m);
+        p.XT0 = take(2 * packed_width(TWO, p.m) * p.n);
+        p.XT1 = take(2 * packed_width(TWO, p.m) * p.n);
+        p.S = take(2 * packed_width(TWO, p.m) * p.m);
+        p.Q = take(2 * packed_width(TWO, p.m) * p.m);
+        const long long stages = (packed_width(TWO, p.n) + 63) / 64;
+        long long shares = want < stages / 4 ? want : stages / 4;
+        if (shares > 16) shares = 16;
+        if (shares > 1) { const long long per = (stages + shares - 1) / shares; shares = (stages + per - 1) / per; } else shares = 1;
+        p.shares = (int)shares;
+        const int low = (int)lower(p.m, size);
+        if (p.shares > 1) p.shares_at = take(4ll * size * size * low * p.shares);
+        p.part0 = part0;
+        p.parts = (int)(((long long)p.rows * p.cols + kChunk - 1) / kChunk);
+        part0 += p.parts;
+        run[kNorm] += p.parts;
+        run[kPack] += ceil_div(p.rows, 64) * ceil_div(p.cols, 64);
+        run[kSquare] += low * p.shares;
+        run[kJoin] += p.shares > 1 ? low : 0;
+        run[kPoly] += low;
+        run[kApply] += (int)full(p.m, p.n, kSizes[g.size_x]);
+        if (problems) {
+            problems[i] = p;
+            for (int k = 0; k < kPhases; ++k) ends[k * count + i] = run[k];
+        }
+    }
+    for (int k = 0; k < kPhases; ++k) g.total[k] = run[k];
+    g.bytes = at;
+    return g;
+}
+static int group_end(const unflow_matrix* a, int count, int first) {
+    long long bytes = 0;
+    int i = first;
+    for (; i < count && i - first < 1024; ++i) {
+        const long long r = a[i].rows, c = a[i].cols;
+        bytes += plane_bytes(r < c ? r : c, r < c ? c : r);
+        if (i > first && bytes > kGroupBytes) break;
+    }
+    return i;
+}
+
+static bool matrices_ok(const unflow_matrix* a, int count, int dtype) {
+    if (!a || count <= 0 || dtype < kFp32 || dtype > kFp16) return false;
+    for (int i = 0; i < count; ++i)
+        if (a[i].rows <= 0 || a[i].cols <= 0 || a[i].rows > UNFLOW_MATRIX_MAX_SIDE || a[i].cols > UNFLOW_MATRIX_MAX_SIDE) return false;
+    return true;
+}
+
+#define WITH_SIZE(index, ...)                                                                                                  \
+    do {                                                                                                                       \
+        if (index == 0) { using TileT = T256t; __VA_ARGS__; } else if (index == 1) { using TileT = T128t; __VA_ARGS__; } else { using TileT = T64t; __VA_ARGS__; } \
+    } while (0)
+#define LAUNCH_TILES(kernel, count, ...)                                                                                              \
+    do {                                                                                                                              \
+        if (TileT::LDS > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS); \
+        UNFLOW_LAUNCH(kernel, dim3(count), dim3(TileT::THREADS), TileT::LDS, stream, __VA_ARGS__);                                    \
+    } while (0)
+
+static void write_table(const void* src, long long bytes, char* dst, hipStream_t stream) {
+    for (long long at = 0; at < bytes; at += sizeof(Words)) {
+        Words w;
+        const long long n = bytes - at < (long long)sizeof(Words) ? bytes - at : (long long)sizeof(Words);
+        memcpy(w.w, (const char*)src + at, n);
+        UNFLOW_LAUNCH(write_table_kernel, dim3(1), dim3(256), 0, stream, w, (int)(n / 4), (unsigned*)(dst + at));
+    }
+}
+
+template <class T, bool STEP>
+static void iterate(const Group& g, int steps, float a, float b, float c, float eps, float mu, int nesterov, Update up, Exponents ex, char* ws, hipStream_t stream) {
+    const Problem* table = (const Problem*)(ws + g.table);
+    const int* ends = (const int*)(ws + g.ends);
+    double* parts = (double*)(ws + g.parts);
+    const int n = g.count;
+    UNFLOW_LAUNCH((norm_kernel<T, STEP>), dim3(g.total[kNorm]), dim3(256), 0, stream, table, ends + kNorm * n, n, mu, nesterov, parts);
+    UNFLOW_LAUNCH((start_kernel<T, STEP>), dim3(g.total[kPack]), dim3(256), 0, stream, table, ends + kPack * n, n, (const double*)parts, mu, nesterov, eps, ex, ws);
+    for (int k = 0; k < steps; ++k) {
+        WITH_SIZE(g.size_s, LAUNCH_TILES((square_kernel<TileT>), g.total[kSquare], table, ends + kSquare * n, n, ex, ws));
+        if (g.total[kJoin]) WITH_SIZE(g.size_s, UNFLOW_LAUNCH((join_kernel<TileT>), dim3(g.total[kJoin]), dim3(TileT::THREADS), 0, stream, table, ends + kJoin * n, n, ex, ws));
+        WITH_SIZE(g.size_s, LAUNCH_TILES((poly_kernel<TileT>), g.total[kPoly], table, ends + kPoly * n, n, a, b, c, ex, ws));
+        if (k + 1 < steps) WITH_SIZE(g.size_x, LAUNCH_TILES((apply_kernel<TileT, false, false, float>), g.total[kApply], table, ends + kApply * n, n, k & 1, ex, up, ws));
+        else WITH_SIZE(g.size_x, LAUNCH_TILES((apply_kernel<TileT, true, STEP, T>), g.total[kApply], table, ends + kApply * n, n, k & 1, ex, up, ws));
+    }
+}
+
+static int workspace_of(const unflow_matrix* a, int count, int dtype, long long* bytes) {
+    long long most = 0;
+    for (int i = 0; i < count;) {
+        const int e = group_end(a, count, i);
+        const long long b = lay_out(a, i, e - i, nullptr, nullptr).bytes;
+        most = most > b ? most : b;
+        i = e;
+    }
+    *bytes = most;
+    return 0;
+}
+
+template <bool STEP>
+static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca, float cb, float cc, float eps, float mu, int nesterov, Update up, void* workspace, long long workspace_bytes, void* stream_) {
+    Exponents ex;
+    UNFLOW_REQUIRE(exponents_of(steps, ca, cb, cc, ex));
+    long long need = 0;
+    workspace_of(a, count, dtype, &need);
+    UNFLOW_REQUIRE(workspace_bytes >= need);
+    hipStream_t stream = (hipStream_t)stream_;
+    char* ws = (char*)workspace;
+    for (int i = 0; i < count;) {
+        const int e = group_end(a, count, i), n = e - i;
+        static thread_local Problem problems[1024];
+        static thread_local int ends[1024 * kPhases];
+        const Group g = lay_out(a, i, n, problems, ends);
+        write_table(problems, (long long)sizeof(Problem) * n, ws + g.table, stream);
+        write_table(ends, 4ll * kPhases * n, ws + g.ends, stream);
+        if (dtype == kFp32) iterate<float, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
+        else if (dtype == kBf16) iterate<__bf16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
+        else iterate<_Float16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
+        i = e;
+    }
+    return unflow_launch_status();
+}
+
+}  // namespace
+
+extern "C" int unflow_orthogonalize_workspace(const unflow_matrix* matrices, int count, int dtype, long long* bytes) {
+    UNFLOW_REQUIRE(bytes && matrices_ok(matrices, count, dtype));
+    return workspace_of(matrices, count, dtype, bytes);
+}
+
+extern "C" int unflow_orthogonalize(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace, long long workspace_bytes, void* stream) {
+    UNFLOW_REQUIRE(matrices_ok(matrices, count, dtype) && workspace && steps >= 1 && steps <= 64 && eps >= 0.f);
+    for (int i = 0; i < count; ++i) UNFLOW_REQUIRE(matrices[i].x && matrices[i].out);
+    return run<false>(matrices, count, dtype, steps, a, b, c, eps, 0.f, 0, Update{1.f, 0.f}, workspace, workspace_bytes, stream);
+}
+
+extern "C" int unflow_muon_step(const unflow_matrix* matrices, int count, int dtype, float lr, float momentum, float weight_decay, int nesterov, int steps, float a, float b, float c, float eps,
+                                void* workspace, long long workspace_bytes, void* stream) {
+    UNFLOW_REQUIRE(matrices_ok(matrices, count, dtype) && workspace && steps >= 1 && steps <= 64 && eps >= 0.f);
+    for (int i = 0; i < count; ++i) UNFLOW_REQUIRE(matrices[i].x && matrices[i].out && matrices[i].momentum);
+    return run<true>(matrices, count, dtype, steps, a, b, c, eps, momentum, nesterov, Update{1.f - lr * weight_decay, lr}, workspace, workspace_bytes, stream);
+}

@@ -14,7 +14,8 @@ import torch
 from . import _lib
 
 __all__ = ['corr', 'warp_flow', 'warp_flow_masked', 'warp_corr', 'occ_weight', 'occ_weight_stacked', 'masked_mean', 'ssim_loss',
-           'ssim_map', 'smooth2_loss', 'consis_loss', 'multiscale_losses', 'multiscale_supported', 'warp_flow_masked_pyramid', 'bias_leaky_relu_', 'bias_leaky_relu_into', 'upsample_bilinear_scaled', 'loss_combine', 'weighted_mean_sum', 'flow_head', 'img_pyramid']
+           'ssim_map', 'smooth2_loss', 'consis_loss', 'multiscale_losses', 'multiscale_supported', 'warp_flow_masked_pyramid', 'bias_leaky_relu_', 'bias_leaky_relu_into', 'upsample_bilinear_scaled', 'loss_combine', 'weighted_mean_sum', 'flow_head', 'img_pyramid',
+           'linear_cross_entropy', 'orthogonalize']
 
 
 def on_device(t):
@@ -1762,3 +1763,178 @@ def prepare_triplets(images, img_hw, flips=None, device=None, src_is_rgb=True, s
               ctypes.c_void_p(base + 16 * B), _ptr(out), B, H, W,
               1 if src_is_rgb else 0, _stream(), nbytes=sum(sizes) + out.numel() * 4, shape=(B, 3, 3 * H, W))
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# training operators: classification over many classes, orthogonalised updates
+# ------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # UNFLOW_DTYPE_*
+_LCE_MAX_ROWS = _LCE_MAX_DIM = 1 << 20
+_MATRIX_MAX_SIDE = 1 << 18
+_REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+
+
+def _dev_typed(what, *tensors):
+    """All operands on one HIP device and of one of the types the training operators take -> (device, UNFLOW_DTYPE_*)."""
+    first = tensors[0]
+    for t in tensors:
+        if not on_device(t):
+            raise RuntimeError('unopticalflow_amd ops run on an MI355X (HIP) device only; got a %s tensor. There is no CPU fallback.' % t.device)
+        if t.dtype not in _DTYPES or t.dtype != first.dtype:
+            raise TypeError('%s takes fp32, bf16 or fp16 tensors of one type; got %s' % (what, sorted({str(u.dtype) for u in tensors})))
+        if t.device != first.device:
+            raise RuntimeError('operands on different devices: %s vs %s' % (first.device, t.device))
+    return first.device, _DTYPES[first.dtype]
+
+
+def _rows_of(t):
+    """A [rows, cols] tensor the kernels can walk (adjacent columns, rows a fixed distance apart) and that distance."""
+    if t.stride(1) == 1 or t.shape[1] == 1:
+        ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        if t.shape[1] <= ld <= _LCE_MAX_DIM:
+            return t, ld
+    t = t.contiguous()
+    return t, t.shape[1]
+
+
+def _linear_ce_workspaces(hidden, ldh, weight, ldw, need_h, need_w):
+    fwd, bwd = ctypes.c_longlong(), ctypes.c_longlong()
+    _call('unflow_linear_ce_workspace', _ptr(hidden), ldh, _ptr(weight), ldw, hidden.shape[0], weight.shape[0], weight.shape[1],
+          _DTYPES[hidden.dtype], int(need_h), int(need_w), ctypes.byref(fwd), ctypes.byref(bwd))
+    return fwd.value, bwd.value
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, ignore_index, scale, reduction):
+        dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
+        (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
+        (N, D), V = hidden.shape, weight.shape[0]
+        loss = torch.empty(N if reduction == 0 else 1, dtype=torch.float32, device=dev)
+        lse = torch.empty(N, dtype=torch.float32, device=dev)
+        ctx.how = (ignore_index, scale, reduction)
+        if N == 0:
+            loss.zero_()
+        else:
+            with _on(dev):
+                need, _ = _linear_ce_workspaces(hidden, ldh, weight, ldw, False, False)
+                ws = torch.empty(need, dtype=torch.uint8, device=dev)
+                _call('unflow_linear_ce_fwd', _ptr(hidden), ldh, _ptr(weight), ldw, _ptr(target), N, V, D, dtype, scale, ignore_index,
+                      reduction, _ptr(loss), _ptr(lse), _ptr(ws), need, _stream(),
+                      nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+        ctx.save_for_backward(hidden, weight, target, lse)
+        return loss if reduction == 0 else loss.view(())
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        hidden, weight, target, lse = ctx.saved_tensors
+        ignore_index, scale, reduction = ctx.how
+        need_h, need_w = ctx.needs_input_grad[:2]
+        (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
+        (N, D), V = hidden.shape, weight.shape[0]
+        dh = torch.empty((N, D), dtype=hidden.dtype, device=hidden.device) if need_h else None
+        dw = torch.empty((V, D), dtype=weight.dtype, device=weight.device) if need_w else None
+        if N == 0:
+            return dh, dw.zero_() if need_w else None, None, None, None, None
+        with _on(hidden.device):
+            _, need = _linear_ce_workspaces(hidden, ldh, weight, ldw, need_h, need_w)
+            ws = torch.empty(need, dtype=torch.uint8, device=hidden.device)
+            _call('unflow_linear_ce_bwd', _ptr(hidden), ldh, _ptr(weight), ldw, _ptr(target), _ptr(lse), _ptr(g.contiguous()), N, V, D,
+                  _DTYPES[hidden.dtype], scale, ignore_index, reduction, _ptr(dh), _ptr(dw), _ptr(ws), need, _stream(),
+                  nbytes=2 * (N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+        return dh, dw, None, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, reduction='mean'):
+    """Softmax cross entropy of the logits ``scale * hidden @ weight.T`` against ``target``, without holding the logits in either pass.
+
+    ``hidden`` [..., D] and ``weight`` [V, D] are fp32, bf16 or fp16 (one type; any row stride); ``target`` [...] is int64.  The classes may be
+    a vocabulary, or the positions of another feature map that a position is to be matched to (``scale`` = 1 / temperature).  The loss is
+    fp32; both gradients come in the inputs' type, from sums in fp32 (fp32 inputs: products and sums of fp32 accuracy).  ``reduction``:
+    'mean' over the rows that are not ignored (0 if there are none), 'sum', or 'none' (the shape of ``target``).  A row whose target is
+    ``ignore_index`` has loss 0 and no part in the gradients, whatever it holds; any other target outside [0, V) makes its row's loss, and
+    the gradients it reaches, NaN.  Results are bitwise reproducible."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got {!r}".format(reduction))
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError('linear_cross_entropy: hidden [..., D] and weight [V, D] do not fit: {} vs {}'.format(tuple(hidden.shape), tuple(weight.shape)))
+    if target.shape != hidden.shape[:-1] or target.dtype != torch.int64:
+        raise ValueError('linear_cross_entropy: target must be int64 of shape {}, got {} {}'.format(tuple(hidden.shape[:-1]), target.dtype, tuple(target.shape)))
+    if target.device != hidden.device:
+        raise RuntimeError('operands on different devices: %s vs %s' % (hidden.device, target.device))
+    if weight.shape[0] < 1 or not 1 <= weight.shape[1] <= _LCE_MAX_DIM or target.numel() > _LCE_MAX_ROWS or weight.shape[0] >= 1 << 31:
+        raise ValueError('linear_cross_entropy: at least one class, 1 to {} dimensions and at most {} rows; got {} rows, weight {}'.format(
+            _LCE_MAX_DIM, _LCE_MAX_ROWS, target.numel(), tuple(weight.shape)))
+    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]) if hidden.dim() != 2 else hidden, weight, target.reshape(-1).contiguous(),
+                                     int(ignore_index), float(scale), _REDUCTIONS[reduction])
+    return loss.view(target.shape) if reduction == 'none' else loss
+
+
+class _Matrix(ctypes.Structure):
+    _fields_ = [('x', ctypes.c_void_p), ('out', ctypes.c_void_p), ('momentum', ctypes.c_void_p), ('rows', ctypes.c_int), ('cols', ctypes.c_int)]
+
+
+def _polynomial_stays_bounded(steps, coefficients):
+    """Whether ``steps`` times s <- a s + b s^3 + c s^5 keeps the singular values of a normalised matrix, all in [0, 1], within [0, 16]."""
+    a, b, c = coefficients
+    s = np.linspace(0.0, 1.0, 513)
+    for _ in range(steps):
+        q = np.abs(a + b * s ** 2 + c * s ** 4)
+        s = s * q
+        if not (s.max() <= 16.0 and q.max() <= 4096.0):
+            return False
+    return True
+
+
+_bounded = {}                                                                # (steps, coefficients) -> bool: a pure function of its arguments
+
+
+def _check_newton_schulz(what, steps, coefficients, eps):
+    key = (int(steps), tuple(_f32(float(v)) for v in coefficients))
+    if not 1 <= key[0] <= 64 or len(key[1]) != 3 or not float(eps) >= 0.0:
+        raise ValueError('{}: 1 to 64 steps, three coefficients and eps >= 0; got steps={}, coefficients={}, eps={}'.format(what, steps, coefficients, eps))
+    if key not in _bounded:
+        if len(_bounded) > 256:
+            _bounded.clear()
+        _bounded[key] = _polynomial_stays_bounded(*key)
+    if not _bounded[key]:
+        raise ValueError('{}: coefficients {} take singular values in [0, 1] out of [0, 16] within {} steps'.format(what, tuple(coefficients), steps))
+    return key
+
+
+def _newton_schulz(entry, dev, dtype, table, count, args):
+    """One call of an entry point that takes a list of matrices and a workspace."""
+    with _on(dev):
+        need = ctypes.c_longlong()
+        _call('unflow_orthogonalize_workspace', table, count, dtype, ctypes.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _call(entry, table, count, dtype, *args, _ptr(ws), need.value, _stream())
+
+
+def orthogonalize(matrices, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """Newton-Schulz orthogonalisation: x = g / (|g|_F + eps), then ``steps`` times x <- a x + (b s + c s s) x with s = x x^T (on the transpose
+    of a matrix with more rows than columns); with the default coefficients the singular values end up near 1.
+
+    ``matrices``: one tensor [..., rows, cols], or a list of such tensors of any shapes (fp32, bf16 or fp16, one type), all of which are
+    worked on together.  Returns the same in the same type; the iteration has the accuracy of fp32 whatever the type.  Not differentiable: it makes updates out of gradients."""
+    single = torch.is_tensor(matrices)
+    given = [matrices] if single else list(matrices)
+    for t in given:
+        if not torch.is_tensor(t) or t.dim() < 2 or max(t.shape[-2:]) > _MATRIX_MAX_SIDE:
+            raise ValueError('orthogonalize: tensors of two or more dimensions, sides up to {}; got {}'.format(
+                _MATRIX_MAX_SIDE, tuple(t.shape) if torch.is_tensor(t) else type(t)))
+    steps, coefficients = _check_newton_schulz('orthogonalize', steps, coefficients, eps)
+    if not given:
+        return []
+    dev, dtype = _dev_typed('orthogonalize', *given)
+    given = [t.detach().contiguous() for t in given]
+    outs = [torch.empty_like(t) for t in given]
+    size, items = given[0].element_size(), []
+    for t, o in zip(given, outs):
+        each = t.shape[-2] * t.shape[-1]
+        if each:
+            items += [(t.data_ptr() + k * each * size, o.data_ptr() + k * each * size, None, t.shape[-2], t.shape[-1]) for k in range(t.numel() // each)]
+    if items:
+        _newton_schulz('unflow_orthogonalize', dev, dtype, (_Matrix * len(items))(*items), len(items), (steps, *coefficients, float(eps)))
+    return outs[0] if single else outs

@@ -154,3 +154,117 @@ class FlowAdam(torch.optim.Adam):
         _lib.check(rc, 'unflow_adam_multi')
         self.native_steps += 1
         return None
+
+
+# ---- Muon: orthogonalised momentum for matrices
+def _walks_as_matrix(t):
+    """A dense tensor whose first dimension is the outermost one: [shape[0], the rest] in memory order (row-major, channels_last)."""
+    return _dense(t) and (t.shape[0] == 1 or t.stride(0) == t.numel() // t.shape[0])
+
+
+@torch.no_grad()
+def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nesterov=True, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """One Muon step over a list of weights, in place: every weight is a matrix [shape[0], the rest] (csrc/train/muon.hip, one launch per phase
+    over all of them).
+
+        m += (1 - momentum) (g - m);   u = g + momentum (m - g)   (nesterov; else m)
+        p  = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u)
+
+    ``params`` and ``grads`` are fp32, bf16 or fp16 (one type), ``momenta`` fp32 in their parameters' layout (row-major or channels_last;
+    a gradient in another layout is copied).  No weight may appear twice."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError('muon_step_: %d parameters, %d gradients, %d momenta' % (len(params), len(grads), len(momenta)))
+    steps, coefficients = ops._check_newton_schulz('muon_step_', steps, coefficients, eps)
+    keep = [i for i, p in enumerate(params) if p.numel()]
+    params, grads, momenta = ([v[i] for i in keep] for v in (params, grads, momenta))
+    if not params:
+        return
+    dev, dtype = ops._dev_typed('muon_step_', *params, *grads)
+    items = []
+    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        if p.dim() < 2 or g.shape != p.shape or m.shape != p.shape:
+            raise ValueError('muon_step_: parameter, gradient and momentum must have one shape of two or more dimensions: {}, {}, {}'.format(
+                tuple(p.shape), tuple(g.shape), tuple(m.shape)))
+        if m.dtype != torch.float32 or m.device != p.device:
+            raise TypeError('muon_step_: momenta are fp32 on their parameter\'s device; got %s on %s' % (m.dtype, m.device))
+        rows, cols = p.shape[0], p.numel() // p.shape[0]
+        if not _walks_as_matrix(p) or any(a != b and n > 1 for a, b, n in zip(m.stride(), p.stride(), p.shape)) or max(rows, cols) > ops._MATRIX_MAX_SIDE:
+            raise ValueError('muon_step_: a parameter must be dense with its first dimension outermost, its momentum of the same layout, sides up to {}; got shape {}, strides {} and {}'.format(
+                ops._MATRIX_MAX_SIDE, tuple(p.shape), p.stride(), m.stride()))
+        if any(a != b and n > 1 for a, b, n in zip(g.stride(), p.stride(), p.shape)):
+            grads[i] = g = torch.empty_like(p).copy_(g)
+        items.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), rows, cols))
+    if len({x[1] for x in items}) < len(items) or len({x[2] for x in items}) < len(items):
+        raise ValueError('muon_step_: a parameter or momentum appears twice')
+    ops._newton_schulz('unflow_muon_step', dev, dtype, (ops._Matrix * len(items))(*items), len(items),
+                       (float(lr), float(momentum), float(weight_decay), int(bool(nesterov)), steps, *coefficients, float(eps)))
+
+
+class FlowMuon(torch.optim.Optimizer):
+    """Muon for the weights of two or more dimensions (``muon_step_``), Adam (``FlowAdam``) for everything else.
+
+    Two parameter groups: 'matrices' (``lr``, ``momentum``, ``nesterov``, ``weight_decay``) and 'others' (``adam_lr``, betas, eps).  Momentum
+    is kept in fp32 whatever the parameters' type.  Like FlowAdam it can be captured into a hipGraph once ``prepare()`` has created its state."""
+
+    def __init__(self, params, lr=0.02, adam_lr=1e-4, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+        params = [p for p in params]
+        if not params or not all(torch.is_tensor(p) for p in params):
+            raise ValueError('FlowMuon takes a non-empty list of parameters')
+        ops._check_newton_schulz('FlowMuon', steps, coefficients, eps)
+        matrices, others = [p for p in params if p.dim() >= 2], [p for p in params if p.dim() < 2]
+        groups = [{'params': matrices, 'kind': 'matrices', 'lr': lr}] if matrices else []
+        groups += [{'params': others, 'kind': 'others', 'lr': adam_lr}] if others else []
+        super().__init__(groups, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=tuple(coefficients), eps=eps))
+        self._adam = FlowAdam(others, lr=adam_lr) if others else None
+        self._share()
+
+    def _group(self, kind):
+        return next((g for g in self.param_groups if g['kind'] == kind), None)
+
+    def _share(self):
+        """One state for both: the inner Adam keeps its moments in this optimizer's ``state``."""
+        if self._adam is not None:
+            self._adam.state = self.state
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        group = self._group('matrices')
+        for p in group['params'] if group else ():
+            if p in self.state:                # Optimizer.load_state_dict casts to the parameter's type
+                m = self.state[p]['momentum_buffer']
+                self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(m)
+        self._share()
+        if self._adam is not None:
+            self._adam._tables = None
+
+    def _momentum(self, p):
+        st = self.state[p]
+        if 'momentum_buffer' not in st:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('FlowMuon.step() inside a hipGraph capture would have to create its state: call FlowMuon.prepare() before the capture')
+            st['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        return st['momentum_buffer']
+
+    def prepare(self):
+        """Create the state of all parameters now (before a capture)."""
+        group = self._group('matrices')
+        for p in group['params'] if group else ():
+            self._momentum(p)
+        return self._adam.prepare() if self._adam is not None else True
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        g = self._group('matrices')
+        if g is not None:
+            params = [p for p in g['params'] if p.grad is not None]
+            muon_step_(params, [p.grad for p in params], [self._momentum(p) for p in params], lr=g['lr'], momentum=g['momentum'], weight_decay=g['weight_decay'],
+                       nesterov=g['nesterov'], steps=g['steps'], coefficients=g['coefficients'], eps=g['eps'])
+        if self._adam is not None:
+            self._adam.param_groups[0]['lr'] = self._group('others')['lr']
+            self._adam.step()
+        return loss

@@ -136,7 +136,8 @@ def train(cfg):
     if getattr(cfg, 'channels_last', None) is None:
         cfg.channels_last = tuning.default_channels_last()              # NHWC only with MIOpen's measured picks
     model = get_model(cfg.mode)(cfg).to(dev)
-    trainer = FlowTrainer(cfg, model, distributed=(world > 1), use_graph=bool(getattr(cfg, 'graph', 1)), gc_freeze_after=2)
+    trainer = FlowTrainer(cfg, model, distributed=(world > 1), use_graph=bool(getattr(cfg, 'graph', 1)), gc_freeze_after=2,
+                          optimizer=getattr(cfg, 'optimizer', 'adam'), muon_lr=getattr(cfg, 'muon_lr', 0.002))
     if cfg.resume:                                                     # train.py:42-46
         name = 'iter_{}.pth'.format(cfg.iter_start) if cfg.iter_start > 0 else 'last.pth'
         cfg.iter_start = trainer.load(os.path.join(cfg.model_dir, name), map_location=dev)
@@ -227,6 +228,8 @@ def main(argv=None):
     ap.add_argument('--graph', type=int, default=1, help='1 (default): replay the train step as a hipGraph -- one process: forward + backward + Adam in one graph; '
                     'several ranks: forward + backward, one all-reduce, Adam graph (the host enqueues 4 things per step instead of ~3000); '
                     '0: eager launches, gradient pieces all-reduced from hooks during backward.')
+    ap.add_argument('--optimizer', type=str, default='adam', choices=['adam', 'muon'], help='muon: orthogonalised momentum (--muon_lr) for the convolution weights, Adam (--lr) for the biases.')
+    ap.add_argument('--muon_lr', type=float, default=0.002, help='learning rate of --optimizer muon.')
     ap.add_argument('--host_input', type=int, default=0, help='1: resize/flip/scale on the CPU workers (PIL) instead of the GPU.')
     args = ap.parse_args(argv)
     if args.config_file is None:

@@ -23,7 +23,8 @@ _PROCESS_GC_FROZEN = False
 
 class FlowTrainer:
     def __init__(self, cfg, model, distributed=False, allreduce_chunks=4, fused_adam=None, use_graph=False,
-                 single_rank_collectives=False, gc_freeze_after=None, own_adam=None, defer_bias_grads=None):
+                 single_rank_collectives=False, gc_freeze_after=None, own_adam=None, defer_bias_grads=None,
+                 optimizer='adam', muon_lr=0.002):
         self.cfg = cfg
         self.model = model
         self.loss_weights = generate_loss_weights_dict(cfg)
@@ -56,7 +57,13 @@ class FlowTrainer:
             fused_adam = _on_device(params[0])
         if own_adam is None:
             own_adam = fused_adam and _on_device(params[0])
-        if own_adam:
+        if optimizer not in ('adam', 'muon'):
+            raise ValueError("optimizer must be 'adam' or 'muon', got %r" % (optimizer,))
+        if optimizer == 'muon':
+            # the convolution weights by orthogonalised momentum, the biases by Adam (optim.FlowMuon)
+            from .optim import FlowMuon
+            self.optimizer = FlowMuon(params, lr=muon_lr, adam_lr=cfg.lr)
+        elif own_adam:
             # torch.optim.Adam whose step is one HIP launch over all tensors (optim.FlowAdam; same state layout and state_dict)
             from .optim import FlowAdam
             self.optimizer = FlowAdam([{'params': params, 'lr': cfg.lr}])
