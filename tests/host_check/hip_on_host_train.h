@@ -67,3 +67,8 @@ extern "C" __attribute__((weak)) __bf16 __truncsfbf2(float f) {          // roun
     memcpy(&r, &h, 2);
     return r;
 }
+
+// LDS-DMA through a byte range (device_forms.h): landed when the call returns
+typedef hip_on_host::Rsrc byte_range;
+static inline byte_range range_of(const void* p, int bytes) { return byte_range{(char*)p, (unsigned)bytes}; }
+static inline void copy16_to_lds(byte_range r, char* to, unsigned offset) { hip_on_host::buf_load<16>(r, (int)offset, 0, to + (hip_on_host::lane_id & 63u) * 16); }

@@ -75,6 +75,21 @@ __device__ __forceinline__ void lds_wait() {
 template <int N>
 __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
+// LDS-DMA that the compiler does not track (csrc/train): every lane moves 16 bytes from `offset` of a range of bytes to the wave's `to` + 16 * lane;
+// offsets outside the range read as zero.  Through the builtin, hipcc puts a vmcnt(0) in front of every LDS read that follows, which waits for
+// the copies the kernel keeps in flight; here the kernel waits by itself (UNFLOW_WAIT_VMCNT0 before the barrier that hands the bytes over).  The
+// instruction has no register result, so nothing can be used before it has arrived.
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef v4i byte_range;
+__device__ __forceinline__ byte_range range_of(const void* p, int bytes) {
+    const unsigned long long a = (unsigned long long)p;
+    return v4i{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+__device__ __forceinline__ void copy16_to_lds(byte_range r, char* to, unsigned offset) {
+    const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(__attribute__((address_space(3))) char*)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(r) : "memory", "m0");
+}
+
 // wave shifts by one lane (ssim.hip): DPP row shifts across the whole wave, not hipcc's __shfl (= ds_bpermute)
 __device__ __forceinline__ float from_lane_below(float v) {       // lane i <- lane i-1 (0 into lane 0)
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x138, 0xf, 0xf, true));

@@ -269,15 +269,21 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
     T.run(A, B, k0, k1, m0, n0, lds);
     C += (long long)share * A.rows * ldc;
 #pragma unroll
-    for (int i = 0; i < TileT::MI; ++i)
+    for (int i = 0; i < TileT::MI; ++i) {
+        const int m = m0 + TileT::row(i);
+        if (m >= A.rows) continue;
+        float* row = C + (long long)m * ldc;
+        if (!first) {                                                  // (all of a row's loads before its sums: one wait, not one per load)
+            f32x4 old[TileT::NI];
 #pragma unroll
-        for (int j = 0; j < TileT::NI; ++j) {
-            const int m = m0 + TileT::row(i), n = n0 + TileT::col(j);
-            if (m < A.rows && n < ldc) {                               // (ldc: the columns rounded up to 4)
-                f32x4* c = reinterpret_cast<f32x4*>(C + (long long)m * ldc + n);
-                *c = first ? T.acc[i][j] : *c + T.acc[i][j];
-            }
+            for (int j = 0; j < TileT::NI; ++j) old[j] = n0 + TileT::col(j) < ldc ? *reinterpret_cast<const f32x4*>(row + n0 + TileT::col(j)) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j) T.acc[i][j] += old[j];
         }
+#pragma unroll
+        for (int j = 0; j < TileT::NI; ++j)
+            if (n0 + TileT::col(j) < ldc) *reinterpret_cast<f32x4*>(row + n0 + TileT::col(j)) = T.acc[i][j];          // (ldc: the columns rounded up to 4)
+    }
 }
 
 // C = A B^T times the uniform factor, in the gradient's type

@@ -110,31 +110,20 @@ struct Tile {
         const int w = wave(), lane = (int)threadIdx.x & 63;
         const int piece = (lane & 7) ^ (((4 * (w & 1)) + (lane >> 4)) & 7);          // of the row 8 q + lane / 8, q = w + WAVES i
         const int k_piece = piece * 8;
-        const int ra = A.rows - m0, rb = B.rows - n0;
-        // (a tile spans at most 256 rows of at most 2^21 numbers: its bytes stay below 2^31)
-        const auto da = __builtin_amdgcn_make_buffer_rsrc((void*)(A.p + (long long)m0 * A.ld), 0, 0x7fffffff, 0x00020000);
-        const auto db = __builtin_amdgcn_make_buffer_rsrc((void*)(B.p + (long long)n0 * B.ld), 0, 0x7fffffff, 0x00020000);
-        unsigned oa[QA], ob[QB];
-#pragma unroll
-        for (int i = 0; i < QA; ++i) {
-            const int r = 8 * (w + WAVES * i) + (lane >> 3);
-            oa[i] = r < ra ? (unsigned)((r * A.ld + k0 + k_piece) * 2) : kOutside;
-        }
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            const int r = 8 * (w + WAVES * i) + (lane >> 3);
-            ob[i] = r < rb ? (unsigned)((r * B.ld + k0 + k_piece) * 2) : kOutside;
-        }
-        auto fetch = [&](int t) {
+        // The descriptors end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most 256
+        // rows of at most 2^21 numbers: its bytes stay below 2^31.)
+        const int ra = A.rows - m0 < BM ? A.rows - m0 : BM, rb = B.rows - n0 < BN ? B.rows - n0 : BN;
+        const byte_range da = range_of(A.p + (long long)m0 * A.ld, (int)(ra * A.ld * 2));
+        const byte_range db = range_of(B.p + (long long)n0 * B.ld, (int)(rb * B.ld * 2));
+        const unsigned step_a = (unsigned)(8 * WAVES * A.ld * 2), step_b = (unsigned)(8 * WAVES * B.ld * 2);
+        const unsigned at_a = (unsigned)(((8 * w + (lane >> 3)) * A.ld + k0 + k_piece) * 2), at_b = (unsigned)(((8 * w + (lane >> 3)) * B.ld + k0 + k_piece) * 2);
+        // copy q (of QA + QB) of stage t; a stage behind the last one is all zeros
+        auto fetch = [&](int t, int q) {
             char* to = lds + (t & 1) * STAGE;
             const bool in = k0 + t * 64 + k_piece < k1;
             const unsigned adv = (unsigned)t * kStageBytes;
-#pragma unroll
-            for (int i = 0; i < QA; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(da, (lds_ptr)(to + (w + WAVES * i) * 1024), 16, (int)(in ? oa[i] + adv : kOutside), 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < QB; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (lds_ptr)(to + BM * kStageBytes + (w + WAVES * i) * 1024), 16, (int)(in ? ob[i] + adv : kOutside), 0, 0, 0);
+            if (q < QA) copy16_to_lds(da, to + (w + WAVES * q) * 1024, (in ? at_a : kOutside) + (adv + q * step_a));
+            else copy16_to_lds(db, to + BM * kStageBytes + (w + WAVES * (q - QA)) * 1024, (in ? at_b : kOutside) + (adv + (q - QA) * step_b));
         };
 #pragma unroll
         for (int i = 0; i < MI; ++i)
@@ -146,37 +135,63 @@ struct Tile {
         const int base_a = ((w / WN) * TM + (lane & 15)) * kStageBytes, base_b = BM * kStageBytes + ((w % WN) * TN + (lane & 15)) * kStageBytes;
         const int p0 = ((pc) ^ swz) * 16, p1 = ((pc + 4) ^ swz) * 16;
 
+        // The operand reads of one half of a stage and the copies of the stage after the next run under the matrix instructions, a few behind every
+        // row of the wave's part: issued together they would fill their queues and hold up the wave.  No wave waits for LDS or memory but at
+        // the one barrier of a stage, by which its reads of stage t have arrived, its copies of stage t + 1 are in LDS (they had a whole stage),
+        // and the buffer of stage t may be written again.
         const int stages = (k1 - k0 + 63) / 64;
-        if (stages > 0) fetch(0);
+        uint4 a0[MI], b0[NI], a1[MI], b1[NI];
+        constexpr int READS = MI + NI, EACH_READ = (READS + MI - 2) / (MI - 1), EACH_COPY = (QA + QB + MI - 1) / MI;
+        auto read = [&](uint4* a, uint4* b, const char* s, int p, int r) {                      // read r of READS
+            if (r < NI) b[r] = *reinterpret_cast<const uint4*>(s + base_b + p + r * 16 * kStageBytes);
+            else a[r - NI] = *reinterpret_cast<const uint4*>(s + base_a + p + (r - NI) * 16 * kStageBytes);
+        };
+        auto multiply = [&](const uint4* a, const uint4* b, int i) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(b[j], a[i], acc[i][j]);
+        };
+#pragma unroll
+        for (int q = 0; q < QA + QB; ++q) fetch(0, q);
+        UNFLOW_WAIT_VMCNT0();
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int q = 0; q < QA + QB; ++q) fetch(1, q);
+#pragma unroll
+        for (int r = 0; r < READS; ++r) read(a0, b0, lds, p0, r);
         for (int t = 0; t < stages; ++t) {
-            UNFLOW_WAIT_VMCNT0();                     // this wave's part of stage t is in LDS,
-            __builtin_amdgcn_s_barrier();             // everyone's is, and nobody reads stage t - 1 any more
-            if (t + 1 < stages) fetch(t + 1);
             const char* s = lds + (t & 1) * STAGE;
-            uint4 a[MI], b[NI], c[NI];
+            const char* next = lds + (~t & 1) * STAGE;
 #pragma unroll
-            for (int j = 0; j < NI; ++j) b[j] = *reinterpret_cast<const uint4*>(s + base_b + j * 16 * kStageBytes + p0);
+            for (int i = 0; i < MI; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const uint4*>(s + base_a + i * 16 * kStageBytes + p0);
+                for (int r = i * EACH_READ; r < (i + 1) * EACH_READ && r < READS; ++r) read(a1, b1, s, p1, r);
+                multiply(a0, b0, i);
+            }
+            if constexpr (PL == TWO) {                                       // hi hi, hi lo; then lo hi
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+                for (int i = 0; i < MI; ++i) multiply(a0, b1, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            UNFLOW_WAIT_LGKMCNT0();
+            UNFLOW_WAIT_VMCNT0();
+            __builtin_amdgcn_s_barrier();
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(b[j], a[i], acc[i][j]);
+            for (int i = 0; i < MI; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) c[j] = *reinterpret_cast<const uint4*>(s + base_b + j * 16 * kStageBytes + p1);
+                for (int q = i * EACH_COPY; q < (i + 1) * EACH_COPY && q < QA + QB; ++q) fetch(t + 2, q);
+#pragma unroll
+                for (int r = i * EACH_READ; r < (i + 1) * EACH_READ && r < READS; ++r) read(a0, PL == TWO ? b1 : b0, next, p0, r);
+                multiply(a1, PL == TWO ? b0 : b1, i);
+            }
             if constexpr (PL == TWO) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(c[j], a[i], acc[i][j]);       // a hi, b lo
+                for (int j = 0; j < NI; ++j) b0[j] = b1[j];
             }
-#pragma unroll
-            for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const uint4*>(s + base_a + i * 16 * kStageBytes + p1);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(PL == TWO ? b[j] : c[j], a[i], acc[i][j]);
         }
+        UNFLOW_WAIT_VMCNT0();
         __syncthreads();
     }
 };
