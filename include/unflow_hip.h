@@ -425,18 +425,20 @@ int unflow_prepare_triplets(const uint8_t* src, const long long* offsets, const 
  *   hidden [N, D] (rows ldh elements apart), weight [V, D] (rows ldw apart), target int64 [N];
  *   loss_i = log sum_v exp(z_iv) - z_i,target(i);  0 where target(i) == ignore_index;  NaN where it is otherwise outside [0, V)
  *   reduction 0: loss [N] holds every loss_i; 1: loss [1] = their sum / the number of rows that are not ignored (at least 1); 2: their sum
- *   lse [N] is left for the backward pass.
+ *   kept is left for the backward pass: 16 bytes of statistics per row, and inputs that are no operands of the matrix instructions by themselves
+ *   (fp32, or rows that are not multiples of 16 bytes) as they are packed.
  * The backward pass takes the upstream gradient gout ([N] for reduction 0, else [1]) and writes dhidden [N, D] and / or dweight [V, D] (dense,
  * in the inputs' type; NULL: not wanted), working through the classes in pieces.  Sums are fp32, in fixed order (bitwise reproducible).
- * Workspace: unflow_linear_ce_workspace() says how much each pass needs, 256-byte aligned; its contents mean nothing between calls. */
+ * unflow_linear_ce_workspace() says how many bytes are kept and how many each pass needs as workspace (256-byte aligned; its contents mean nothing
+ * between calls).  The alignment of hidden and weight is part of the question: ask with the pointers of the call. */
 #define UNFLOW_LCE_MAX_ROWS (1 << 20)      /* N; split longer batches */
 #define UNFLOW_LCE_MAX_DIM (1 << 20)       /* D, ldh, ldw */
 int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_dhidden, int need_dweight,
-                               long long* forward_bytes, long long* backward_bytes);
+                               long long* kept_bytes, long long* forward_bytes, long long* backward_bytes);
 int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V, int D, int dtype, float scale,
-                         long long ignore_index, int reduction, float* loss, float* lse, void* workspace, long long workspace_bytes, void* stream);
-int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* lse, const float* gout, int N, int V, int D, int dtype,
-                         float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, void* workspace, long long workspace_bytes, void* stream);
+                         long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes, void* stream);
+int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* gout, int N, int V, int D, int dtype,
+                         float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept, void* workspace, long long workspace_bytes, void* stream);
 
 /* Newton-Schulz orthogonalisation of `count` matrices of any shapes (HOST array of descriptors; everything is enqueued, nothing of it is kept):
  *   X = x / (|x|_F + eps);  `steps` times  X <- a X + (b S + c S S) X,  S = X X^T  (on the transpose of a matrix with more rows than columns)

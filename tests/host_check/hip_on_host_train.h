@@ -68,6 +68,20 @@ extern "C" __attribute__((weak)) __bf16 __truncsfbf2(float f) {          // roun
     return r;
 }
 
+// v_mfma_f32_16x16x4_f32: lane l holds row (column) l & 15, k = l >> 4
+static inline hip_on_host_v4f hip_on_host_mfma_16x16x4_f32(float a, float b, hip_on_host_v4f c) {
+    const unsigned me = hip_on_host::lane_id, wave0 = me & ~63u, l = me & 63u;
+    static float fa[1024], fb[1024];
+    fa[me] = a; fb[me] = b;
+    __syncthreads();
+    hip_on_host_v4f d = c;
+    for (int reg = 0; reg < 4; ++reg)
+        for (unsigned k = 0; k < 4; ++k) d[reg] += fa[wave0 + 4u * (l >> 4) + (unsigned)reg + 16u * k] * fb[wave0 + (l & 15u) + 16u * k];
+    __syncthreads();
+    return d;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, x, y, z) hip_on_host_mfma_16x16x4_f32(a, b, c)
+
 // LDS-DMA through a byte range (device_forms.h): landed when the call returns
 typedef hip_on_host::Rsrc byte_range;
 static inline byte_range range_of(const void* p, int bytes) { return byte_range{(char*)p, (unsigned)bytes}; }

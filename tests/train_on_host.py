@@ -69,9 +69,9 @@ def patched():
     if lib is None:
         import pytest
         pytest.skip('needs the ROCm clang++')
-    old = (_lib._lib, ops._stream, ops._on, ops.on_device)
-    _lib._lib, ops._stream, ops._on, ops.on_device = lib, (lambda: None), (lambda d: contextlib.nullcontext()), (lambda t: True)
+    old = (_lib._lib, ops._stream_of, ops._on, ops.on_device)
+    _lib._lib, ops._stream_of, ops._on, ops.on_device = lib, (lambda d: None), (lambda d: contextlib.nullcontext()), (lambda t: True)
     try:
         yield lib
     finally:
-        _lib._lib, ops._stream, ops._on, ops.on_device = old
+        _lib._lib, ops._stream_of, ops._on, ops.on_device = old

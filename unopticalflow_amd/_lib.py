@@ -102,9 +102,9 @@ SIGNATURES = {
     'unflow_bias_leaky_bwd2_bf16': [_P, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P],
     'unflow_img_pyramid': [_P, _P, _P, _I, _I, _I, _P],
     'unflow_prepare_triplets': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
-    'unflow_linear_ce_workspace': [_P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _P, _P],
+    'unflow_linear_ce_workspace': [_P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P],
     'unflow_linear_ce_fwd': [_P, _L, _P, _L, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P],
-    'unflow_linear_ce_bwd': [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P],
+    'unflow_linear_ce_bwd': [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _P, _L, _P],
     'unflow_orthogonalize_workspace': [_P, _I, _I, _P],
     'unflow_orthogonalize': [_P, _I, _I, _I, _F, _F, _F, _F, _P, _L, _P],
     'unflow_muon_step': [_P, _I, _I, _F, _F, _F, _I, _I, _F, _F, _F, _F, _P, _L, _P],

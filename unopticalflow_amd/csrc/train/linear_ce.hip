@@ -16,66 +16,83 @@
 // A row whose target is `ignore_index` has loss 0 and no gradient, whatever its hidden row holds (it is left out of the largest magnitude, and
 // enters the transposed H as zeros: 0 * NaN never meets a sum).  Any other target outside [0, V) makes its row's loss and gradients NaN.
 #include "pack.h"
+#include "plan.h"
 #include <cmath>
 #include <cstring>
 
 namespace {
 
 constexpr int kFp32 = 0, kBf16 = 1, kFp16 = 2;                     // UNFLOW_DTYPE_*
-constexpr int kMaxima = 256;                                       // workgroups that look for the largest magnitude of one input
+constexpr int kMaxima = 1024;                                      // workgroups at most that pack one input, each noting the largest magnitude it met
 
-// Device scalars of one call.
-struct Scalars {
-    int eh, ew;                  // H and W are multiplied by 2^eh, 2^ew when they are packed
-    float gmax;                  // largest finite |upstream| of the rows (reduction none), else 1
-    float factor;                // the uniform factor of both gradients: scale, times the upstream gradient (sum), divided by the count (mean)
-};
+// fp32 rows are packed with a power of two of their own that brings the row's largest magnitude to [2^14, 2^15), their transposes (where rows are
+// what is summed over) with one for the whole matrix.
+struct Exponents { int h, w; };      // of the transposes
+struct Row { float top, inverse, others, unused; };                // of a row: max z, 1 / sum exp(z - top), sum over all classes but the target times that
 
-// ---- largest finite magnitude of W and of the rows of H that count (fp32 only): kMaxima workgroups each, one maximum per workgroup
-__global__ __launch_bounds__(256) void largest_kernel(Source h, Source w, const long long* __restrict__ target, long long ignore, float* __restrict__ maxima) {
-    const Source s = blockIdx.y ? w : h;
-    float m = 0.f;
-    for (long long r = blockIdx.x; r < s.rows; r += kMaxima) {
-        if (blockIdx.y == 0 && target[r] == ignore) continue;
-        const float* p = (const float*)s.p + r * s.ld;
-        for (int c = threadIdx.x; c < s.cols; c += 256) {
-            const float v = fabsf(p[c]);
-            m = v <= 3.4028235e38f ? fmaxf(m, v) : m;
-        }
+__device__ __forceinline__ float finite_magnitude(float m, f32x4 v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float a = fabsf(v[k]);
+        m = a <= 3.4028235e38f ? fmaxf(m, a) : m;
     }
-    __shared__ float red[4];
+    return m;
+}
+__device__ __forceinline__ float wave_largest(float m) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) maxima[blockIdx.y * kMaxima + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    return m;
 }
-// the power of two that brings the largest magnitude to [2^14, 2^15)
-__global__ __launch_bounds__(256) void exponents_kernel(const float* __restrict__ maxima, Scalars* __restrict__ sc) {
-    __shared__ float red[2][4];
-    for (int q = 0; q < 2; ++q) {
-        float m = maxima[q * kMaxima + threadIdx.x];
+__device__ __forceinline__ int exponent_for(float largest) { return largest > 0.f ? 14 - ilogbf(largest) : 0; }
+
+// H and W into packed rows, one launch: the first `blocks_h` workgroups take H (0: H needs no packing), the rest W; a wave takes a row at a time.
+// fp32: the rows' exponents, and the workgroups' largest finite magnitudes of the rows that count (maxima [2][kMaxima]).
+struct Packed { u16 *h, *w; int *eh, *ew; float* maxima; };
+template <class T, int PL, int EL>
+__global__ __launch_bounds__(256) void pack_inputs_kernel(Source h, Source w, int blocks_h, Packed to, long long ldd, int width) {
+    __shared__ float red[4];
+    const bool second = (int)blockIdx.x >= blocks_h;
+    const Source s = second ? w : h;
+    u16* dst = second ? to.w : to.h;
+    const int block = (int)blockIdx.x - (second ? blocks_h : 0), blocks = second ? (int)gridDim.x - blocks_h : blocks_h;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    float all = 0.f;
+    for (int first = block * 4; first < s.rows; first += blocks * 4) {
+        const int r = first + wave < s.rows ? first + wave : s.rows - 1;                  // (waves past the last row repeat it)
+        const T* row = (const T*)s.p + (long long)r * s.ld;
+        int e = 0;
+        if constexpr (PL == TWO) {
+            float m = 0.f;
+            for (int k = lane * 4; k < s.cols; k += 256) m = finite_magnitude(m, load4(row + k, s.cols - k));
+            m = wave_largest(m);
+            e = exponent_for(m);
+            if (!(s.label && s.label[r] == s.skip)) all = fmaxf(all, m);
+            if (lane == 0) (second ? to.ew : to.eh)[r] = e;
+        }
+        for (int k = lane * 4; k < width; k += 256) pack4<PL, EL>(dst + r * ldd, k, scaled(load4(row + k, s.cols - k), e));
+    }
+    if constexpr (PL == TWO) {
+        if (lane == 0) red[wave] = all;
+        __syncthreads();
+        if (threadIdx.x == 0) to.maxima[(second ? kMaxima : 0) + block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
+}
+
+// z of an accumulator of row m and column n
+struct Logits { float scale; const int *eh, *ew; };
+template <int PL> __device__ __forceinline__ f32x4 logits_of(const Logits& l, f32x4 acc, int eh, int n, int last) {
+    acc *= l.scale;
+    if constexpr (PL == TWO) {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        if ((threadIdx.x & 63) == 0) red[q][threadIdx.x >> 6] = m;
+        for (int r = 0; r < 4; ++r) acc[r] = ldexpf(acc[r], -(eh + l.ew[n + r < last ? n + r : last]));
     }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const float* r = red[threadIdx.x];
-        const float m = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
-        const int e = m > 0.f ? 14 - ilogbf(m) : 0;
-        if (threadIdx.x == 0) sc->eh = e; else sc->ew = e;
-    }
+    return acc;
 }
 
-template <int PL> __device__ __forceinline__ float logit_factor(const Scalars* sc, float scale) {
-    if constexpr (PL == TWO) return ldexpf(scale, -(sc->eh + sc->ew));
-    else return scale;
-}
-
-// ---- forward: maximum and sum of exponentials of each row of a tile of z, and the target's z.  partial [tile column][N]
+// ---- forward: of each row of a tile of z the maximum and the sum of exp(z - maximum) over the classes that are not the row's target, and the
+// target's z.  partial [tile column][N]
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void lce_forward_kernel(Operand H, Operand W, int width, const Scalars* __restrict__ sc, float scale,
+__global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand H, Operand W, int width, Logits how,
                                                                                                     const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(W.rows, TileT::BN);
@@ -84,24 +101,26 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
     const int m0 = tm * TileT::BM, n0 = tn * TileT::BN;
     TileT T;
     T.run(H, W, 0, width, m0, n0, lds);
-    const float f = logit_factor<TileT::PL>(sc, scale);
     float2* rows = reinterpret_cast<float2*>(lds);                                       // [WN][BM]
     const int wn = TileT::wave() % TileT::WN, group = ((int)threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
         const long long t = m < H.rows ? target[m] : -1;
+        const int eh = TileT::PL == TWO && m < H.rows ? how.eh[m] : 0;
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < TileT::NI; ++j)
+        for (int j = 0; j < TileT::NI; ++j) {
+            const f32x4 zs = logits_of<TileT::PL>(how, T.acc[i][j], eh, n0 + TileT::col(j), W.rows - 1);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int n = n0 + TileT::col(j) + r;
-                const float z = n < W.rows ? T.acc[i][j][r] * f : -INFINITY;
-                T.acc[i][j][r] = z;
-                if (n == t && n < W.rows) ztarget[m] = z;
+                const float z = n < W.rows ? zs[r] : -INFINITY;
                 top = fmaxf(top, z);
+                if (n == t && n < W.rows) ztarget[m] = z;
+                T.acc[i][j][r] = n == t ? -INFINITY : z;
             }
+        }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float base = top == -INFINITY ? 0.f : top;
@@ -122,21 +141,105 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
 #pragma unroll
         for (int q = 0; q < TileT::WN; ++q) {
             const float2 v = rows[q * TileT::BM + r];
-            if (v.x != -INFINITY) sum += v.y * __expf(v.x - top);
-            else sum += v.y;                                                              // (0, or NaN from a row of NaN, which fmaxf passes over)
+            sum += v.x != -INFINITY ? v.y * __expf(v.x - top) : v.y;                      // (without a maximum: 0, or NaN from NaNs, which fmaxf passes over)
         }
         partial[(long long)tn * H.rows + m0 + r] = make_float2(top, sum);
     }
 }
 
-// the tiles' (maximum, sum) pairs of a row joined in fixed order: 16 rows x 16 shares of the tiles per workgroup
+// ---- forward of few rows (at most 16 NF): reading W is all there is to it.  A workgroup takes 64 classes, its four waves a quarter of D each, four
+// steps of loads in flight; the rows of W go from memory to the matrix instruction as they lie there.  16-bit numbers: 32 k a step, lane l holds
+// k = 8 (l >> 4) .. of row l & 15.  fp32: 16 k a step as four v_mfma_f32_16x16x4_f32, the e-th taking k = 4 (l >> 4) + e -- fp32 arithmetic
+// throughout, and no packing.
+template <class T> struct Few { static constexpr int EACH = 16 / sizeof(T), STEP = 4 * EACH; };
+template <class T> __device__ __forceinline__ f32x4 few_product(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    } else return mfma16<__is_same(T, __bf16) ? BF16 : FP16>(a, b, c);
+}
+template <class T, int NF>
+__global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, long long ldh, const T* __restrict__ W, long long ldw, int N, int V, int D, float scale, const long long* __restrict__ target,
+                                                      float2* __restrict__ partial, float* __restrict__ ztarget) {
+    constexpr int ROWS = 16 * NF, PER = 256 / ROWS, CLASSES = 64 / PER, AHEAD = 4, PITCH = 66;
+    __shared__ float sums[4][ROWS][PITCH];
+    const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int v0 = (int)blockIdx.x * 64, k_lane = (lane >> 4) * Few<T>::EACH, r_lane = lane & 15;
+    const T* wrow[4];
+    const T* hrow[NF];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) wrow[c] = W + (long long)(v0 + 16 * c + r_lane < V ? v0 + 16 * c + r_lane : V - 1) * ldw;          // (classes behind the last repeat it, unused)
+#pragma unroll
+    for (int i = 0; i < NF; ++i) hrow[i] = H + (long long)(16 * i + r_lane < N ? 16 * i + r_lane : N - 1) * ldh;
+    f32x4 acc[4][NF];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < NF; ++i) acc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int steps = ceil_div(D, Few<T>::STEP);
+    for (int first = 0; first < steps; first += 4 * AHEAD) {
+        const int s = first + w;
+        uint4 a[AHEAD][4], b[AHEAD][NF];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = (s + 4 * u) * Few<T>::STEP + k_lane;
+            const bool in = k < D;                                                         // (D is a multiple of what a lane loads)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) a[u][c] = in ? *reinterpret_cast<const uint4*>(wrow[c] + k) : uint4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NF; ++i) b[u][i] = in ? *reinterpret_cast<const uint4*>(hrow[i] + k) : uint4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < NF; ++i) acc[c][i] = few_product<T>(a[u][c], b[u][i], acc[c][i]);
+    }
+    // a lane holds row 16 i + (lane & 15), classes 16 c + 4 (lane >> 4) ..
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < NF; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[w][16 * i + r_lane][16 * c + 4 * (lane >> 4) + r] = acc[c][i][r];
+    __syncthreads();
+    const int m = (int)threadIdx.x / PER, part = (int)threadIdx.x % PER;
+    const long long t = m < N ? target[m] : -1;
+    float z[CLASSES], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < CLASSES; ++c) {
+        const int at = part + PER * c, n = v0 + at;
+        z[c] = n < V ? ((sums[0][m][at] + sums[1][m][at]) + (sums[2][m][at] + sums[3][m][at])) * scale : -INFINITY;
+        top = fmaxf(top, z[c]);
+        if (n == t && n < V) {
+            ztarget[m] = z[c];
+            z[c] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int o = PER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int c = 0; c < CLASSES; ++c) sum += __expf(z[c] - base);
+#pragma unroll
+    for (int o = PER / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (part == 0 && m < N) partial[(long long)blockIdx.x * N + m] = make_float2(top, sum);
+}
+
+// the tiles' (maximum, sum) pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup.  The target's own term joins
+// here: where it outweighs the others, loss = log1p(others / own) and others / all = 1 - p keep the digits that 1 - p would lose.
+template <int R>
 __global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict__ partial, int tiles, int N, int V, const long long* __restrict__ target, long long ignore,
-                                                       const float* __restrict__ ztarget, float* __restrict__ lse, float* __restrict__ losses) {
-    __shared__ float2 part[16][17];
-    const int r = threadIdx.x & 15, share = threadIdx.x >> 4, m = blockIdx.x * 16 + r;
+                                                       const float* __restrict__ ztarget, Row* __restrict__ stats, float* __restrict__ losses) {
+    constexpr int SHARES = 256 / R;
+    __shared__ float2 part[SHARES][R + 1];
+    const int r = threadIdx.x % R, share = threadIdx.x / R, m = blockIdx.x * R + r;
     float top = -INFINITY, sum = 0.f;
     if (m < N)
-        for (int t = share; t < tiles; t += 16) {
+        for (int t = share; t < tiles; t += SHARES) {
             const float2 v = partial[(long long)t * N + m];
             const float both = fmaxf(top, v.x);
             const float base = both == -INFINITY ? 0.f : both;
@@ -145,21 +248,30 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict_
         }
     part[share][r] = make_float2(top, sum);
     __syncthreads();
+    for (int half = SHARES / 2; half > 0; half /= 2) {
+        if (share < half) {
+            const float2 x = part[share][r], y = part[share + half][r];
+            const float both = fmaxf(x.x, y.x);
+            const float base = both == -INFINITY ? 0.f : both;
+            part[share][r] = make_float2(both, x.y * (x.x == -INFINITY ? 1.f : __expf(x.x - base)) + y.y * (y.x == -INFINITY ? 1.f : __expf(y.x - base)));
+        }
+        __syncthreads();
+    }
     if (share == 0 && m < N) {
-        top = -INFINITY;
-        for (int q = 0; q < 16; ++q) top = fmaxf(top, part[q][r].x);
-        const float base = top == -INFINITY ? 0.f : top;
-        sum = 0.f;
-        for (int q = 0; q < 16; ++q) sum += part[q][r].y * (part[q][r].x == -INFINITY ? 1.f : expf(part[q][r].x - base));
-        const float l = base + logf(sum);
+        top = part[0][r].x;
+        const float others = part[0][r].y, base = top == -INFINITY ? 0.f : top;
         const long long t = target[m];
-        lse[m] = l;
-        losses[m] = t == ignore ? 0.f : (t >= 0 && t < V) ? l - ztarget[m] : NAN;
+        const bool known = t >= 0 && t < V;
+        const float zt = known ? ztarget[m] : -INFINITY, own = known ? expf(zt - base) : 0.f, all = others + own;
+        stats[m] = Row{base, 1.f / all, others / all, 0.f};
+        losses[m] = t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) + logf(all);
     }
 }
 
-// loss = sum of the rows' losses (mean: divided by the number of rows that are not ignored, at least 1), one workgroup, fixed order
-__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restrict__ losses, const long long* __restrict__ target, long long ignore, int N, int mean, float* __restrict__ loss) {
+// loss = sum of the rows' losses (mean: divided by the number of rows that are not ignored, at least 1, which is left for the backward pass); one
+// workgroup, fixed order
+__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restrict__ losses, const long long* __restrict__ target, long long ignore, int N, int mean, float* __restrict__ loss,
+                                                          float* __restrict__ count) {
     __shared__ float red[16], cnt[16];
     float s = 0.f, c = 0.f;
     for (int i = threadIdx.x; i < N; i += 1024) {
@@ -173,48 +285,67 @@ __global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restric
     if (threadIdx.x == 0) {
         s = c = 0.f;
         for (int q = 0; q < 16; ++q) { s += red[q]; c += cnt[q]; }
+        count[0] = fmaxf(c, 1.f);
         loss[0] = mean ? s / fmaxf(c, 1.f) : s;
     }
 }
 
 // ---- backward
-// uniform factors and the rows' weights: gscale[m] = upstream gradient of the row (1 where the loss is reduced; 0 where the row is ignored),
-// one workgroup
-__global__ __launch_bounds__(1024) void lce_weights_kernel(const float* __restrict__ gout, int reduction, float scale, const long long* __restrict__ target, long long ignore, int N,
-                                                           int exponents, Scalars* __restrict__ sc, float* __restrict__ weight) {
-    __shared__ float red[16], cnt[16];
-    float top = 0.f, c = 0.f;
+// The upstream gradient: one number for a reduced loss, one per row for reduction none (these relative to the largest, so that fp16 planes hold them).
+struct Upstream { const float* g; const float* largest; const float* count; const long long* target; long long ignore; int reduction; float scale; };
+__device__ __forceinline__ float uniform_factor(const Upstream& u) {
+    return u.reduction == 0 ? u.scale : u.reduction == 1 ? u.scale * u.g[0] / u.count[0] : u.scale * u.g[0];
+}
+__device__ __forceinline__ float row_factor(const Upstream& u, int m) { return u.target[m] == u.ignore ? 0.f : u.reduction == 0 ? u.g[m] : 1.f; }
+
+__global__ __launch_bounds__(1024) void lce_largest_upstream_kernel(Upstream u, int N, float* __restrict__ largest) {
+    __shared__ float red[16];
+    float top = 0.f;
     for (int i = threadIdx.x; i < N; i += 1024) {
-        const bool used = target[i] != ignore;
-        const float g = used ? (reduction == 0 ? gout[i] : 1.f) : 0.f;
-        weight[i] = g;
-        const float a = fabsf(g);
+        const float a = fabsf(row_factor(u, i));
         top = a <= 3.4028235e38f ? fmaxf(top, a) : top;
-        c += used ? 1.f : 0.f;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    c = wave_sum(c);
-    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = top; cnt[threadIdx.x >> 6] = c; }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
-        top = c = 0.f;
-        for (int q = 0; q < 16; ++q) { top = fmaxf(top, red[q]); c += cnt[q]; }
-        sc->gmax = top > 0.f ? top : 1.f;
-        if (!exponents) sc->eh = sc->ew = 0;
-        sc->factor = reduction == 0 ? scale : reduction == 1 ? scale * gout[0] / fmaxf(c, 1.f) : scale * gout[0];
+        for (int q = 0; q < 16; ++q) top = fmaxf(top, red[q]);
+        largest[0] = top > 0.f ? top : 1.f;
     }
+}
+
+// Transposes of a piece of W and (with the first piece) of H, one launch: the first `blocks_w` workgroups take W.  fp32: with the exponent of the
+// largest of the `counts` magnitudes that packing noted, left in `ex`.
+struct Columns { Source s; u16* dst; long long ldd; int width; const float* maxima; int counts; };
+template <class T, int PL, int EL>
+__global__ __launch_bounds__(256) void pack_transposes_kernel(Columns w, Columns h, int blocks_w, Exponents* __restrict__ ex) {
+    __shared__ float red[4];
+    const bool second = (int)blockIdx.x >= blocks_w;
+    const Columns c = second ? h : w;
+    const int id = (int)blockIdx.x - (second ? blocks_w : 0), across = ceil_div(c.width, 64);
+    int e = 0;
+    if constexpr (PL == TWO) {
+        float m = 0.f;
+        for (int i = threadIdx.x; i < c.counts; i += 256) m = fmaxf(m, c.maxima[i]);
+        m = wave_largest(m);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+        __syncthreads();
+        e = exponent_for(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+        if (threadIdx.x == 0 && id == 0) (second ? ex->h : ex->w) = e;
+    }
+    pack_columns_tile<T, PL, EL>(c.s, e, c.dst, c.ldd, c.width, id % across, id / across);
 }
 
 // fp16 planes hold probabilities times 2^14: 11 (22) bits of every probability down to 2^-28 (2^-17)
 template <int EL> __host__ __device__ constexpr int probability_exponent() { return EL == FP16 ? 14 : 0; }
 
 // a piece of G and of its transpose: classes [v0, v0 + vp).  G [N][packed vp] holds p - [v = t] (0 where the row is ignored), GT [vp][packed N] the
-// same times the row's weight / gmax; columns behind N and vp up to the packed width are zero
+// same times the row's upstream gradient relative to the largest; columns behind N and vp up to the packed width are zero
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void lce_gradient_kernel(Operand H, Operand W, int width, const Scalars* __restrict__ sc, float scale,
-                                                                                                     const long long* __restrict__ target, const float* __restrict__ lse, const float* __restrict__ weight,
-                                                                                                     long long ignore, int v0, int vp, int V, u16* __restrict__ G, long long ldg, u16* __restrict__ GT, long long ldgt) {
+__global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand H, Operand W, int width, Logits how,
+                                                                                                     const Row* __restrict__ stats, Upstream up, int v0, int vp, int V, u16* __restrict__ G, long long ldg,
+                                                                                                     u16* __restrict__ GT, long long ldgt) {
     constexpr int PL = TileT::PL, EL = TileT::EL;
     UNFLOW_DYNAMIC_LDS(char, lds);
     const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(vp, TileT::BN);
@@ -224,181 +355,189 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
     TileT T;
     const Operand piece{W.p + (long long)v0 * W.ld, W.ld, vp};
     T.run(H, piece, 0, width, m0, n0, lds);
-    const float f = logit_factor<TileT::PL>(sc, scale), unit = (float)(1 << probability_exponent<EL>()), inv = 1.f / sc->gmax;
-    const int wide_n = PL == TWO ? (int)round_up(vp, 32) : (int)round_up(vp, 8), wide_m = PL == TWO ? (int)round_up(H.rows, 32) : (int)round_up(H.rows, 8);
+    how.ew += PL == TWO ? v0 : 0;
+    const float unit = (float)(1 << probability_exponent<EL>());
+    const int wide_n = (int)round_up(vp, PL == TWO ? 32 : 8);
+    float weights[TileT::MI];
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
         const bool there = m < H.rows;
-        const long long t = there ? target[m] : ignore;
-        const bool used = t != ignore, known = t >= 0 && t < V;
-        const float l = there ? lse[m] : 0.f, wgt = there ? weight[m] * inv : 0.f;
+        const long long t = there ? up.target[m] : up.ignore;
+        const bool used = there && t != up.ignore, known = t >= 0 && t < V;
+        const Row s = there ? stats[m] : Row{0.f, 0.f, 0.f, 0.f};
+        weights[i] = !used ? 0.f : up.reduction == 0 ? up.g[m] / up.largest[0] : 1.f;
+        const int eh = PL == TWO && there ? how.eh[m] : 0;
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j) {
             const int n = n0 + TileT::col(j);
+            const f32x4 z = logits_of<PL>(how, T.acc[i][j], eh, n, vp - 1);
             f32x4 g;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float p = __expf(T.acc[i][j][r] * f - l);
-                if (v0 + n + r == t) p -= 1.f;
+                float p = __expf(z[r] - s.top) * s.inverse;
+                if (v0 + n + r == t) p = -s.others;
                 p = used ? (known ? p : NAN) : 0.f;
                 g[r] = n + r < vp ? p * unit : 0.f;
             }
+            T.acc[i][j] = g;
             if (there && n < wide_n) pack4<PL, EL>(G + (long long)m * ldg, n, g);
-            if (m < wide_m) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < vp) pack1<PL, EL>(GT + (long long)(n + r) * ldgt, m, used ? g[r] * wgt : 0.f);
-            }
         }
     }
+    // (a row that is not used, or behind the last, is zeros already: 0 times its weight)
+    if (GT) T.store_transposed(lds, GT, ldgt, vp, ldgt, m0, n0, [&](int i, int j) { return T.acc[i][j] * weights[i]; });
 }
 
-// C = A B^T over share `s` of `shares` of the packed width, added to (or, with `first`, stored in) fp32 sums [shares][rows of A][ldc]
+template <class TileT> struct OutputOf { using type = __bf16; };
+template <int BM, int BN, int WM, int WN> struct OutputOf<Tile<BM, BN, WM, WN, ONE, FP16>> { using type = _Float16; };
+template <int BM, int BN, int WM, int WN> struct OutputOf<Tile<BM, BN, WM, WN, TWO, FP16>> { using type = float; };
+
+// The two products of a piece, one launch: job 0 is dH += G W, job 1 dW = G^T H.  C = A B^T in `shares` shares of what is summed.  A job without
+// `sums` is one share and goes to the gradient as it is; else the shares' accumulators go to fp32 sums [shares][rows of A][ldc], added to what
+// is there unless it is the first piece.
+struct Product { Operand A, B; int width, shares, tiles; float* sums; long long ldc; int first; void* out; int by_h; };
+
+// what turns a job's sums into gradients: the uniform factor, and the row's own (dH; for dW it is in GT, relative to the largest)
+template <int PL, int EL> __device__ __forceinline__ float product_factor(const Exponents* ex, const Upstream& up, int by_h) {
+    float f = uniform_factor(up) * (by_h && up.reduction == 0 ? up.largest[0] : 1.f);
+    if constexpr (PL == TWO) f = ldexpf(f, -(by_h ? ex->h : ex->w));
+    return ldexpf(f, -probability_exponent<EL>());
+}
+
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void gather_product_kernel(Operand A, Operand B, int width, int shares, float* __restrict__ C, long long ldc, int first) {
+__global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product a, Product b, const Exponents* __restrict__ ex, Upstream up) {
+    using T_ = typename OutputOf<TileT>::type;
     UNFLOW_DYNAMIC_LDS(char, lds);
-    const int mt = ceil_div(A.rows, TileT::BM), nt = ceil_div(B.rows, TileT::BN);
-    const int id = xcd_remap((int)blockIdx.x, (int)gridDim.x), share = id / (mt * nt);
+    // (each job is dealt over the XCDs by itself: their units differ in length)
+    const int units_a = a.tiles * a.shares;
+    const bool second = (int)blockIdx.x >= units_a;
+    const Product p = second ? b : a;
+    const int id = second ? xcd_remap((int)blockIdx.x - units_a, (int)gridDim.x - units_a) : xcd_remap((int)blockIdx.x, units_a);
+    const int share = id / p.tiles;
     int tm, tn;
-    tile_of(id % (mt * nt), mt, nt, tm, tn);
+    tile_of(id % p.tiles, ceil_div(p.A.rows, TileT::BM), ceil_div(p.B.rows, TileT::BN), tm, tn);
     const int m0 = tm * TileT::BM, n0 = tn * TileT::BN;
-    const int stages = ceil_div(width, 64), per = ceil_div(stages, shares);
-    const int k0 = share * per * 64, k1 = (share + 1) * per * 64 < width ? (share + 1) * per * 64 : width;
+    const int per = ceil_div(ceil_div(p.width, 64), p.shares) * 64;
+    const int k0 = share * per, k1 = k0 + per < p.width ? k0 + per : p.width;
     TileT T;
-    T.run(A, B, k0, k1, m0, n0, lds);
-    C += (long long)share * A.rows * ldc;
+    T.run(p.A, p.B, k0, k1, m0, n0, lds);
+    if (p.sums) {
+        float* C = p.sums + (long long)share * p.A.rows * p.ldc;
+#pragma unroll
+        for (int i = 0; i < TileT::MI; ++i) {
+            const int m = m0 + TileT::row(i);
+            if (m >= p.A.rows) continue;
+            float* row = C + (long long)m * p.ldc;
+            if (!p.first) {                                            // (all of a row's loads before its sums: one wait, not one per load)
+                f32x4 old[TileT::NI];
+#pragma unroll
+                for (int j = 0; j < TileT::NI; ++j) old[j] = n0 + TileT::col(j) < p.ldc ? *reinterpret_cast<const f32x4*>(row + n0 + TileT::col(j)) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < TileT::NI; ++j) T.acc[i][j] += old[j];
+            }
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j)
+                if (n0 + TileT::col(j) < p.ldc) *reinterpret_cast<f32x4*>(row + n0 + TileT::col(j)) = T.acc[i][j];   // (ldc: the columns rounded up to 4)
+        }
+        return;
+    }
+    const float f = product_factor<TileT::PL, TileT::EL>(ex, up, p.by_h);
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
-        if (m >= A.rows) continue;
-        float* row = C + (long long)m * ldc;
-        if (!first) {                                                  // (all of a row's loads before its sums: one wait, not one per load)
-            f32x4 old[TileT::NI];
+        if (m >= p.A.rows) continue;
+        const float fm = p.by_h ? f : f * row_factor(up, m);
 #pragma unroll
-            for (int j = 0; j < TileT::NI; ++j) old[j] = n0 + TileT::col(j) < ldc ? *reinterpret_cast<const f32x4*>(row + n0 + TileT::col(j)) : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < TileT::NI; ++j) T.acc[i][j] += old[j];
+        for (int j = 0; j < TileT::NI; ++j) {
+            const int n = n0 + TileT::col(j), left = p.B.rows - n;
+            if (left > 0) store4<T_>((T_*)p.out + (long long)m * p.B.rows + n, T.acc[i][j] * fm, left < 4 ? left : 4);
         }
-#pragma unroll
-        for (int j = 0; j < TileT::NI; ++j)
-            if (n0 + TileT::col(j) < ldc) *reinterpret_cast<f32x4*>(row + n0 + TileT::col(j)) = T.acc[i][j];          // (ldc: the columns rounded up to 4)
     }
 }
 
-// C = A B^T times the uniform factor, in the gradient's type
-template <class TileT, class T_>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void weight_product_kernel(Operand A, Operand B, int width, const Scalars* __restrict__ sc, T_* __restrict__ C, long long ldc) {
-    UNFLOW_DYNAMIC_LDS(char, lds);
-    const int mt = ceil_div(A.rows, TileT::BM), nt = ceil_div(B.rows, TileT::BN);
-    int tm, tn;
-    tile_of(xcd_remap((int)blockIdx.x, (int)gridDim.x), mt, nt, tm, tn);
-    const int m0 = tm * TileT::BM, n0 = tn * TileT::BN;
-    TileT T;
-    T.run(A, B, 0, width, m0, n0, lds);
-    const float f = ldexpf(sc->factor * sc->gmax, -sc->eh - probability_exponent<TileT::EL>());
-#pragma unroll
-    for (int i = 0; i < TileT::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < TileT::NI; ++j) {
-            const int m = m0 + TileT::row(i), n = n0 + TileT::col(j), left = B.rows - n;
-            if (m < A.rows && left > 0) store4<T_>(C + (long long)m * ldc + n, T.acc[i][j] * f, left < 4 ? left : 4);
-        }
-}
-
-// gradient = (sum of the shares, in order) * uniform factor * (the row's weight), in the gradient's type
-template <class T_>
-__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ C, long long ldc, int shares, int rows, int cols, const Scalars* __restrict__ sc, int by_h, int unit_exponent,
-                                                     const float* __restrict__ weight, T_* __restrict__ out, long long ldo) {
-    const float f = ldexpf(sc->factor * (weight ? 1.f : sc->gmax), -(by_h ? sc->eh : sc->ew) - unit_exponent);
-    const long long per = ldc / 4, total = per * rows;
-    for (long long g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
+// gradients = sums over the shares, in order, times the factors; one launch for the jobs that have sums (blocks of the first, then of the second)
+template <class T_, int PL, int EL>
+__global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, int blocks_a, const Exponents* __restrict__ ex, Upstream up) {
+    const bool second = (int)blockIdx.x >= blocks_a;
+    const Product p = second ? b : a;
+    const int block = (int)blockIdx.x - (second ? blocks_a : 0), blocks = second ? (int)gridDim.x - blocks_a : blocks_a;
+    const float f = product_factor<PL, EL>(ex, up, p.by_h);
+    const int rows = p.A.rows, cols = p.B.rows;
+    const long long per = p.ldc / 4, total = per * rows;
+    for (long long g = block * 256ll + threadIdx.x; g < total; g += blocks * 256ll) {
         const long long r = g / per;
         const int n = (int)(g - r * per) * 4;
-        f32x4 v = *reinterpret_cast<const f32x4*>(C + r * ldc + n);
-        for (int s = 1; s < shares; ++s) v += *reinterpret_cast<const f32x4*>(C + ((long long)s * rows + r) * ldc + n);
-        v *= weight ? f * weight[r] : f;
-        store4<T_>(out + r * ldo + n, v, cols - n < 4 ? cols - n : 4);
+        f32x4 v = *reinterpret_cast<const f32x4*>(p.sums + r * p.ldc + n);
+        for (int s = 1; s < p.shares; ++s) v += *reinterpret_cast<const f32x4*>(p.sums + ((long long)s * rows + r) * p.ldc + n);
+        v *= p.by_h ? f : f * row_factor(up, (int)r);
+        store4<T_>((T_*)p.out + r * cols + n, v, cols - n < 4 ? cols - n : 4);
     }
 }
 
 // ---- the host side
-using T256b = Tile<256, 256, 2, 4, ONE, BF16>;
-using T128b = Tile<128, 128, 2, 2, ONE, BF16>;
-using T64b = Tile<64, 64, 2, 2, ONE, BF16>;
-using T256h = Tile<256, 256, 2, 4, ONE, FP16>;
-using T128h = Tile<128, 128, 2, 2, ONE, FP16>;
-using T64h = Tile<64, 64, 2, 2, ONE, FP16>;
-using T256t = Tile<256, 256, 2, 4, TWO, FP16>;
-using T128t = Tile<128, 128, 2, 2, TWO, FP16>;
-using T64t = Tile<64, 64, 2, 2, TWO, FP16>;
-
-static int tiles(long long m, long long n, int size) { return (int)(((m + size - 1) / size) * ((n + size - 1) / size)); }
-// The largest tile that still gives every CU one (256 of them): a tile of twice the side reads half as much per product.  Below that the chip
-// is not full and the smaller tile wins.
-static int tile_size(long long m, long long n) { return tiles(m, n, 256) >= 224 ? 256 : tiles(m, n, 128) >= 224 ? 128 : 64; }
-
-#define WITH_TILE(planes, el, size, ...)                                                                                      \
-    do {                                                                                                                      \
-        if (planes == TWO) { if (size == 256) { using TileT = T256t; __VA_ARGS__; } else if (size == 128) { using TileT = T128t; __VA_ARGS__; } else { using TileT = T64t; __VA_ARGS__; } } \
-        else if (el == FP16) { if (size == 256) { using TileT = T256h; __VA_ARGS__; } else if (size == 128) { using TileT = T128h; __VA_ARGS__; } else { using TileT = T64h; __VA_ARGS__; } } \
-        else { if (size == 256) { using TileT = T256b; __VA_ARGS__; } else if (size == 128) { using TileT = T128b; __VA_ARGS__; } else { using TileT = T64b; __VA_ARGS__; } }                   \
-    } while (0)
-
-#define LAUNCH_TILES(kernel, count, ...)                                                                                      \
-    do {                                                                                                                      \
+#define LAUNCH_TILES(kernel, count, ...)                                                                                              \
+    do {                                                                                                                              \
         if (TileT::LDS > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS); \
-        UNFLOW_LAUNCH(kernel, dim3(count), dim3(TileT::THREADS), TileT::LDS, stream, __VA_ARGS__);                            \
+        UNFLOW_LAUNCH(kernel, dim3(count), dim3(TileT::THREADS), TileT::LDS, stream, __VA_ARGS__);                                    \
     } while (0)
-
-// What a call needs of its workspace, and where.
-struct Plan {
-    int planes, el;
-    bool pack_h, pack_w;                 // the inputs are not operands as they are
-    long long wd, wn;                    // packed width of D and of N
-    int size_z;                          // tile of the logits
-    // forward
-    long long scalars, maxima, hp, wp, partial, ztarget, losses, forward_bytes;
-    // backward
-    int vp, size_g, size_h, size_w, shares_h, shares_w;
-    long long wvp, ldh_sum, ldw_sum;
-    long long weight, ht, wt, g, gt, sum_h, sum_w, backward_bytes;
-};
-
-static bool as_is(const void* p, long long ld, int D, int dtype) { return dtype != kFp32 && D % 8 == 0 && ld % 8 == 0 && ((size_t)p & 15) == 0; }
-
-// Products whose tiles do not fill the chip are cut along what they sum over, into at most 16 shares of at least 8 stages.
-static int shares_of(long long m, long long n, int size, long long width) {
-    const long long stages = (width + 63) / 64;
-    long long want = 256 / tiles(m, n, size);
-    if (want > stages / 8) want = stages / 8;
-    if (want > 16) want = 16;
-    if (want <= 1) return 1;
-    const long long per = (stages + want - 1) / want;          // (no share is empty)
-    return (int)((stages + per - 1) / per);
+template <int PL, int EL, class F> static void with_tile(int size, F&& f) {
+    if (size == 0) f(Tile<256, 256, 2, 4, PL, EL>{});
+    else if (size == 1) f(Tile<192, 192, 2, 4, PL, EL>{});
+    else if (size == 2) f(Tile<128, 128, 2, 2, PL, EL>{});
+    else f(Tile<64, 64, 2, 2, PL, EL>{});
 }
 
-static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, bool need_h, bool need_w) {
+// What a call needs of its buffers, and where.  `kept`: what the forward pass leaves for the backward pass.
+struct Plan {
+    int planes;
+    bool few, pack_h, pack_w, keeps;
+    long long wd, wn;                    // packed widths of D and N
+    long long stats, maxima, eh, ew, hp, wp, kept_bytes;
+    int size_z;
+    long long partial, ztarget, losses, forward_bytes;
+    int vp, size_g, size_p, limit;
+    long long wvp, ldc;
+    long long repacked, exponents, largest, g, gt, ht, wt, sum_h, sum_w, backward_bytes;
+};
+
+// 16-byte loads of whole rows
+static bool aligned(const void* p, long long ld, int D, int dtype) {
+    const int each = dtype == kFp32 ? 4 : 8;
+    return D % each == 0 && ld % each == 0 && ((size_t)p & 15) == 0;
+}
+
+static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, bool train, bool need_h, bool need_w) {
     Plan p{};
     p.planes = dtype == kFp32 ? TWO : ONE;
-    p.el = dtype == kBf16 ? BF16 : FP16;
-    p.pack_h = !as_is(h, ldh, D, dtype);
-    p.pack_w = !as_is(w, ldw, D, dtype);
+    p.few = N <= 64 && aligned(h, ldh, D, dtype) && aligned(w, ldw, D, dtype);
+    p.pack_h = dtype == kFp32 || !aligned(h, ldh, D, dtype);
+    p.pack_w = dtype == kFp32 || !aligned(w, ldw, D, dtype);
+    p.keeps = (p.pack_h || p.pack_w) && !p.few;
     p.wd = packed_width(p.planes, D);
     p.wn = packed_width(p.planes, N);
     long long at = 0;
     auto take = [&](long long bytes) { const long long a = at; at += round_up(bytes, 256); return a; };
-    p.scalars = take(sizeof(Scalars));
-    p.maxima = take(2 * kMaxima * 4);
-    p.hp = p.pack_h ? take(2 * p.wd * N) : 0;
-    p.wp = p.pack_w ? take(2 * p.wd * V) : 0;
-    const long long common = at;
-    p.size_z = tile_size(N, V);
-    p.partial = take(8ll * ceil_div(V, p.size_z) * N);
+    p.stats = take(4ll * (4 * (long long)N + 1));
+    const long long bare = at;
+    if (p.planes == TWO) {
+        p.maxima = take(2 * kMaxima * 4);
+        p.eh = take(4ll * N);
+        p.ew = take(4ll * V);
+    }
+    if (p.pack_h) p.hp = take(2 * p.wd * N);
+    if (p.pack_w) p.wp = take(2 * p.wd * V);
+    const long long packed = at;
+    p.kept_bytes = p.keeps ? packed : bare;
+    at = 0;
+    const Job z{N, V, stages_of(p.wd), false, false};
+    p.size_z = choose(p.planes, &z, 1).size;
+    p.partial = take(8ll * ceil_div(V, p.few ? 64 : kSizes[p.size_z]) * N);
     p.ztarget = take(4ll * N);
     p.losses = take(4ll * N);
     p.forward_bytes = at;
-    at = common;
+    if (!train) return p;
+    at = 0;
+    if (p.few && (p.pack_h || p.pack_w)) p.repacked = take(packed);
     // A piece of G and its transpose take 256 MB at most (and hold 1024 classes at least): as long as a piece's two products fill the chip and
     // sum over thousands of classes, larger pieces gain nothing.
     const long long per_class = 2ll * p.planes * 2 * round_up(N, 32);
@@ -409,70 +548,133 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
     vp = round_up((V + pieces - 1) / pieces, 256);                       // equal pieces
     p.vp = (int)(vp < V ? vp : V);
     p.wvp = packed_width(p.planes, p.vp);
-    p.size_g = tile_size(N, p.vp);
-    p.size_h = tile_size(N, D);
-    p.size_w = tile_size(p.vp, D);
-    p.shares_h = shares_of(N, D, p.size_h, p.wvp);
-    p.shares_w = shares_of(p.vp, D, p.size_w, p.wn);
-    p.weight = take(4ll * N);
+    const Job g{N, p.vp, stages_of(p.wd), false, false};
+    p.size_g = choose(p.planes, &g, 1).size;
+    Job both[2];
+    int jobs = 0;
+    if (need_h) both[jobs++] = Job{N, D, stages_of(p.wvp), false, true};
+    if (need_w) both[jobs++] = Job{p.vp, D, stages_of(p.wn), false, true};
+    if (jobs) {
+        const Choice c = choose(p.planes, both, jobs);
+        p.size_p = c.size;
+        p.limit = c.limit;
+    }
+    p.exponents = take(sizeof(Exponents));
+    p.largest = take(4);
     p.g = take(2 * p.wvp * N);
     p.gt = take(2 * p.wn * p.vp);
-    p.ldh_sum = round_up(D, 4);
+    p.ldc = round_up(D, 4);
     if (need_h) {
         p.wt = take(2 * p.wvp * D);
-        p.sum_h = take(4ll * p.shares_h * p.ldh_sum * N);
+        p.sum_h = take(4ll * shares_of(stages_of(p.wvp), p.limit) * p.ldc * N);
     }
     if (need_w) {
         p.ht = take(2 * p.wn * D);
-        if (p.shares_w > 1) p.sum_w = take(4ll * p.shares_w * p.ldh_sum * p.vp);
+        const int shares = shares_of(stages_of(p.wn), p.limit);
+        if (shares > 1) p.sum_w = take(4ll * shares * p.ldc * p.vp);
     }
     p.backward_bytes = at;
     return p;
 }
 
-static int blocks_for(long long work) { const long long b = (work + 255) / 256; return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b); }
+static int blocks_for(long long work) { const long long b = (work + 255) / 256; return (int)(b < 1 ? 1 : b > 4096 ? 4096 : b); }
 
-template <int PL, int EL, class T>
-static void pack_rows(const Source& s, u16* dst, long long ldd, hipStream_t stream) {
-    const int width = (int)(PL == TWO ? ldd / 2 : ldd);
-    UNFLOW_LAUNCH((pack_rows_kernel<T, PL, EL>), dim3(blocks_for((long long)s.rows * (width / 4))), dim3(256), 0, stream, s, dst, ldd, width);
-}
-template <int PL, int EL, class T>
-static void pack_columns(const Source& s, u16* dst, long long ldd, hipStream_t stream) {
-    const int width = (int)(PL == TWO ? ldd / 2 : ldd);
-    UNFLOW_LAUNCH((pack_columns_kernel<T, PL, EL>), dim3(ceil_div(width, 64), ceil_div(s.cols, 64)), dim3(256), 0, stream, s, dst, ldd, width);
-}
-static void pack_rows_of(int dtype, const Source& s, u16* dst, long long ldd, hipStream_t stream) {
-    if (dtype == kFp32) pack_rows<TWO, FP16, float>(s, dst, ldd, stream);
-    else if (dtype == kBf16) pack_rows<ONE, BF16, __bf16>(s, dst, ldd, stream);
-    else pack_rows<ONE, FP16, _Float16>(s, dst, ldd, stream);
-}
-static void pack_columns_of(int dtype, const Source& s, u16* dst, long long ldd, hipStream_t stream) {
-    if (dtype == kFp32) pack_columns<TWO, FP16, float>(s, dst, ldd, stream);
-    else if (dtype == kBf16) pack_columns<ONE, BF16, __bf16>(s, dst, ldd, stream);
-    else pack_columns<ONE, FP16, _Float16>(s, dst, ldd, stream);
+struct Inputs { const void* h; long long ldh; const void* w; long long ldw; const long long* target; long long ignore; int N, V, D; float scale; };
+
+static int pack_blocks(int rows) { return rows > 4 * kMaxima ? kMaxima : ceil_div(rows, 4); }
+
+// H and W as operands: as they are, or packed at `to`
+template <class T, int PL, int EL>
+static Logits operands(const Plan& p, const Inputs& in, char* to, bool pack, hipStream_t stream, Operand& H, Operand& W) {
+    H = p.pack_h ? Operand{(const u16*)(to + p.hp), p.wd, in.N} : Operand{(const u16*)in.h, in.ldh, in.N};
+    W = p.pack_w ? Operand{(const u16*)(to + p.wp), p.wd, in.V} : Operand{(const u16*)in.w, in.ldw, in.V};
+    const Packed at{(u16*)(to + p.hp), (u16*)(to + p.wp), (int*)(to + p.eh), (int*)(to + p.ew), (float*)(to + p.maxima)};
+    if (pack && (p.pack_h || p.pack_w)) {
+        const int blocks_h = p.pack_h ? pack_blocks(in.N) : 0, blocks_w = p.pack_w ? pack_blocks(in.V) : 0;
+        UNFLOW_LAUNCH((pack_inputs_kernel<T, PL, EL>), dim3(blocks_h + blocks_w), dim3(256), 0, stream, Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, Source{in.w, in.ldw, in.V, in.D}, blocks_h,
+                      at, p.wd, (int)(PL == TWO ? p.wd / 2 : p.wd));
+    }
+    return Logits{in.scale, at.eh, at.ew};
 }
 
-// H and W as operands (packed into the workspace where they are none by themselves), and the exponents they were packed with
-static void operands(const Plan& p, const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long ignore, int N, int V, int D, int dtype, char* ws, hipStream_t stream,
-                     Operand& H, Operand& W) {
-    Scalars* sc = (Scalars*)(ws + p.scalars);
-    const int *eh = nullptr, *ew = nullptr;
-    if (dtype == kFp32) {
-        UNFLOW_LAUNCH(largest_kernel, dim3(kMaxima, 2), dim3(256), 0, stream, Source{h, ldh, N, D, nullptr}, Source{w, ldw, V, D, nullptr}, target, ignore, (float*)(ws + p.maxima));
-        UNFLOW_LAUNCH(exponents_kernel, dim3(1), dim3(256), 0, stream, (const float*)(ws + p.maxima), sc);
-        eh = &sc->eh;
-        ew = &sc->ew;
+template <class T, int PL, int EL>
+static void forward(const Plan& p, const Inputs& in, int reduction, float* loss, char* kept, char* ws, hipStream_t stream) {
+    float* stats = (float*)(kept + p.stats);
+    float2* partial = (float2*)(ws + p.partial);
+    float* zt = (float*)(ws + p.ztarget);
+    float* losses = reduction == 0 ? loss : (float*)(ws + p.losses);
+    int columns;
+    if (p.few) {
+        columns = ceil_div(in.V, 64);
+        const T *h = (const T*)in.h, *w = (const T*)in.w;
+        if (in.N <= 16) UNFLOW_LAUNCH((lce_few_kernel<T, 1>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, in.scale, in.target, partial, zt);
+        else if (in.N <= 32) UNFLOW_LAUNCH((lce_few_kernel<T, 2>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, in.scale, in.target, partial, zt);
+        else UNFLOW_LAUNCH((lce_few_kernel<T, 4>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, in.scale, in.target, partial, zt);
+    } else {
+        Operand H, W;
+        const Logits how = operands<T, PL, EL>(p, in, kept, true, stream, H, W);
+        columns = ceil_div(in.V, kSizes[p.size_z]);
+        with_tile<PL, EL>(p.size_z, [&](auto tile) {
+            using TileT = decltype(tile);
+            LAUNCH_TILES((lce_forward_kernel<TileT>), (int)tiles_of(in.N, in.V, TileT::BM), H, W, (int)p.wd, how, in.target, partial, zt);
+        });
     }
-    H = Operand{(const u16*)h, ldh, N};
-    W = Operand{(const u16*)w, ldw, V};
-    if (p.pack_h) {
-        H = Operand{(const u16*)(ws + p.hp), p.wd, N};
-        pack_rows_of(dtype, Source{h, ldh, N, D, eh}, (u16*)(ws + p.hp), p.wd, stream);
-    }
-    if (p.pack_w) {
-        W = Operand{(const u16*)(ws + p.wp), p.wd, V};
-        pack_rows_of(dtype, Source{w, ldw, V, D, ew}, (u16*)(ws + p.wp), p.wd, stream);
+    // (a workgroup for 16 rows reads their pairs in whole lines; few rows over many columns need more of them)
+    if (in.N <= 256) UNFLOW_LAUNCH((lce_join_kernel<1>), dim3(in.N), dim3(256), 0, stream, (const float2*)partial, columns, in.N, in.V, in.target, in.ignore, (const float*)zt, (Row*)stats, losses);
+    else UNFLOW_LAUNCH((lce_join_kernel<16>), dim3(ceil_div(in.N, 16)), dim3(256), 0, stream, (const float2*)partial, columns, in.N, in.V, in.target, in.ignore, (const float*)zt, (Row*)stats, losses);
+    if (reduction != 0) UNFLOW_LAUNCH(lce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)losses, in.target, in.ignore, in.N, reduction == 1 ? 1 : 0, loss, stats + 4ll * in.N);
+}
+
+template <class T, int PL, int EL>
+static void backward(const Plan& p, const Inputs& in, int reduction, const float* gout, void* dh, void* dw, char* kept, char* ws, hipStream_t stream) {
+    const float* stats = (const float*)(kept + p.stats);
+    char* to = p.keeps ? kept : ws + p.repacked;
+    Operand H, W;
+    const Logits how = operands<T, PL, EL>(p, in, to, !p.keeps, stream, H, W);
+    Exponents* ex = (Exponents*)(ws + p.exponents);
+    const float* maxima = (const float*)(to + p.maxima);
+    const Upstream up{gout, (const float*)(ws + p.largest), stats + 4ll * in.N, in.target, in.ignore, reduction, in.scale};
+    if (reduction == 0) UNFLOW_LAUNCH(lce_largest_upstream_kernel, dim3(1), dim3(1024), 0, stream, up, in.N, (float*)(ws + p.largest));
+    u16 *G = (u16*)(ws + p.g), *GT = (u16*)(ws + p.gt);
+    const bool single = p.vp >= in.V;
+    for (int v0 = 0; v0 < in.V; v0 += p.vp) {
+        const int vp = in.V - v0 < p.vp ? in.V - v0 : p.vp;
+        const long long wvp = packed_width(PL, vp);
+        Columns wc{}, hc{};
+        int blocks_w = 0, blocks_h = 0;
+        if (dh) {
+            wc = Columns{Source{(const T*)in.w + (long long)v0 * in.ldw, in.ldw, vp, in.D}, (u16*)(ws + p.wt), wvp, (int)(PL == TWO ? wvp / 2 : wvp), maxima + kMaxima, pack_blocks(in.V)};
+            blocks_w = ceil_div(wc.width, 64) * ceil_div(in.D, 64);
+        }
+        if (dw && v0 == 0) {
+            hc = Columns{Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, (u16*)(ws + p.ht), p.wn, (int)(PL == TWO ? p.wn / 2 : p.wn), maxima, pack_blocks(in.N)};
+            blocks_h = ceil_div(hc.width, 64) * ceil_div(in.D, 64);
+        }
+        if (blocks_w + blocks_h) UNFLOW_LAUNCH((pack_transposes_kernel<T, PL, EL>), dim3(blocks_w + blocks_h), dim3(256), 0, stream, wc, hc, blocks_w, ex);
+        with_tile<PL, EL>(p.size_g, [&](auto tile) {
+            using TileT = decltype(tile);
+            LAUNCH_TILES((lce_gradient_kernel<TileT>), (int)tiles_of(in.N, vp, TileT::BM), H, W, (int)p.wd, how, (const Row*)stats, up, v0, vp, in.V, G, p.wvp, dw ? GT : nullptr, p.wn);
+        });
+        Product a{}, b{};
+        a.shares = b.shares = 1;
+        if (dh) {
+            a = Product{Operand{G, p.wvp, in.N}, Operand{(const u16*)(ws + p.wt), wvp, in.D}, (int)wvp, shares_of(stages_of(p.wvp), p.limit), 0, (float*)(ws + p.sum_h), p.ldc, v0 == 0 ? 1 : 0, dh, 0};
+            if (single && a.shares == 1) a.sums = nullptr;
+        }
+        if (dw) {
+            b = Product{Operand{GT, p.wn, vp}, Operand{(const u16*)(ws + p.ht), p.wn, in.D}, (int)p.wn, shares_of(stages_of(p.wn), p.limit), 0, (float*)(ws + p.sum_w), p.ldc, 1, (T*)dw + (long long)v0 * in.D, 1};
+            if (b.shares == 1) b.sums = nullptr;
+        }
+        with_tile<PL, EL>(p.size_p, [&](auto tile) {
+            using TileT = decltype(tile);
+            if (dh) a.tiles = (int)tiles_of(in.N, in.D, TileT::BM);
+            if (dw) b.tiles = (int)tiles_of(vp, in.D, TileT::BM);
+            const bool swap = dw && (!dh || b.width / b.shares > a.width / a.shares);        // the longer units first
+            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, swap ? b : a, swap ? a : b, (const Exponents*)ex, up);
+        });
+        const bool last = v0 + vp >= in.V;
+        const int finish_a = dh && last && a.sums ? blocks_for((long long)in.N * (p.ldc / 4)) : 0, finish_b = dw && b.sums ? blocks_for((long long)vp * (p.ldc / 4)) : 0;
+        if (finish_a + finish_b) UNFLOW_LAUNCH((lce_finish_kernel<T, PL, EL>), dim3(finish_a + finish_b), dim3(256), 0, stream, a, b, finish_a, (const Exponents*)ex, up);
     }
 }
 
@@ -483,93 +685,38 @@ static bool sizes_ok(long long ldh, long long ldw, int N, int V, int D, int dtyp
 
 }  // namespace
 
-extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_h, int need_w,
-                                          long long* forward_bytes, long long* backward_bytes) {
-    UNFLOW_REQUIRE(forward_bytes && backward_bytes && sizes_ok(ldh, ldw, N, V, D, dtype, 0));
-    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, need_h != 0, need_w != 0);
+extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_dhidden, int need_dweight,
+                                          long long* kept_bytes, long long* forward_bytes, long long* backward_bytes) {
+    UNFLOW_REQUIRE(kept_bytes && forward_bytes && backward_bytes && sizes_ok(ldh, ldw, N, V, D, dtype, 0));
+    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, need_dhidden || need_dweight, need_dhidden != 0, need_dweight != 0);
+    *kept_bytes = p.kept_bytes;
     *forward_bytes = p.forward_bytes;
     *backward_bytes = p.backward_bytes;
     return 0;
 }
 
 extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V, int D, int dtype, float scale,
-                                    long long ignore_index, int reduction, float* loss, float* lse, void* workspace, long long workspace_bytes, void* stream_) {
-    UNFLOW_REQUIRE(hidden && weight && target && loss && lse && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
-    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, false, false);
+                                    long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes, void* stream) {
+    UNFLOW_REQUIRE(hidden && weight && target && loss && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
+    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, false, false, false);
     UNFLOW_REQUIRE(workspace_bytes >= p.forward_bytes);
-    hipStream_t stream = (hipStream_t)stream_;
-    char* ws = (char*)workspace;
-    Operand H, W;
-    operands(p, hidden, ldh, weight, ldw, target, ignore_index, N, V, D, dtype, ws, stream, H, W);
-    const Scalars* sc = (const Scalars*)(ws + p.scalars);
-    const int width = (int)(p.planes == TWO ? p.wd : D + (8 - D % 8) % 8);
-    const int count = tiles(N, V, p.size_z);
-    float2* partial = (float2*)(ws + p.partial);
-    float* zt = (float*)(ws + p.ztarget);
-    WITH_TILE(p.planes, p.el, p.size_z, LAUNCH_TILES((lce_forward_kernel<TileT>), count, H, W, width, sc, scale, target, partial, zt));
-    float* losses = reduction == 0 ? loss : (float*)(ws + p.losses);
-    UNFLOW_LAUNCH(lce_join_kernel, dim3(ceil_div(N, 16)), dim3(256), 0, stream, (const float2*)partial, ceil_div(V, p.size_z), N, V, target, ignore_index, (const float*)zt, lse, losses);
-    if (reduction != 0) UNFLOW_LAUNCH(lce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)losses, target, ignore_index, N, reduction == 1 ? 1 : 0, loss);
+    const Inputs in{hidden, ldh, weight, ldw, target, ignore_index, N, V, D, scale};
+    char *k = (char*)kept, *ws = (char*)workspace;
+    if (dtype == kFp32) forward<float, TWO, FP16>(p, in, reduction, loss, k, ws, (hipStream_t)stream);
+    else if (dtype == kBf16) forward<__bf16, ONE, BF16>(p, in, reduction, loss, k, ws, (hipStream_t)stream);
+    else forward<_Float16, ONE, FP16>(p, in, reduction, loss, k, ws, (hipStream_t)stream);
     return unflow_launch_status();
 }
 
-extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* lse, const float* gout, int N, int V, int D,
-                                    int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, void* workspace, long long workspace_bytes, void* stream_) {
-    UNFLOW_REQUIRE(hidden && weight && target && lse && gout && (dhidden || dweight) && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
-    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, dhidden != nullptr, dweight != nullptr);
+extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* gout, int N, int V, int D,
+                                    int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept, void* workspace, long long workspace_bytes, void* stream) {
+    UNFLOW_REQUIRE(hidden && weight && target && gout && (dhidden || dweight) && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
+    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, true, dhidden != nullptr, dweight != nullptr);
     UNFLOW_REQUIRE(workspace_bytes >= p.backward_bytes);
-    hipStream_t stream = (hipStream_t)stream_;
-    char* ws = (char*)workspace;
-    Operand H, W;
-    operands(p, hidden, ldh, weight, ldw, target, ignore_index, N, V, D, dtype, ws, stream, H, W);
-    Scalars* sc = (Scalars*)(ws + p.scalars);
-    const int width = (int)(p.planes == TWO ? p.wd : D + (8 - D % 8) % 8);
-    const int unit = p.el == FP16 ? probability_exponent<FP16>() : probability_exponent<BF16>();
-    const long long esize = dtype == kFp32 ? 4 : 2;
-    float* rows = (float*)(ws + p.weight);
-    UNFLOW_LAUNCH(lce_weights_kernel, dim3(1), dim3(1024), 0, stream, gout, reduction, scale, target, ignore_index, N, dtype == kFp32 ? 1 : 0, sc, rows);
-    const int* eh = dtype == kFp32 ? &sc->eh : nullptr;
-    const int* ew = dtype == kFp32 ? &sc->ew : nullptr;
-    u16 *G = (u16*)(ws + p.g), *GT = (u16*)(ws + p.gt);
-    const Operand HT{(const u16*)(ws + p.ht), p.wn, D};
-    if (dweight) pack_columns_of(dtype, Source{hidden, ldh, N, D, eh, target, ignore_index}, (u16*)(ws + p.ht), p.wn, stream);
-    for (int v0 = 0; v0 < V; v0 += p.vp) {
-        const int vp = V - v0 < p.vp ? V - v0 : p.vp;
-        const long long wvp = packed_width(p.planes, vp);
-        const int count_g = tiles(N, vp, p.size_g);
-        WITH_TILE(p.planes, p.el, p.size_g, LAUNCH_TILES((lce_gradient_kernel<TileT>), count_g, H, W, width, (const Scalars*)sc, scale, target, lse, (const float*)rows, ignore_index, v0, vp, V, G, p.wvp, GT, p.wn));
-        if (dhidden) {
-            pack_columns_of(dtype, Source{(const char*)weight + v0 * ldw * esize, ldw, vp, D, ew}, (u16*)(ws + p.wt), wvp, stream);
-            const Operand A{G, p.wvp, N}, B{(const u16*)(ws + p.wt), wvp, D};
-            float* sums = (float*)(ws + p.sum_h);
-            const int count = tiles(N, D, p.size_h) * p.shares_h;
-            WITH_TILE(p.planes, p.el, p.size_h, LAUNCH_TILES((gather_product_kernel<TileT>), count, A, B, (int)wvp, p.shares_h, sums, p.ldh_sum, v0 == 0 ? 1 : 0));
-        }
-        if (dweight) {
-            const Operand A{GT, p.wn, vp};
-            char* out = (char*)dweight + (long long)v0 * D * esize;
-            if (p.shares_w > 1) {
-                float* sums = (float*)(ws + p.sum_w);
-                const int count = tiles(vp, D, p.size_w) * p.shares_w;
-                WITH_TILE(p.planes, p.el, p.size_w, LAUNCH_TILES((gather_product_kernel<TileT>), count, A, HT, (int)p.wn, p.shares_w, sums, p.ldh_sum, 1));
-                const int blocks = blocks_for((long long)vp * (p.ldh_sum / 4));
-                if (dtype == kFp32) UNFLOW_LAUNCH((finish_kernel<float>), dim3(blocks), dim3(256), 0, stream, (const float*)sums, p.ldh_sum, p.shares_w, vp, D, (const Scalars*)sc, 1, unit, (const float*)nullptr, (float*)out, (long long)D);
-                else if (dtype == kBf16) UNFLOW_LAUNCH((finish_kernel<__bf16>), dim3(blocks), dim3(256), 0, stream, (const float*)sums, p.ldh_sum, p.shares_w, vp, D, (const Scalars*)sc, 1, unit, (const float*)nullptr, (__bf16*)out, (long long)D);
-                else UNFLOW_LAUNCH((finish_kernel<_Float16>), dim3(blocks), dim3(256), 0, stream, (const float*)sums, p.ldh_sum, p.shares_w, vp, D, (const Scalars*)sc, 1, unit, (const float*)nullptr, (_Float16*)out, (long long)D);
-            } else {
-                const int count = tiles(vp, D, p.size_w);
-                if (p.planes == TWO) WITH_TILE(TWO, FP16, p.size_w, LAUNCH_TILES((weight_product_kernel<TileT, float>), count, A, HT, (int)p.wn, (const Scalars*)sc, (float*)out, (long long)D));
-                else if (p.el == FP16) WITH_TILE(ONE, FP16, p.size_w, LAUNCH_TILES((weight_product_kernel<TileT, _Float16>), count, A, HT, (int)p.wn, (const Scalars*)sc, (_Float16*)out, (long long)D));
-                else WITH_TILE(ONE, BF16, p.size_w, LAUNCH_TILES((weight_product_kernel<TileT, __bf16>), count, A, HT, (int)p.wn, (const Scalars*)sc, (__bf16*)out, (long long)D));
-            }
-        }
-    }
-    if (dhidden) {
-        const float* sums = (const float*)(ws + p.sum_h);
-        const int blocks = blocks_for((long long)N * (p.ldh_sum / 4));
-        if (dtype == kFp32) UNFLOW_LAUNCH((finish_kernel<float>), dim3(blocks), dim3(256), 0, stream, sums, p.ldh_sum, p.shares_h, N, D, (const Scalars*)sc, 0, unit, (const float*)rows, (float*)dhidden, (long long)D);
-        else if (dtype == kBf16) UNFLOW_LAUNCH((finish_kernel<__bf16>), dim3(blocks), dim3(256), 0, stream, sums, p.ldh_sum, p.shares_h, N, D, (const Scalars*)sc, 0, unit, (const float*)rows, (__bf16*)dhidden, (long long)D);
-        else UNFLOW_LAUNCH((finish_kernel<_Float16>), dim3(blocks), dim3(256), 0, stream, sums, p.ldh_sum, p.shares_h, N, D, (const Scalars*)sc, 0, unit, (const float*)rows, (_Float16*)dhidden, (long long)D);
-    }
+    const Inputs in{hidden, ldh, weight, ldw, target, ignore_index, N, V, D, scale};
+    char *k = (char*)const_cast<void*>(kept), *ws = (char*)workspace;
+    if (dtype == kFp32) backward<float, TWO, FP16>(p, in, reduction, gout, dhidden, dweight, k, ws, (hipStream_t)stream);
+    else if (dtype == kBf16) backward<__bf16, ONE, BF16>(p, in, reduction, gout, dhidden, dweight, k, ws, (hipStream_t)stream);
+    else backward<_Float16, ONE, FP16>(p, in, reduction, gout, dhidden, dweight, k, ws, (hipStream_t)stream);
     return unflow_launch_status();
 }

@@ -94,7 +94,8 @@ struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PL = PL_, EL = EL_;
     static constexpr int WAVES = WM * WN, THREADS = WAVES * 64, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
     static constexpr int STAGE = (BM + BN) * kStageBytes;
-    static constexpr int LDS = 2 * STAGE;
+    static constexpr int PITCH = BM + 8;                                      // of a row of the transposed tile (store_transposed)
+    static constexpr int LDS = 2 * STAGE > BN * PITCH * 2 ? 2 * STAGE : BN * PITCH * 2;
     static constexpr int QA = BM / 8 / WAVES, QB = BN / 8 / WAVES;            // 1 KB copies (8 rows) of a wave per stage
     static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0, "a wave copies whole groups of 8 rows");
 
@@ -193,6 +194,36 @@ struct Tile {
         }
         UNFLOW_WAIT_VMCNT0();
         __syncthreads();
+    }
+
+    // The transpose of the tile, value(i, j) being the four numbers that belong to acc[i][j], into packed rows: dst row n holds the numbers of
+    // column n at k = m.  A lane's four numbers lie in four dst rows; through LDS (half of m at a time for TWO planes) the rows leave in 16-byte
+    // pieces.  `width`: elements of a dst row; LDS is free when this is called and not when it returns.
+    template <class F>
+    __device__ __forceinline__ void store_transposed(char* lds, u16* __restrict__ dst, long long ld, int rows, long long width, int m0, int n0, F&& value) {
+        static_assert(WM == 2, "the halves of m are the wave rows");
+        constexpr int R = BM / PL;
+        u16* s = reinterpret_cast<u16*>(lds);
+#pragma unroll
+        for (int pass = 0; pass < PL; ++pass) {
+            if (PL == 1 || wave() / WN == pass) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) {
+                        const f32x4 v = value(i, j);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) pack1<PL, EL>(s + (col(j) + r) * PITCH, row(i) - pass * R, v[r]);
+                    }
+            }
+            __syncthreads();
+            const long long first = packed_at(PL, m0 + pass * R);
+            for (int c = (int)threadIdx.x; c < BN * BM / 8; c += THREADS) {
+                const int n = c / (BM / 8), e = c % (BM / 8) * 8;
+                if (n0 + n < rows && first + e < width) *reinterpret_cast<uint4*>(dst + (long long)(n0 + n) * ld + first + e) = *reinterpret_cast<const uint4*>(s + n * PITCH + e);
+            }
+            if (pass + 1 < PL) __syncthreads();
+        }
     }
 };
 

@@ -14,13 +14,14 @@
 // the planes are scaled by.  A matrix whose norm is far below eps comes out as nearly zero, as the definition has it, but without relative
 // accuracy.
 #include "pack.h"
+#include "plan.h"
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
 namespace {
 
 constexpr int kFp32 = 0, kBf16 = 1, kFp16 = 2;                     // UNFLOW_DTYPE_*
-constexpr int kChunk = 16384;                                      // numbers a workgroup of the norm takes
 
 struct Problem {
     const void* x;               // gradient / input
@@ -37,6 +38,8 @@ static_assert(sizeof(Problem) % 4 == 0, "copied by words");
 
 // running counts of the work items of all problems, one row per phase
 enum { kNorm, kPack, kSquare, kJoin, kPoly, kApply, kPhases };
+// behind them, for the three product phases: first and last + 1 work item of the matrices of the same length
+enum { kSquareClass = kPhases, kPolyClass = kSquareClass + 2, kApplyClass = kPolyClass + 2, kTables = kApplyClass + 2 };
 
 struct Exponents { int x, s, q; };                                 // planes hold X 2^x, S 2^s, Q 2^q
 
@@ -47,32 +50,47 @@ __global__ __launch_bounds__(256) void write_table_kernel(Words src, int count, 
     for (int i = threadIdx.x; i < count; i += 256) dst[i] = src.w[i];
 }
 
-// the problem that work item `id` of a phase belongs to, and the item's number within it
-__device__ __forceinline__ int problem_of(const int* __restrict__ ends, int count, int id, int& local) {
-    const int lane = (int)threadIdx.x & 63;
+// the problem that work item `id` of a phase belongs to, and the item's number within it; e: this lane's running count if one load holds them all
+__device__ __forceinline__ int count_before(const int* __restrict__ ends, int count, int e, int id) {
+    if (count <= 64) return __popcll(__ballot(e <= id));
     int at = 0;
     for (int base = 0; base < count; base += 64) {
-        const int e = base + lane < count ? ends[base + lane] : 0x7fffffff;
-        const int before = __popcll(__ballot(e <= id));
+        const int lane = base + ((int)threadIdx.x & 63), before = __popcll(__ballot((lane < count ? ends[lane] : 0x7fffffff) <= id));
         at += before;
         if (before < 64) break;
     }
-    at = __builtin_amdgcn_readfirstlane(at);
+    return at;
+}
+__device__ __forceinline__ int lane_end(const int* __restrict__ ends, int count) {
+    const int lane = (int)threadIdx.x & 63;
+    return lane < count ? ends[lane] : 0x7fffffff;
+}
+__device__ __forceinline__ int problem_of(const int* __restrict__ ends, int count, int id, int& local) {
+    const int at = __builtin_amdgcn_readfirstlane(count_before(ends, count, lane_end(ends, count), id));
     local = id - (at > 0 ? ends[at - 1] : 0);
     return at;
+}
+// The same for the product phases.  Work items are sorted by length, the longest first; the matrices of one length are dealt over the XCDs by
+// themselves, so that every XCD has its share of the long ones and a matrix stays in one L2 as far as it goes.
+__device__ __forceinline__ int dealt_problem_of(const int* __restrict__ ends, int count, const int* __restrict__ classes, int& local) {
+    const int e = lane_end(ends, count), at = __builtin_amdgcn_readfirstlane(count_before(ends, count, e, (int)blockIdx.x));
+    const int first = classes[2 * at], end = classes[2 * at + 1], id = first + xcd_remap((int)blockIdx.x - first, end - first);
+    const int mine = __builtin_amdgcn_readfirstlane(count_before(ends, count, e, id));
+    local = id - (mine > 0 ? ends[mine - 1] : 0);
+    return mine;
 }
 
 __device__ __forceinline__ float direction(float g, float m, float mu, int nesterov) { return nesterov ? g + mu * (m - g) : m; }
 
-// ---- sum of squares of a chunk (after the momentum's update)
+// ---- sum of squares of a chunk of `size` numbers (after the momentum's update)
 template <class T, bool STEP>
-__global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, float mu, int nesterov, double* __restrict__ parts) {
+__global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size, float mu, int nesterov, double* __restrict__ parts) {
     int chunk;
     const Problem p = table[problem_of(ends, count, (int)blockIdx.x, chunk)];
-    const long long total = (long long)p.rows * p.cols, e0 = (long long)chunk * kChunk;
+    const long long total = (long long)p.rows * p.cols, e0 = (long long)chunk * size;
     const T* x = (const T*)p.x;
     double sum = 0.;
-    for (int k = 0; k < kChunk / 1024; ++k) {
+    for (int k = 0; k < size / 1024; ++k) {
         const long long e = e0 + k * 1024 + threadIdx.x * 4;
         const long long left = total - e;
         if (left <= 0) break;
@@ -171,22 +189,26 @@ __device__ __forceinline__ void triangle_of(int id, int& tm, int& tn) {
     tn = id - tm * (tm + 1) / 2;
 }
 
-// four numbers of a row of a symmetric matrix [m][packed m], and (off the diagonal tiles) their mirror
-__device__ __forceinline__ void symmetric_store(u16* p, long long ld, int m, int wide, int row, int col, f32x4 v, bool mirror) {
-    if (row < m && col < wide) pack4<TWO, FP16>(p + row * ld, col, v);
-    if (mirror && row < wide) {
+// a tile of a symmetric matrix [m][packed m], value(i, j) being its numbers, and (off the diagonal) its mirror
+template <class TileT, class F>
+__device__ __forceinline__ void symmetric_store(TileT& T, char* lds, u16* __restrict__ p, long long ld, int m, int tm, int tn, F&& value) {
+    const int wide = (int)(ld / 2);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (col + r < m) pack1<TWO, FP16>(p + (col + r) * ld, row, v[r]);
-    }
+    for (int i = 0; i < TileT::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < TileT::NI; ++j) {
+            const int row = tm * TileT::BM + TileT::row(i), col = tn * TileT::BN + TileT::col(j);
+            if (row < m && col < wide) pack4<TWO, FP16>(p + row * ld, col, value(i, j));
+        }
+    if (tm != tn) T.store_transposed(lds, p, ld, m, ld, tm * TileT::BM, tn * TileT::BN, value);
 }
 
-// ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves its accumulators for join_kernel
+// ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves fp32 tiles for join_kernel
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, Exponents ex, char* __restrict__ ws) {
+__global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const int* __restrict__ classes, Exponents ex, char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
-    const Problem p = table[problem_of(ends, count, xcd_remap((int)blockIdx.x, (int)gridDim.x), id)];
+    const Problem p = table[dealt_problem_of(ends, count, classes, id)];
     triangle_of(id / p.shares, tm, tn);
     const int share = id % p.shares;
     const long long ld = packed_width(TWO, p.n), lds_ = packed_width(TWO, p.m);
@@ -196,48 +218,64 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
     TileT T;
     T.run(X, X, k0, k1, tm * TileT::BM, tn * TileT::BN, lds);
     if (p.shares > 1) {
-        f32x4* to = (f32x4*)(ws + p.shares_at) + (long long)id * (TileT::MI * TileT::NI * TileT::THREADS) + threadIdx.x;
+        float* to = (float*)(ws + p.shares_at) + (long long)id * (TileT::BM * TileT::BN);
 #pragma unroll
         for (int i = 0; i < TileT::MI; ++i)
 #pragma unroll
-            for (int j = 0; j < TileT::NI; ++j) to[(i * TileT::NI + j) * TileT::THREADS] = T.acc[i][j];
+            for (int j = 0; j < TileT::NI; ++j) *reinterpret_cast<f32x4*>(to + TileT::row(i) * TileT::BN + TileT::col(j)) = T.acc[i][j];
         return;
     }
     const float f = ldexpf(1.f, ex.s - 2 * ex.x);
-    const int wide = (int)(lds_ / 2);
-#pragma unroll
-    for (int i = 0; i < TileT::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < TileT::NI; ++j)
-            symmetric_store((u16*)(ws + p.S), lds_, p.m, wide, tm * TileT::BM + TileT::row(i), tn * TileT::BN + TileT::col(j), T.acc[i][j] * f, tm != tn);
+    symmetric_store(T, lds, (u16*)(ws + p.S), lds_, p.m, tm, tn, [&](int i, int j) { return T.acc[i][j] * f; });
 }
-template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS) void join_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, Exponents ex, char* __restrict__ ws) {
-    constexpr int EACH = TileT::MI * TileT::NI * TileT::THREADS;
+// (64 x 64 of a tile of side `size` per workgroup)
+__global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size, Exponents ex, char* __restrict__ ws) {
+    __shared__ float tile[64][65];
     int id, tm, tn;
     const Problem p = table[problem_of(ends, count, (int)blockIdx.x, id)];
-    triangle_of(id, tm, tn);
-    const f32x4* from = (const f32x4*)(ws + p.shares_at) + (long long)id * p.shares * EACH + threadIdx.x;
+    const int side = size / 64, part = id % (side * side), at = id / (side * side);
+    triangle_of(at, tm, tn);
+    const int r0 = part / side * 64, c0 = part % side * 64, row0 = tm * size + r0, col0 = tn * size + c0;
+    const long long each = (long long)size * size, ld = packed_width(TWO, p.m);
+    const float* from = (const float*)(ws + p.shares_at) + at * p.shares * each + r0 * size + c0;
+    u16* S = (u16*)(ws + p.S);
     const float f = ldexpf(1.f, ex.s - 2 * ex.x);
-    const long long lds_ = packed_width(TWO, p.m);
-    const int wide = (int)(lds_ / 2);
+    const int x = (threadIdx.x & 15) * 4, y = threadIdx.x >> 4, wide = (int)(ld / 2);
+    f32x4 v[4];
 #pragma unroll
-    for (int i = 0; i < TileT::MI; ++i)
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4*>(from + (y + 16 * i) * size + x);
+    for (int s = 1; s < p.shares; ++s)
 #pragma unroll
-        for (int j = 0; j < TileT::NI; ++j) {
-            f32x4 v = from[(i * TileT::NI + j) * TileT::THREADS];
-            for (int s = 1; s < p.shares; ++s) v += from[(long long)s * EACH + (i * TileT::NI + j) * TileT::THREADS];
-            symmetric_store((u16*)(ws + p.S), lds_, p.m, wide, tm * TileT::BM + TileT::row(i), tn * TileT::BN + TileT::col(j), v * f, tm != tn);
+        for (int i = 0; i < 4; ++i) v[i] += *reinterpret_cast<const f32x4*>(from + s * each + (y + 16 * i) * size + x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] *= f;
+        const int row = row0 + y + 16 * i, col = col0 + x;
+        if (row < p.m && col < wide) pack4<TWO, FP16>(S + row * ld, col, v[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tile[y + 16 * i][x + k] = v[i][k];
+    }
+    __syncthreads();
+    if (tm == tn) return;                                            // (a tile on the diagonal holds its own mirror)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = col0 + y + 16 * i, col = row0 + x;
+        if (row < p.m && col < wide) {
+            f32x4 u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) u[k] = tile[x + k][y + 16 * i];
+            pack4<TWO, FP16>(S + row * ld, col, u);
         }
+    }
 }
 
 // ---- Q = a I + b S + c S S: lower tiles
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, float a, float b, float c, Exponents ex,
+__global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const int* __restrict__ classes, float a, float b, float c, Exponents ex,
                                                                                              char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
-    const Problem p = table[problem_of(ends, count, xcd_remap((int)blockIdx.x, (int)gridDim.x), id)];
+    const Problem p = table[dealt_problem_of(ends, count, classes, id)];
     triangle_of(id, tm, tn);
     const long long ld = packed_width(TWO, p.m);
     const u16* s = (const u16*)(ws + p.S);
@@ -251,31 +289,29 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j) {
             const int row = tm * TileT::BM + TileT::row(i), col = tn * TileT::BN + TileT::col(j);
-            f32x4 v{0.f, 0.f, 0.f, 0.f};
-            if (row < p.m && col < wide) {
-                v = unpack4<TWO, FP16>(s + row * ld, col);
+            if (row >= p.m || col >= wide) continue;                   // (what is not there is zero already)
+            const f32x4 v = unpack4<TWO, FP16>(s + row * ld, col);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = fmaf(fc, T.acc[i][j][r], fb * v[r]) + (row == col + r ? fa : 0.f);
-            }
-            symmetric_store((u16*)(ws + p.Q), ld, p.m, wide, row, col, v, tm != tn);
+            for (int r = 0; r < 4; ++r) T.acc[i][j][r] = fmaf(fc, T.acc[i][j][r], fb * v[r]) + (row == col + r ? fa : 0.f);
         }
+    symmetric_store(T, lds, (u16*)(ws + p.Q), ld, p.m, tm, tn, [&](int i, int j) { return T.acc[i][j]; });
 }
 
 // ---- X <- Q X.  LAST: the output, or the parameter's update
 struct Update { float keep, lr; };                                   // 1 - lr wd, lr
 template <class TileT, bool LAST, bool STEP, class T>
-__global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int odd, Exponents ex, Update up,
+__global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const int* __restrict__ classes, int odd, Exponents ex, Update up,
                                                                                               char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
-    const Problem p = table[problem_of(ends, count, xcd_remap((int)blockIdx.x, (int)gridDim.x), id)];
+    const Problem p = table[dealt_problem_of(ends, count, classes, id)];
     tile_of(id, ceil_div(p.m, TileT::BM), ceil_div(p.n, TileT::BN), tm, tn);
     const long long ldm = packed_width(TWO, p.m), ldn = packed_width(TWO, p.n);
     const Operand Q{(const u16*)(ws + p.Q), ldm, p.m}, XT{(const u16*)(ws + (odd ? p.XT1 : p.XT0)), ldm, p.n};
     TileT T_;
     T_.run(Q, XT, 0, (int)ldm, tm * TileT::BM, tn * TileT::BN, lds);
     const float f = ldexpf(1.f, LAST ? -(ex.q + ex.x) : -ex.q);
-    const int wide_m = (int)(ldm / 2), wide_n = (int)(ldn / 2);
+    const int wide_n = (int)(ldn / 2);
     u16 *X = (u16*)(ws + p.X), *next = (u16*)(ws + (odd ? p.XT0 : p.XT1));
     const bool tall = p.rows > p.cols;
     const float lr = up.lr * p.boost;
@@ -284,7 +320,7 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j) {
             const int row = tm * TileT::BM + TileT::row(i), col = tn * TileT::BN + TileT::col(j);
-            f32x4 v = T_.acc[i][j] * f;
+            f32x4 v = T_.acc[i][j] *= f;
             if constexpr (LAST) {
                 if (row >= p.m || col >= p.n) continue;
                 const int n = p.n - col < 4 ? p.n - col : 4;
@@ -302,35 +338,18 @@ __global__ __launch_bounds__(TileT::THREADS, TileT::THREADS == 512 ? 2 : 1) void
                             *o = (T)(STEP ? (float)*o * up.keep - v[r] * lr : v[r]);
                         }
                 }
-            } else {
-                if (row < p.m && col < wide_n) pack4<TWO, FP16>(X + row * ldn, col, v);
-                if (row < wide_m) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (col + r < p.n) pack1<TWO, FP16>(next + (col + r) * ldm, row, v[r]);
-                }
-            }
+            } else if (row < p.m && col < wide_n) pack4<TWO, FP16>(X + row * ldn, col, v);
         }
+    __builtin_amdgcn_sched_barrier(0);                                // (the addresses of both stores at once do not fit the registers)
+    if constexpr (!LAST) T_.store_transposed(lds, next, ldm, p.n, ldm, tm * TileT::BM, tn * TileT::BN, [&](int i, int j) { return T_.acc[i][j]; });
 }
 
 // ---- the host side
-using T256t = Tile<256, 256, 2, 4, TWO, FP16>;
-using T128t = Tile<128, 128, 2, 2, TWO, FP16>;
-using T64t = Tile<64, 64, 2, 2, TWO, FP16>;
-
-static const int kSizes[3] = {256, 128, 64};
-
-// One tile size per phase and call: the one with the least time of a model in which the chip's 256 CUs take a tile each, a tile of size t costs
-// t^2 / e(t) for every k, and the phase lasts as long as one tile at least.  e: what part of the 256-tile's rate the smaller ones reach.
-static int best_size(const long long counts[3]) {
-    const double cost[3] = {65536., 16384. / 0.75, 4096. / 0.45};
-    int best = 0;
-    double least = 0.;
-    for (int i = 0; i < 3; ++i) {
-        const double t = cost[i] * (counts[i] > 256 ? counts[i] / 256. : 1.);
-        if (i == 0 || t < least) { best = i; least = t; }
-    }
-    return best;
+template <class F> static void with_tile(int size, F&& f) {
+    if (size == 0) f(Tile<256, 256, 2, 4, TWO, FP16>{});
+    else if (size == 1) f(Tile<192, 192, 2, 4, TWO, FP16>{});
+    else if (size == 2) f(Tile<128, 128, 2, 2, TWO, FP16>{});
+    else f(Tile<64, 64, 2, 2, TWO, FP16>{});
 }
 
 // Bounds of |X|, |S|, |Q| (spectral norms: every singular value of X_0 is in [0, 1]) over all steps, as powers of two that keep the planes
@@ -358,7 +377,8 @@ constexpr long long kGroupBytes = 4ll << 30;                         // matrices
 
 struct Group {
     int first, count;
-    int size_s, size_x;                                              // indices into kSizes
+    int size_s, size_q, size_x;                                      // indices into kSizes
+    int chunk;                                                       // numbers a workgroup of the norm takes: few of a small list, so that it fills the chip
     int total[kPhases];
     long long table, ends, parts, bytes;
 };
@@ -366,64 +386,105 @@ struct Group {
 static long long plane_bytes(long long m, long long n) {
     return round_up(2 * packed_width(TWO, n) * m, 256) + 2 * round_up(2 * packed_width(TWO, m) * n, 256) + 2 * round_up(2 * packed_width(TWO, m) * m, 256);
 }
-static long long lower(long long m, int size) { const long long t = (m + size - 1) / size; return t * (t + 1) / 2; }
-static long long full(long long m, long long n, int size) { return ((m + size - 1) / size) * ((n + size - 1) / size); }
 
-// lays out matrices [first, first + count): problems and running counts on the host, offsets into the workspace
+constexpr int kMost = 1024;                                          // matrices of one group
+
+// the matrices [first, first + count) of a list, sorted by the longer side and then the shorter one, the largest first
+struct Sorted {
+    int at[kMost];
+    int m[kMost], n[kMost];
+};
+static void sort_of(const unflow_matrix* a, int first, int count, Sorted& s) {
+    for (int i = 0; i < count; ++i) s.at[i] = first + i;
+    auto side = [&](int i, bool longer) { return (a[i].rows < a[i].cols) == longer ? a[i].cols : a[i].rows; };
+    std::stable_sort(s.at, s.at + count, [&](int x, int y) {
+        const int nx = side(x, true), ny = side(y, true);
+        return nx != ny ? nx > ny : side(x, false) > side(y, false);
+    });
+    for (int i = 0; i < count; ++i) {
+        s.m[i] = side(s.at[i], false);
+        s.n[i] = side(s.at[i], true);
+    }
+}
+
+// lays out a group: problems and running counts on the host, offsets into the workspace
 static Group lay_out(const unflow_matrix* a, int first, int count, Problem* problems, int* ends) {
+    static thread_local Sorted order;
+    static thread_local Job jobs[kMost];
+    sort_of(a, first, count, order);
     Group g{};
     g.first = first;
     g.count = count;
-    long long at = 0;
+    long long at = 0, chunks = 0;
     auto take = [&](long long bytes) { const long long p = at; at += round_up(bytes, 256); return p; };
     g.table = take((long long)sizeof(Problem) * count);
-    g.ends = take(4ll * kPhases * count);
-    long long cs[3] = {}, cx[3] = {}, chunks = 0;
-    for (int i = 0; i < count; ++i) {
-        const long long r = a[first + i].rows, c = a[first + i].cols, m = r < c ? r : c, n = r < c ? c : r;
-        for (int k = 0; k < 3; ++k) { cs[k] += lower(m, kSizes[k]); cx[k] += full(m, n, kSizes[k]); }
-        chunks += (r * c + kChunk - 1) / kChunk;
-    }
-    g.size_s = best_size(cs);
-    g.size_x = best_size(cx);
+    g.ends = take(4ll * kTables * count);
+    // matrices of one shape are one job of the model
+    auto plan = [&](auto job_of) {
+        int k = 0;
+        for (int i = 0; i < count;) {
+            int e = i + 1;
+            while (e < count && order.m[e] == order.m[i] && order.n[e] == order.n[i]) ++e;
+            jobs[k] = job_of(order.m[i], order.n[i]);
+            jobs[k++].times = e - i;
+            i = e;
+        }
+        return choose(TWO, jobs, k);
+    };
+    const Choice cs = plan([](long long m, long long n) { return Job{m, m, stages_of(packed_width(TWO, n)), true, true}; });
+    g.size_s = cs.size;
+    g.size_q = plan([](long long m, long long n) { return Job{m, m, stages_of(packed_width(TWO, m)), true, false}; }).size;
+    g.size_x = plan([](long long m, long long n) { return Job{m, n, stages_of(packed_width(TWO, m)), false, false}; }).size;
+    long long numbers = 0;
+    for (int i = 0; i < count; ++i) numbers += (long long)order.m[i] * order.n[i];
+    g.chunk = numbers < (16 << 20) ? 4096 : 16384;
+    for (int i = 0; i < count; ++i) chunks += ((long long)order.m[i] * order.n[i] + g.chunk - 1) / g.chunk;
     g.parts = take(8 * chunks);
-    const int size = kSizes[g.size_s];
-    // S sums over the long side; where its tiles do not fill the chip the sum is cut into shares of at least 4 stages
-    const long long want = 256 / cs[g.size_s];
     int part0 = 0, run[kPhases] = {};
     for (int i = 0; i < count; ++i) {
-        const unflow_matrix& q = a[first + i];
+        const unflow_matrix& q = a[order.at[i]];
         Problem p{};
         p.x = q.x; p.out = q.out; p.momentum = q.momentum;
         p.rows = q.rows; p.cols = q.cols;
-        p.m = q.rows < q.cols ? q.rows : q.cols;
-        p.n = q.rows < q.cols ? q.cols : q.rows;
+        p.m = order.m[i]; p.n = order.n[i];
         p.boost = q.rows > q.cols ? sqrtf((float)q.rows / (float)q.cols) : 1.f;
         p.X = take(2 * packed_width(TWO, p.n) * p.m);
         p.XT0 = take(2 * packed_width(TWO, p.m) * p.n);
         p.XT1 = take(2 * packed_width(TWO, p.m) * p.n);
         p.S = take(2 * packed_width(TWO, p.m) * p.m);
         p.Q = take(2 * packed_width(TWO, p.m) * p.m);
-        const long long stages = (packed_width(TWO, p.n) + 63) / 64;
-        long long shares = want < stages / 4 ? want : stages / 4;
-        if (shares > 16) shares = 16;
-        if (shares > 1) { const long long per = (stages + shares - 1) / shares; shares = (stages + per - 1) / per; } else shares = 1;
-        p.shares = (int)shares;
-        const int low = (int)lower(p.m, size);
-        if (p.shares > 1) p.shares_at = take(4ll * size * size * low * p.shares);
+        p.shares = shares_of(stages_of(packed_width(TWO, p.n)), cs.limit);
+        const int low = (int)lower_tiles_of(p.m, kSizes[g.size_s]);
+        if (p.shares > 1) p.shares_at = take(4ll * kSizes[g.size_s] * kSizes[g.size_s] * low * p.shares);
         p.part0 = part0;
-        p.parts = (int)(((long long)p.rows * p.cols + kChunk - 1) / kChunk);
+        p.parts = (int)(((long long)p.rows * p.cols + g.chunk - 1) / g.chunk);
         part0 += p.parts;
         run[kNorm] += p.parts;
         run[kPack] += ceil_div(p.rows, 64) * ceil_div(p.cols, 64);
         run[kSquare] += low * p.shares;
-        run[kJoin] += p.shares > 1 ? low : 0;
-        run[kPoly] += low;
-        run[kApply] += (int)full(p.m, p.n, kSizes[g.size_x]);
+        run[kJoin] += p.shares > 1 ? low * (kSizes[g.size_s] / 64) * (kSizes[g.size_s] / 64) : 0;
+        run[kPoly] += (int)lower_tiles_of(p.m, kSizes[g.size_q]);
+        run[kApply] += (int)tiles_of(p.m, p.n, kSizes[g.size_x]);
         if (problems) {
             problems[i] = p;
             for (int k = 0; k < kPhases; ++k) ends[k * count + i] = run[k];
         }
+    }
+    if (problems) {
+        // matrices whose work items of a phase are equally long are dealt out together (they are neighbours for S, which sums over n; the other two
+        // sum over m, which need not be in order: as far as neighbours are alike)
+        const int phases[3] = {kSquare, kPoly, kApply}, tables[3] = {kSquareClass, kPolyClass, kApplyClass};
+        for (int k = 0; k < 3; ++k)
+            for (int i = 0; i < count;) {
+                int e = i + 1;
+                while (e < count && (k == 0 ? order.n[e] == order.n[i] && problems[e].shares == problems[i].shares : order.m[e] == order.m[i])) ++e;
+                const int* run_of = ends + phases[k] * count;
+                for (int j = i; j < e; ++j) {
+                    ends[tables[k] * count + 2 * j] = i ? run_of[i - 1] : 0;
+                    ends[tables[k] * count + 2 * j + 1] = run_of[e - 1];
+                }
+                i = e;
+            }
     }
     for (int k = 0; k < kPhases; ++k) g.total[k] = run[k];
     g.bytes = at;
@@ -432,7 +493,7 @@ static Group lay_out(const unflow_matrix* a, int first, int count, Problem* prob
 static int group_end(const unflow_matrix* a, int count, int first) {
     long long bytes = 0;
     int i = first;
-    for (; i < count && i - first < 1024; ++i) {
+    for (; i < count && i - first < kMost; ++i) {
         const long long r = a[i].rows, c = a[i].cols;
         bytes += plane_bytes(r < c ? r : c, r < c ? c : r);
         if (i > first && bytes > kGroupBytes) break;
@@ -447,10 +508,6 @@ static bool matrices_ok(const unflow_matrix* a, int count, int dtype) {
     return true;
 }
 
-#define WITH_SIZE(index, ...)                                                                                                  \
-    do {                                                                                                                       \
-        if (index == 0) { using TileT = T256t; __VA_ARGS__; } else if (index == 1) { using TileT = T128t; __VA_ARGS__; } else { using TileT = T64t; __VA_ARGS__; } \
-    } while (0)
 #define LAUNCH_TILES(kernel, count, ...)                                                                                              \
     do {                                                                                                                              \
         if (TileT::LDS > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS); \
@@ -472,14 +529,23 @@ static void iterate(const Group& g, int steps, float a, float b, float c, float 
     const int* ends = (const int*)(ws + g.ends);
     double* parts = (double*)(ws + g.parts);
     const int n = g.count;
-    UNFLOW_LAUNCH((norm_kernel<T, STEP>), dim3(g.total[kNorm]), dim3(256), 0, stream, table, ends + kNorm * n, n, mu, nesterov, parts);
+    UNFLOW_LAUNCH((norm_kernel<T, STEP>), dim3(g.total[kNorm]), dim3(256), 0, stream, table, ends + kNorm * n, n, g.chunk, mu, nesterov, parts);
     UNFLOW_LAUNCH((start_kernel<T, STEP>), dim3(g.total[kPack]), dim3(256), 0, stream, table, ends + kPack * n, n, (const double*)parts, mu, nesterov, eps, ex, ws);
     for (int k = 0; k < steps; ++k) {
-        WITH_SIZE(g.size_s, LAUNCH_TILES((square_kernel<TileT>), g.total[kSquare], table, ends + kSquare * n, n, ex, ws));
-        if (g.total[kJoin]) WITH_SIZE(g.size_s, UNFLOW_LAUNCH((join_kernel<TileT>), dim3(g.total[kJoin]), dim3(TileT::THREADS), 0, stream, table, ends + kJoin * n, n, ex, ws));
-        WITH_SIZE(g.size_s, LAUNCH_TILES((poly_kernel<TileT>), g.total[kPoly], table, ends + kPoly * n, n, a, b, c, ex, ws));
-        if (k + 1 < steps) WITH_SIZE(g.size_x, LAUNCH_TILES((apply_kernel<TileT, false, false, float>), g.total[kApply], table, ends + kApply * n, n, k & 1, ex, up, ws));
-        else WITH_SIZE(g.size_x, LAUNCH_TILES((apply_kernel<TileT, true, STEP, T>), g.total[kApply], table, ends + kApply * n, n, k & 1, ex, up, ws));
+        with_tile(g.size_s, [&](auto tile) {
+            using TileT = decltype(tile);
+            LAUNCH_TILES((square_kernel<TileT>), g.total[kSquare], table, ends + kSquare * n, n, ends + kSquareClass * n, ex, ws);
+        });
+        if (g.total[kJoin]) UNFLOW_LAUNCH(join_kernel, dim3(g.total[kJoin]), dim3(256), 0, stream, table, ends + kJoin * n, n, kSizes[g.size_s], ex, ws);
+        with_tile(g.size_q, [&](auto tile) {
+            using TileT = decltype(tile);
+            LAUNCH_TILES((poly_kernel<TileT>), g.total[kPoly], table, ends + kPoly * n, n, ends + kPolyClass * n, a, b, c, ex, ws);
+        });
+        with_tile(g.size_x, [&](auto tile) {
+            using TileT = decltype(tile);
+            if (k + 1 < steps) LAUNCH_TILES((apply_kernel<TileT, false, false, float>), g.total[kApply], table, ends + kApply * n, n, ends + kApplyClass * n, k & 1, ex, up, ws);
+            else LAUNCH_TILES((apply_kernel<TileT, true, STEP, T>), g.total[kApply], table, ends + kApply * n, n, ends + kApplyClass * n, k & 1, ex, up, ws);
+        });
     }
 }
 
@@ -506,11 +572,11 @@ static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca
     char* ws = (char*)workspace;
     for (int i = 0; i < count;) {
         const int e = group_end(a, count, i), n = e - i;
-        static thread_local Problem problems[1024];
-        static thread_local int ends[1024 * kPhases];
+        static thread_local Problem problems[kMost];
+        static thread_local int ends[kMost * kTables];
         const Group g = lay_out(a, i, n, problems, ends);
         write_table(problems, (long long)sizeof(Problem) * n, ws + g.table, stream);
-        write_table(ends, 4ll * kPhases * n, ws + g.ends, stream);
+        write_table(ends, 4ll * kTables * n, ws + g.ends, stream);
         if (dtype == kFp32) iterate<float, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else if (dtype == kBf16) iterate<__bf16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else iterate<_Float16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);

@@ -5,9 +5,8 @@
 
 namespace {
 
-// What is read: rows x cols, `ld` elements from row to row.  Numbers are multiplied by 2^*exp (exp == nullptr: as they are).  A row r with
-// label[r] == skip counts as zeros (pack_columns; label == nullptr: none does).
-struct Source { const void* p; long long ld; int rows, cols; const int* exp; const long long* label = nullptr; long long skip = 0; };
+// What is read: rows x cols, `ld` elements from row to row.  A row r with label[r] == skip does not count (label == nullptr: every row does).
+struct Source { const void* p; long long ld; int rows, cols; const long long* label = nullptr; long long skip = 0; };
 
 template <class T> __device__ __forceinline__ f32x4 load4(const T* p, int n) {               // the first n = 0 .. 4 of four numbers, zeros behind them
     f32x4 v{0.f, 0.f, 0.f, 0.f};
@@ -28,25 +27,13 @@ template <class T> __device__ __forceinline__ f32x4 load4(const T* p, int n) {  
 }
 __device__ __forceinline__ f32x4 scaled(f32x4 v, int e) { return f32x4{ldexpf(v[0], e), ldexpf(v[1], e), ldexpf(v[2], e), ldexpf(v[3], e)}; }
 
-// dst row r = source row r; `width` (numbers a row holds, a multiple of 4: packed_width of ONE, half of it for TWO) >= cols, zeros behind cols
+// dst row c = source column c times 2^e, for the `cols` columns; `width` >= rows numbers a dst row holds, zeros behind rows and for rows that do
+// not count.  The 64 x 64 tile (bx, by) of
+// ceil(width / 64) x ceil(cols / 64)
 template <class T, int PL, int EL>
-__global__ __launch_bounds__(256) void pack_rows_kernel(Source s, u16* __restrict__ dst, long long ldd, int width) {
-    const int e = s.exp ? *s.exp : 0;
-    const long long per = width / 4, total = per * s.rows;
-    for (long long g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
-        const long long r = g / per;
-        const int k = (int)(g - r * per) * 4;
-        pack4<PL, EL>(dst + r * ldd, k, scaled(load4((const T*)s.p + r * s.ld + k, s.cols - k), e));
-    }
-}
-
-// dst row c = source column c, for the `cols` columns; `width` >= rows numbers a dst row holds, zeros behind rows.  64 x 64 tiles, grid
-// (ceil(width / 64), ceil(cols / 64))
-template <class T, int PL, int EL>
-__global__ __launch_bounds__(256) void pack_columns_kernel(Source s, u16* __restrict__ dst, long long ldd, int width) {
+__device__ __forceinline__ void pack_columns_tile(const Source& s, int e, u16* __restrict__ dst, long long ldd, int width, int bx, int by) {
     __shared__ float tile[64][65];
-    const int e = s.exp ? *s.exp : 0;
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+    const int r0 = bx * 64, c0 = by * 64;
     const int x = (threadIdx.x & 15) * 4, y = threadIdx.x >> 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

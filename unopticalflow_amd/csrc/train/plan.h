@@ -1,0 +1,74 @@
+// Which tile size a launch takes, and into how many shares its sums are cut, from a model of what the launch costs.
+//
+// A launch works on jobs: `tiles` tiles of a side, each summing over `stages` stages of 64 packed elements.  A tile of side 256 has the best rate
+// (an operand is read once for 256 rows of the other), smaller ones fill the chip better; sums cut into shares fill it too, but leave fp32
+// partial sums that are written, read and added.  The model: units (a share of a tile) run on `slots` places in rounds of the longest
+// unit; a unit costs its stages times the measured time of one, and a start and an end.
+#pragma once
+#include "mfma16.h"
+#include <cmath>
+
+namespace {
+
+constexpr int kSizes[4] = {256, 192, 128, 64};
+
+struct Job { long long m, n; int stages; bool lower, cut; int times = 1; };  // m x n outputs (lower: the lower triangle of m x m) of `times` matrices; cut: may be cut into shares
+struct Choice { int size, limit; double us; };                            // index into kSizes; stages of the longest share
+
+// how many shares a sum of `stages` is cut into so that none is longer than `limit` (at most 16 shares, none empty)
+static int shares_of(int stages, int limit) {
+    int shares = (stages + limit - 1) / limit;
+    shares = shares > 16 ? 16 : shares < 1 ? 1 : shares;
+    const int each = (stages + shares - 1) / shares;
+    return each > 0 ? (stages + each - 1) / each : 1;
+}
+static int stages_of(long long packed_width_) { return (int)((packed_width_ + 63) / 64); }
+
+static long long tiles_of(long long m, long long n, int size) { return ((m + size - 1) / size) * ((n + size - 1) / size); }
+static long long lower_tiles_of(long long m, int size) { const long long t = (m + size - 1) / size; return t * (t + 1) / 2; }
+
+// Measured: microseconds of one stage of a unit on a full chip (of the units that share a CU, together) and on one that is not, and of a unit's
+// start and end.  (8192 x 8192 x 2048 and 1024 x 1024 x 4096, ONE and TWO planes)
+struct Cost { double full, alone, ends; int per_cu; };
+static const Cost kCost[2][4] = {{{1.43, 1.10, 10., 1}, {1.00, 0.75, 7., 1}, {1.00, 0.60, 6., 2}, {0.75, 0.46, 4., 4}},
+                                 {{2.05, 1.45, 10., 1}, {1.17, 0.87, 7., 1}, {1.15, 0.56, 6., 2}, {0.80, 0.40, 4., 4}}};
+constexpr double kJoinBytesPerUs = 3.0e6, kLaunchUs = 5.0;
+
+static Choice choose(int planes, const Job* jobs, int count) {
+    Choice best{0, 1, -1.};
+    int longest = 1;
+    bool any = false;
+    for (int i = 0; i < count; ++i) {
+        if (jobs[i].cut && jobs[i].stages > longest) longest = jobs[i].stages;
+        any = any || jobs[i].cut;
+    }
+    for (int z = 0; z < 4; ++z) {
+        const Cost& c = kCost[planes == TWO ? 1 : 0][z];
+        for (int s = 1; s <= 16; s = s < 4 ? s + 1 : s < 8 ? s + 2 : s + 4) {
+            const int limit = (longest + s - 1) / s;
+            if (s > 1 && (!any || limit < 4)) break;
+            double most = 0., least = 1e30, sum = 0., count_ = 0., joined = 0.;      // microseconds of a unit on a full chip, and of all of them
+            int stages = 1;                                                // of the longest
+            for (int i = 0; i < count; ++i) {
+                const int shares = jobs[i].cut ? shares_of(jobs[i].stages, limit) : 1, each = (jobs[i].stages + shares - 1) / shares;
+                const double tiles = (double)jobs[i].times * (jobs[i].lower ? lower_tiles_of(jobs[i].m, kSizes[z]) : tiles_of(jobs[i].m, jobs[i].n, kSizes[z]));
+                const double us = each * c.full + c.ends;
+                most = us > most ? us : most;
+                least = us < least ? us : least;
+                stages = each > stages ? each : stages;
+                sum += tiles * shares * us;
+                count_ += tiles * shares;
+                if (shares > 1) joined += tiles * shares * kSizes[z] * kSizes[z] * 8.;
+            }
+            // every CU busy to the end but for a part of the shortest unit; the longest are started first
+            double us = ceil(sum / (256. * c.per_cu) / least - 1e-9) * least;
+            us = us > most ? us : most;
+            if (count_ <= 256.) us = stages * c.alone + c.ends;
+            us += joined > 0. ? kLaunchUs + joined / kJoinBytesPerUs : 0.;
+            if (best.us < 0. || us < best.us) best = Choice{z, limit, us};
+        }
+    }
+    return best;
+}
+
+}  // namespace

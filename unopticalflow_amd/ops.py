@@ -1776,15 +1776,19 @@ _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
 
 def _dev_typed(what, *tensors):
     """All operands on one HIP device and of one of the types the training operators take -> (device, UNFLOW_DTYPE_*)."""
-    first = tensors[0]
-    for t in tensors:
-        if not on_device(t):
-            raise RuntimeError('unopticalflow_amd ops run on an MI355X (HIP) device only; got a %s tensor. There is no CPU fallback.' % t.device)
-        if t.dtype not in _DTYPES or t.dtype != first.dtype:
-            raise TypeError('%s takes fp32, bf16 or fp16 tensors of one type; got %s' % (what, sorted({str(u.dtype) for u in tensors})))
-        if t.device != first.device:
-            raise RuntimeError('operands on different devices: %s vs %s' % (first.device, t.device))
-    return first.device, _DTYPES[first.dtype]
+    devices, dtypes = {t.device for t in tensors}, {t.dtype for t in tensors}
+    if not on_device(tensors[0]) or len(devices) > 1:
+        if all(on_device(t) for t in tensors):
+            raise RuntimeError('operands on different devices: %s' % sorted(map(str, devices)))
+        raise RuntimeError('unopticalflow_amd ops run on an MI355X (HIP) device only; got tensors on %s. There is no CPU fallback.' % sorted(map(str, devices)))
+    if len(dtypes) > 1 or tensors[0].dtype not in _DTYPES:
+        raise TypeError('%s takes fp32, bf16 or fp16 tensors of one type; got %s' % (what, sorted(map(str, dtypes))))
+    return tensors[0].device, _DTYPES[tensors[0].dtype]
+
+
+def _stream_of(dev):
+    """The current stream of a device as the C entries take it."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _rows_of(t):
@@ -1797,51 +1801,48 @@ def _rows_of(t):
     return t, t.shape[1]
 
 
-def _linear_ce_workspaces(hidden, ldh, weight, ldw, need_h, need_w):
-    fwd, bwd = ctypes.c_longlong(), ctypes.c_longlong()
-    _call('unflow_linear_ce_workspace', _ptr(hidden), ldh, _ptr(weight), ldw, hidden.shape[0], weight.shape[0], weight.shape[1],
-          _DTYPES[hidden.dtype], int(need_h), int(need_w), ctypes.byref(fwd), ctypes.byref(bwd))
-    return fwd.value, bwd.value
-
-
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, scale, reduction):
         dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
         (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
         (N, D), V = hidden.shape, weight.shape[0]
-        loss = torch.empty(N if reduction == 0 else 1, dtype=torch.float32, device=dev)
-        lse = torch.empty(N, dtype=torch.float32, device=dev)
-        ctx.how = (ignore_index, scale, reduction)
+        loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
+        need_h, need_w = ctx.needs_input_grad[:2]
         if N == 0:
-            loss.zero_()
-        else:
-            with _on(dev):
-                need, _ = _linear_ce_workspaces(hidden, ldh, weight, ldw, False, False)
-                ws = torch.empty(need, dtype=torch.uint8, device=dev)
-                _call('unflow_linear_ce_fwd', _ptr(hidden), ldh, _ptr(weight), ldw, _ptr(target), N, V, D, dtype, scale, ignore_index,
-                      reduction, _ptr(loss), _ptr(lse), _ptr(ws), need, _stream(),
-                      nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
-        ctx.save_for_backward(hidden, weight, target, lse)
-        return loss if reduction == 0 else loss.view(())
+            ctx.how = (ignore_index, scale, reduction, ldh, ldw, dtype, 0)
+            ctx.save_for_backward(hidden, weight, target, None)
+            return loss.zero_()
+        with _on(dev):
+            sizes = (ctypes.c_longlong * 3)()            # bytes kept for the backward pass, of the forward's workspace, of the backward's
+            at = ctypes.addressof(sizes)
+            _call('unflow_linear_ce_workspace', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, N, V, D, dtype, need_h, need_w, at, at + 8, at + 16)
+            kept = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
+            ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
+            _call('unflow_linear_ce_fwd', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), N, V, D, dtype, scale, ignore_index,
+                  reduction, loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), sizes[1], _stream_of(dev),
+                  nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+        if need_h or need_w:
+            ctx.how = (ignore_index, scale, reduction, ldh, ldw, dtype, sizes[2])
+            ctx.save_for_backward(hidden, weight, target, kept)
+        return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        hidden, weight, target, lse = ctx.saved_tensors
-        ignore_index, scale, reduction = ctx.how
+        hidden, weight, target, kept = ctx.saved_tensors
+        ignore_index, scale, reduction, ldh, ldw, dtype, need = ctx.how
         need_h, need_w = ctx.needs_input_grad[:2]
-        (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
-        (N, D), V = hidden.shape, weight.shape[0]
-        dh = torch.empty((N, D), dtype=hidden.dtype, device=hidden.device) if need_h else None
-        dw = torch.empty((V, D), dtype=weight.dtype, device=weight.device) if need_w else None
+        (N, D), V, dev = hidden.shape, weight.shape[0], hidden.device
+        dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if need_h else None
+        dw = torch.empty((V, D), dtype=weight.dtype, device=dev) if need_w else None
         if N == 0:
             return dh, dw.zero_() if need_w else None, None, None, None, None
-        with _on(hidden.device):
-            _, need = _linear_ce_workspaces(hidden, ldh, weight, ldw, need_h, need_w)
-            ws = torch.empty(need, dtype=torch.uint8, device=hidden.device)
-            _call('unflow_linear_ce_bwd', _ptr(hidden), ldh, _ptr(weight), ldw, _ptr(target), _ptr(lse), _ptr(g.contiguous()), N, V, D,
-                  _DTYPES[hidden.dtype], scale, ignore_index, reduction, _ptr(dh), _ptr(dw), _ptr(ws), need, _stream(),
+        with _on(dev):
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            g = g.contiguous()
+            _call('unflow_linear_ce_bwd', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), g.data_ptr(), N, V, D,
+                  dtype, scale, ignore_index, reduction, dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None,
+                  kept.data_ptr(), ws.data_ptr(), need, _stream_of(dev),
                   nbytes=2 * (N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
         return dh, dw, None, None, None, None
 
@@ -1854,7 +1855,9 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
     fp32; both gradients come in the inputs' type, from sums in fp32 (fp32 inputs: products and sums of fp32 accuracy).  ``reduction``:
     'mean' over the rows that are not ignored (0 if there are none), 'sum', or 'none' (the shape of ``target``).  A row whose target is
     ``ignore_index`` has loss 0 and no part in the gradients, whatever it holds; any other target outside [0, V) makes its row's loss, and
-    the gradients it reaches, NaN.  Results are bitwise reproducible."""
+    the gradients it reaches, NaN.  Results are bitwise reproducible.
+
+    Between the passes 16 bytes per row are kept, and for fp32 inputs (or rows that are not multiples of 16 bytes) a packed copy of both."""
     if reduction not in _REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got {!r}".format(reduction))
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
@@ -1907,9 +1910,9 @@ def _newton_schulz(entry, dev, dtype, table, count, args):
     """One call of an entry point that takes a list of matrices and a workspace."""
     with _on(dev):
         need = ctypes.c_longlong()
-        _call('unflow_orthogonalize_workspace', table, count, dtype, ctypes.byref(need))
+        _call('unflow_orthogonalize_workspace', table, count, dtype, ctypes.addressof(need))
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        _call(entry, table, count, dtype, *args, _ptr(ws), need.value, _stream())
+        _call(entry, table, count, dtype, *args, ws.data_ptr(), need.value, _stream_of(dev))
 
 
 def orthogonalize(matrices, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):

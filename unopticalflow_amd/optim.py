@@ -162,6 +162,10 @@ def _walks_as_matrix(t):
     return _dense(t) and (t.shape[0] == 1 or t.stride(0) == t.numel() // t.shape[0])
 
 
+def _other_strides(a, b):
+    return any(x != y and n > 1 for x, y, n in zip(a.stride(), b.stride(), b.shape))
+
+
 @torch.no_grad()
 def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nesterov=True, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     """One Muon step over a list of weights, in place: every weight is a matrix [shape[0], the rest] (csrc/train/muon.hip, one launch per phase
@@ -177,23 +181,27 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
         raise ValueError('muon_step_: %d parameters, %d gradients, %d momenta' % (len(params), len(grads), len(momenta)))
     steps, coefficients = ops._check_newton_schulz('muon_step_', steps, coefficients, eps)
     keep = [i for i, p in enumerate(params) if p.numel()]
-    params, grads, momenta = ([v[i] for i in keep] for v in (params, grads, momenta))
+    if len(keep) < len(params):
+        params, grads, momenta = ([v[i] for i in keep] for v in (params, grads, momenta))
     if not params:
         return
+    copied = []                                    # (alive until the work on them is enqueued)
     dev, dtype = ops._dev_typed('muon_step_', *params, *grads)
+    if {m.dtype for m in momenta} != {torch.float32} or {m.device for m in momenta} != {dev}:
+        raise TypeError('muon_step_: momenta are fp32 on the parameters\' device')
     items = []
-    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        if p.dim() < 2 or g.shape != p.shape or m.shape != p.shape:
+    for p, g, m in zip(params, grads, momenta):
+        shape, stride = p.shape, p.stride()
+        if len(shape) < 2 or g.shape != shape or m.shape != shape:
             raise ValueError('muon_step_: parameter, gradient and momentum must have one shape of two or more dimensions: {}, {}, {}'.format(
-                tuple(p.shape), tuple(g.shape), tuple(m.shape)))
-        if m.dtype != torch.float32 or m.device != p.device:
-            raise TypeError('muon_step_: momenta are fp32 on their parameter\'s device; got %s on %s' % (m.dtype, m.device))
-        rows, cols = p.shape[0], p.numel() // p.shape[0]
-        if not _walks_as_matrix(p) or any(a != b and n > 1 for a, b, n in zip(m.stride(), p.stride(), p.shape)) or max(rows, cols) > ops._MATRIX_MAX_SIDE:
+                tuple(shape), tuple(g.shape), tuple(m.shape)))
+        rows, cols = shape[0], p.numel() // shape[0]
+        if not (p.is_contiguous() or _walks_as_matrix(p)) or (m.stride() != stride and _other_strides(m, p)) or rows > ops._MATRIX_MAX_SIDE or cols > ops._MATRIX_MAX_SIDE:
             raise ValueError('muon_step_: a parameter must be dense with its first dimension outermost, its momentum of the same layout, sides up to {}; got shape {}, strides {} and {}'.format(
-                ops._MATRIX_MAX_SIDE, tuple(p.shape), p.stride(), m.stride()))
-        if any(a != b and n > 1 for a, b, n in zip(g.stride(), p.stride(), p.shape)):
-            grads[i] = g = torch.empty_like(p).copy_(g)
+                ops._MATRIX_MAX_SIDE, tuple(shape), stride, m.stride()))
+        if g.stride() != stride and _other_strides(g, p):
+            g = torch.empty_like(p).copy_(g)
+            copied.append(g)
         items.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), rows, cols))
     if len({x[1] for x in items}) < len(items) or len({x[2] for x in items}) < len(items):
         raise ValueError('muon_step_: a parameter or momentum appears twice')
