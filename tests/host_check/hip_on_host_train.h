@@ -16,7 +16,6 @@ static inline unsigned long long __ballot(int p) {
     return hip_on_host::ballots[wave];
 }
 static inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
-#define __expf(v) expf(v)                                                  // (the name is glibc's own)
 
 // v_mfma_f32_16x16x32_f16: the lane layouts of the bf16 form (hip_on_host.h)
 typedef _Float16 hip_on_host_f16x8 __attribute__((ext_vector_type(8)));
@@ -82,7 +81,11 @@ static inline hip_on_host_v4f hip_on_host_mfma_16x16x4_f32(float a, float b, hip
 }
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, x, y, z) hip_on_host_mfma_16x16x4_f32(a, b, c)
 
+#define __builtin_amdgcn_exp2f(v) exp2f(v)
+
 // LDS-DMA through a byte range (device_forms.h): landed when the call returns
 typedef hip_on_host::Rsrc byte_range;
 static inline byte_range range_of(const void* p, int bytes) { return byte_range{(char*)p, (unsigned)bytes}; }
-static inline void copy16_to_lds(byte_range r, char* to, unsigned offset) { hip_on_host::buf_load<16>(r, (int)offset, 0, to + (hip_on_host::lane_id & 63u) * 16); }
+typedef char* lds_address;
+static inline lds_address address_in_lds(char* p) { return p; }
+static inline void copy16_to_lds(byte_range r, lds_address to, unsigned offset) { hip_on_host::buf_load<16>(r, (int)offset, 0, to + (hip_on_host::lane_id & 63u) * 16); }

@@ -85,9 +85,10 @@ __device__ __forceinline__ byte_range range_of(const void* p, int bytes) {
     const unsigned long long a = (unsigned long long)p;
     return v4i{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
-__device__ __forceinline__ void copy16_to_lds(byte_range r, char* to, unsigned offset) {
-    const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(__attribute__((address_space(3))) char*)to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(r) : "memory", "m0");
+typedef unsigned lds_address;                                         // of a wave's copy: bytes from the start of the workgroup's LDS
+__device__ __forceinline__ lds_address address_in_lds(const char* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
+__device__ __forceinline__ void copy16_to_lds(byte_range r, lds_address to, unsigned offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)to)), "v"(offset), "s"(r) : "memory", "m0");
 }
 
 // wave shifts by one lane (ssim.hip): DPP row shifts across the whole wave, not hipcc's __shfl (= ds_bpermute)

@@ -28,7 +28,7 @@ constexpr int kMaxima = 1024;                                      // workgroups
 // fp32 rows are packed with a power of two of their own that brings the row's largest magnitude to [2^14, 2^15), their transposes (where rows are
 // what is summed over) with one for the whole matrix.
 struct Exponents { int h, w; };      // of the transposes
-struct Row { float top, inverse, others, unused; };                // of a row: max z, 1 / sum exp(z - top), sum over all classes but the target times that
+struct Row { float top, inverse, others, unused; };                // of a row: log2(e) max z, 1 / sum exp(z - max z), sum over all classes but the target times that
 
 __device__ __forceinline__ float finite_magnitude(float m, f32x4 v) {
 #pragma unroll
@@ -78,8 +78,10 @@ __global__ __launch_bounds__(256) void pack_inputs_kernel(Source h, Source w, in
     }
 }
 
-// z of an accumulator of row m and column n
-struct Logits { float scale; const int *eh, *ew; };
+// log2(e) z of an accumulator of row m and column n: exponentials are then single instructions
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+struct Logits { float scale; const int *eh, *ew; };             // scale: of the loss, times log2(e)
 template <int PL> __device__ __forceinline__ f32x4 logits_of(const Logits& l, f32x4 acc, int eh, int n, int last) {
     acc *= l.scale;
     if constexpr (PL == TWO) {
@@ -89,38 +91,55 @@ template <int PL> __device__ __forceinline__ f32x4 logits_of(const Logits& l, f3
     return acc;
 }
 
-// ---- forward: of each row of a tile of z the maximum and the sum of exp(z - maximum) over the classes that are not the row's target, and the
-// target's z.  partial [tile column][N]
+// ---- forward: of each row of a tile of z the maximum (times log2(e), as all that follows) and the sum of exp(z - maximum) over the classes that
+// are not the row's target, and the target's z.  partial [tile column][N]
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand H, Operand W, int width, Logits how,
                                                                                                     const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
     UNFLOW_DYNAMIC_LDS(char, lds);
-    const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(W.rows, TileT::BN);
-    int tm, tn;
-    tile_of(xcd_remap((int)blockIdx.x, (int)gridDim.x), mt, nt, tm, tn);
-    const int m0 = tm * TileT::BM, n0 = tn * TileT::BN;
-    TileT T;
-    T.run(H, W, 0, width, m0, n0, lds);
-    float2* rows = reinterpret_cast<float2*>(lds);                                       // [WN][BM]
+    const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(W.rows, TileT::BN), total = mt * nt;
+    float2* rows = reinterpret_cast<float2*>(lds + 2 * TileT::STAGE);                    // [WN][BM]
     const int wn = TileT::wave() % TileT::WN, group = ((int)threadIdx.x & 63) >> 4;
+    int id = (int)blockIdx.x, tm, tn;
+    tile_of(xcd_remap(id, total), mt, nt, tm, tn);
+    TileT T;
+    T.start(H, W, 0, width, tm * TileT::BM, tn * TileT::BN, lds);
+    // a workgroup goes through tiles a grid apart: the copies of the next one are under way while this one's sums are dealt with
+    for (bool more = true; more;) {
+    T.finish(lds);
+    const int m0 = tm * TileT::BM, n0 = tn * TileT::BN, column = tn;
+    id += (int)gridDim.x;
+    more = id < total;
+    if (more) {
+        tile_of(xcd_remap(id, total), mt, nt, tm, tn);
+        T.start(H, W, 0, width, tm * TileT::BM, tn * TileT::BN, lds);
+    }
+    const bool edge = n0 + TileT::BN > W.rows;
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
-        const long long t = m < H.rows ? target[m] : -1;
-        const int eh = TileT::PL == TWO && m < H.rows ? how.eh[m] : 0;
+        const long long t = m < H.rows ? target[m] - n0 : -1;                            // the target's place in this tile
+        const int own = t >= 0 && t < TileT::BN && t + n0 < W.rows ? (int)t : -1, eh = TileT::PL == TWO && m < H.rows ? how.eh[m] : 0;
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j) {
-            const f32x4 zs = logits_of<TileT::PL>(how, T.acc[i][j], eh, n0 + TileT::col(j), W.rows - 1);
+            f32x4 z = logits_of<TileT::PL>(how, T.acc[i][j], eh, n0 + TileT::col(j), W.rows - 1);
+            if (edge)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int n = n0 + TileT::col(j) + r;
-                const float z = n < W.rows ? zs[r] : -INFINITY;
-                top = fmaxf(top, z);
-                if (n == t && n < W.rows) ztarget[m] = z;
-                T.acc[i][j][r] = n == t ? -INFINITY : z;
-            }
+                for (int r = 0; r < 4; ++r) z[r] = n0 + TileT::col(j) + r < W.rows ? z[r] : -INFINITY;
+            T.acc[i][j] = z;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, z[r]);
         }
+        if (__ballot(own >= 0))                                                          // (few of a wave's rows have their target among its columns)
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (TileT::col(j) + r == own) {
+                        ztarget[m] = T.acc[i][j][r];
+                        T.acc[i][j][r] = -INFINITY;
+                    }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float base = top == -INFINITY ? 0.f : top;
@@ -128,7 +147,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum += __expf(T.acc[i][j][r] - base);
+            for (int r = 0; r < 4; ++r) sum += exp2_of(T.acc[i][j][r] - base);
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
         if (group == 0) rows[wn * TileT::BM + TileT::row(i)] = make_float2(top, sum);
@@ -141,13 +160,16 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
 #pragma unroll
         for (int q = 0; q < TileT::WN; ++q) {
             const float2 v = rows[q * TileT::BM + r];
-            sum += v.x != -INFINITY ? v.y * __expf(v.x - top) : v.y;                      // (without a maximum: 0, or NaN from NaNs, which fmaxf passes over)
+            sum += v.x != -INFINITY ? v.y * exp2_of(v.x - top) : v.y;                      // (without a maximum: 0, or NaN from NaNs, which fmaxf passes over)
         }
-        partial[(long long)tn * H.rows + m0 + r] = make_float2(top, sum);
+        partial[(long long)column * H.rows + m0 + r] = make_float2(top, sum);
+    }
     }
 }
 
-// ---- forward of few rows (at most 16 NF): reading W is all there is to it.  A workgroup takes 64 classes, its four waves a quarter of D each, four
+// ---- forward of few rows (at most 16 NF): reading W is all there is to it.  16-bit inputs of more than 16 rows are better served by the tiles
+// above, where the four waves share the rows of H (61 rows against 50257 classes of 1024 fp16: 28 us against 36); fp32 inputs stay here up to 64
+// rows, for packing W would read and write all of it once more.  A workgroup takes 16 CF classes, its four waves a quarter of D each, AHEAD
 // steps of loads in flight; the rows of W go from memory to the matrix instruction as they lie there.  16-bit numbers: 32 k a step, lane l holds
 // k = 8 (l >> 4) .. of row l & 15.  fp32: 16 k a step as four v_mfma_f32_16x16x4_f32, the e-th taking k = 4 (l >> 4) + e -- fp32 arithmetic
 // throughout, and no packing.
@@ -160,47 +182,46 @@ template <class T> __device__ __forceinline__ f32x4 few_product(uint4 a, uint4 b
         return c;
     } else return mfma16<__is_same(T, __bf16) ? BF16 : FP16>(a, b, c);
 }
-template <class T, int NF>
+template <class T, int NF, int CF, int AHEAD>
 __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, long long ldh, const T* __restrict__ W, long long ldw, int N, int V, int D, float scale, const long long* __restrict__ target,
                                                       float2* __restrict__ partial, float* __restrict__ ztarget) {
-    constexpr int ROWS = 16 * NF, PER = 256 / ROWS, CLASSES = 64 / PER, AHEAD = 4, PITCH = 66;
+    constexpr int ROWS = 16 * NF, PER = 256 / ROWS, CLASSES = 16 * CF / PER, PITCH = 16 * CF + 2;
     __shared__ float sums[4][ROWS][PITCH];
     const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int v0 = (int)blockIdx.x * 64, k_lane = (lane >> 4) * Few<T>::EACH, r_lane = lane & 15;
-    const T* wrow[4];
+    const int v0 = (int)blockIdx.x * 16 * CF, k_lane = (lane >> 4) * Few<T>::EACH, r_lane = lane & 15;
+    const T* wrow[CF];
     const T* hrow[NF];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) wrow[c] = W + (long long)(v0 + 16 * c + r_lane < V ? v0 + 16 * c + r_lane : V - 1) * ldw;          // (classes behind the last repeat it, unused)
+    for (int c = 0; c < CF; ++c) wrow[c] = W + (long long)(v0 + 16 * c + r_lane < V ? v0 + 16 * c + r_lane : V - 1) * ldw;          // (classes behind the last repeat it, unused)
 #pragma unroll
     for (int i = 0; i < NF; ++i) hrow[i] = H + (long long)(16 * i + r_lane < N ? 16 * i + r_lane : N - 1) * ldh;
-    f32x4 acc[4][NF];
+    f32x4 acc[CF][NF];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < CF; ++c)
 #pragma unroll
         for (int i = 0; i < NF; ++i) acc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int steps = ceil_div(D, Few<T>::STEP);
     for (int first = 0; first < steps; first += 4 * AHEAD) {
-        const int s = first + w;
-        uint4 a[AHEAD][4], b[AHEAD][NF];
+        uint4 a[AHEAD][CF], b[AHEAD][NF];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int k = (s + 4 * u) * Few<T>::STEP + k_lane;
+            const int k = (first + (u / 2) * 8 + w * 2 + u % 2) * Few<T>::STEP + k_lane;              // (a wave takes two steps in a row: whole lines of W)
             const bool in = k < D;                                                         // (D is a multiple of what a lane loads)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) a[u][c] = in ? *reinterpret_cast<const uint4*>(wrow[c] + k) : uint4{0, 0, 0, 0};
+            for (int c = 0; c < CF; ++c) a[u][c] = in ? *reinterpret_cast<const uint4*>(wrow[c] + k) : uint4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < NF; ++i) b[u][i] = in ? *reinterpret_cast<const uint4*>(hrow[i] + k) : uint4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < CF; ++c)
 #pragma unroll
                 for (int i = 0; i < NF; ++i) acc[c][i] = few_product<T>(a[u][c], b[u][i], acc[c][i]);
     }
     // a lane holds row 16 i + (lane & 15), classes 16 c + 4 (lane >> 4) ..
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < CF; ++c)
 #pragma unroll
         for (int i = 0; i < NF; ++i)
 #pragma unroll
@@ -223,7 +244,7 @@ __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, l
     for (int o = PER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int c = 0; c < CLASSES; ++c) sum += __expf(z[c] - base);
+    for (int c = 0; c < CLASSES; ++c) sum += exp2_of(z[c] - base);
 #pragma unroll
     for (int o = PER / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if (part == 0 && m < N) partial[(long long)blockIdx.x * N + m] = make_float2(top, sum);
@@ -243,7 +264,7 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict_
             const float2 v = partial[(long long)t * N + m];
             const float both = fmaxf(top, v.x);
             const float base = both == -INFINITY ? 0.f : both;
-            sum = sum * (top == -INFINITY ? 1.f : __expf(top - base)) + v.y * (v.x == -INFINITY ? 1.f : __expf(v.x - base));
+            sum = sum * (top == -INFINITY ? 1.f : exp2_of(top - base)) + v.y * (v.x == -INFINITY ? 1.f : exp2_of(v.x - base));
             top = both;
         }
     part[share][r] = make_float2(top, sum);
@@ -253,7 +274,7 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict_
             const float2 x = part[share][r], y = part[share + half][r];
             const float both = fmaxf(x.x, y.x);
             const float base = both == -INFINITY ? 0.f : both;
-            part[share][r] = make_float2(both, x.y * (x.x == -INFINITY ? 1.f : __expf(x.x - base)) + y.y * (y.x == -INFINITY ? 1.f : __expf(y.x - base)));
+            part[share][r] = make_float2(both, x.y * (x.x == -INFINITY ? 1.f : exp2_of(x.x - base)) + y.y * (y.x == -INFINITY ? 1.f : exp2_of(y.x - base)));
         }
         __syncthreads();
     }
@@ -262,9 +283,9 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict_
         const float others = part[0][r].y, base = top == -INFINITY ? 0.f : top;
         const long long t = target[m];
         const bool known = t >= 0 && t < V;
-        const float zt = known ? ztarget[m] : -INFINITY, own = known ? expf(zt - base) : 0.f, all = others + own;
+        const float zt = known ? ztarget[m] : -INFINITY, own = known ? exp2_of(zt - base) : 0.f, all = others + own;
         stats[m] = Row{base, 1.f / all, others / all, 0.f};
-        losses[m] = t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) + logf(all);
+        losses[m] = t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) * kLn2 + logf(all);
     }
 }
 
@@ -358,31 +379,38 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
     how.ew += PL == TWO ? v0 : 0;
     const float unit = (float)(1 << probability_exponent<EL>());
     const int wide_n = (int)round_up(vp, PL == TWO ? 32 : 8);
+    const bool edge = n0 + TileT::BN > vp;
     float weights[TileT::MI];
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
         const bool there = m < H.rows;
-        const long long t = there ? up.target[m] : up.ignore;
+        const long long t = there ? up.target[m] : up.ignore, in_tile = t - v0 - n0;
         const bool used = there && t != up.ignore, known = t >= 0 && t < V;
         const Row s = there ? stats[m] : Row{0.f, 0.f, 0.f, 0.f};
+        const int own = used && in_tile >= 0 && in_tile < TileT::BN ? (int)in_tile : -1, eh = PL == TWO && there ? how.eh[m] : 0;
+        const float inverse = used ? (known ? s.inverse * unit : NAN) : 0.f;
         weights[i] = !used ? 0.f : up.reduction == 0 ? up.g[m] / up.largest[0] : 1.f;
-        const int eh = PL == TWO && there ? how.eh[m] : 0;
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j) {
-            const int n = n0 + TileT::col(j);
-            const f32x4 z = logits_of<PL>(how, T.acc[i][j], eh, n, vp - 1);
-            f32x4 g;
+            const f32x4 z = logits_of<PL>(how, T.acc[i][j], eh, n0 + TileT::col(j), vp - 1);
+            // (z - top is at most 0; the minimum is there for a row that is not used and may hold anything: NaN becomes a number, and 0 times it)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float p = __expf(z[r] - s.top) * s.inverse;
-                if (v0 + n + r == t) p = -s.others;
-                p = used ? (known ? p : NAN) : 0.f;
-                g[r] = n + r < vp ? p * unit : 0.f;
-            }
-            T.acc[i][j] = g;
-            if (there && n < wide_n) pack4<PL, EL>(G + (long long)m * ldg, n, g);
+            for (int r = 0; r < 4; ++r) T.acc[i][j][r] = exp2_of(fminf(z[r] - s.top, 1.f)) * inverse;
+            if (edge)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) T.acc[i][j][r] = n0 + TileT::col(j) + r < vp ? T.acc[i][j][r] : 0.f;
         }
+        if (__ballot(own >= 0))
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (TileT::col(j) + r == own) T.acc[i][j][r] = -s.others * unit;
+        if (there)
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j)
+                if (n0 + TileT::col(j) < wide_n) pack4<PL, EL>(G + (long long)m * ldg, n0 + TileT::col(j), T.acc[i][j]);
     }
     // (a row that is not used, or behind the last, is zeros already: 0 times its weight)
     if (GT) T.store_transposed(lds, GT, ldgt, vp, ldgt, m0, n0, [&](int i, int j) { return T.acc[i][j] * weights[i]; });
@@ -408,7 +436,8 @@ template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product a, Product b, const Exponents* __restrict__ ex, Upstream up) {
     using T_ = typename OutputOf<TileT>::type;
     UNFLOW_DYNAMIC_LDS(char, lds);
-    // (each job is dealt over the XCDs by itself: their units differ in length)
+    // Each job is dealt over the XCDs by itself: their units differ in length.  (A workgroup that goes through units of its own, as in the forward
+    // pass, gains nothing where they are alike and loses a third where they are not.)
     const int units_a = a.tiles * a.shares;
     const bool second = (int)blockIdx.x >= units_a;
     const Product p = second ? b : a;
@@ -475,11 +504,13 @@ __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, i
 }
 
 // ---- the host side
-#define LAUNCH_TILES(kernel, count, ...)                                                                                              \
-    do {                                                                                                                              \
-        if (TileT::LDS > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS); \
-        UNFLOW_LAUNCH(kernel, dim3(count), dim3(TileT::THREADS), TileT::LDS, stream, __VA_ARGS__);                                    \
+#define LAUNCH_TILES(kernel, count, lds, ...)                                                                                  \
+    do {                                                                                                                       \
+        if (lds > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);      \
+        UNFLOW_LAUNCH(kernel, dim3(count), dim3(TileT::THREADS), lds, stream, __VA_ARGS__);                                    \
     } while (0)
+// workgroups of a kernel that goes through its tiles itself
+template <class TileT> static int resident(long long units) { return (int)(units < 256 * TileT::PER_CU ? units : 256 * TileT::PER_CU); }
 template <int PL, int EL, class F> static void with_tile(int size, F&& f) {
     if (size == 0) f(Tile<256, 256, 2, 4, PL, EL>{});
     else if (size == 1) f(Tile<192, 192, 2, 4, PL, EL>{});
@@ -500,6 +531,9 @@ struct Plan {
     long long repacked, exponents, largest, g, gt, ht, wt, sum_h, sum_w, backward_bytes;
 };
 
+// classes a workgroup of lce_few_kernel takes
+static int few_classes(int N) { return N <= 16 ? 64 : 32; }
+
 // 16-byte loads of whole rows
 static bool aligned(const void* p, long long ld, int D, int dtype) {
     const int each = dtype == kFp32 ? 4 : 8;
@@ -509,7 +543,7 @@ static bool aligned(const void* p, long long ld, int D, int dtype) {
 static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, bool train, bool need_h, bool need_w) {
     Plan p{};
     p.planes = dtype == kFp32 ? TWO : ONE;
-    p.few = N <= 64 && aligned(h, ldh, D, dtype) && aligned(w, ldw, D, dtype);
+    p.few = N <= (dtype == kFp32 ? 64 : 16) && aligned(h, ldh, D, dtype) && aligned(w, ldw, D, dtype);
     p.pack_h = dtype == kFp32 || !aligned(h, ldh, D, dtype);
     p.pack_w = dtype == kFp32 || !aligned(w, ldw, D, dtype);
     p.keeps = (p.pack_h || p.pack_w) && !p.few;
@@ -531,7 +565,7 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
     at = 0;
     const Job z{N, V, stages_of(p.wd), false, false};
     p.size_z = choose(p.planes, &z, 1).size;
-    p.partial = take(8ll * ceil_div(V, p.few ? 64 : kSizes[p.size_z]) * N);
+    p.partial = take(8ll * ceil_div(V, p.few ? few_classes(N) : kSizes[p.size_z]) * N);
     p.ztarget = take(4ll * N);
     p.losses = take(4ll * N);
     p.forward_bytes = at;
@@ -594,7 +628,7 @@ static Logits operands(const Plan& p, const Inputs& in, char* to, bool pack, hip
         UNFLOW_LAUNCH((pack_inputs_kernel<T, PL, EL>), dim3(blocks_h + blocks_w), dim3(256), 0, stream, Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, Source{in.w, in.ldw, in.V, in.D}, blocks_h,
                       at, p.wd, (int)(PL == TWO ? p.wd / 2 : p.wd));
     }
-    return Logits{in.scale, at.eh, at.ew};
+    return Logits{in.scale * kLog2E, at.eh, at.ew};
 }
 
 template <class T, int PL, int EL>
@@ -605,18 +639,21 @@ static void forward(const Plan& p, const Inputs& in, int reduction, float* loss,
     float* losses = reduction == 0 ? loss : (float*)(ws + p.losses);
     int columns;
     if (p.few) {
-        columns = ceil_div(in.V, 64);
+        columns = ceil_div(in.V, few_classes(in.N));
         const T *h = (const T*)in.h, *w = (const T*)in.w;
-        if (in.N <= 16) UNFLOW_LAUNCH((lce_few_kernel<T, 1>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, in.scale, in.target, partial, zt);
-        else if (in.N <= 32) UNFLOW_LAUNCH((lce_few_kernel<T, 2>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, in.scale, in.target, partial, zt);
-        else UNFLOW_LAUNCH((lce_few_kernel<T, 4>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, in.scale, in.target, partial, zt);
+        const float scale = in.scale * kLog2E;
+        // (beyond 16 rows a wave holds fewer classes, so that more waves fit a CU: 61 rows against 50257 classes of 1024 fp16)
+        if (in.N <= 16) UNFLOW_LAUNCH((lce_few_kernel<T, 1, 4, 4>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, scale, in.target, partial, zt);
+        else if constexpr (sizeof(T) < 4) return;
+        else if (in.N <= 32) UNFLOW_LAUNCH((lce_few_kernel<T, 2, 2, 4>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, scale, in.target, partial, zt);
+        else UNFLOW_LAUNCH((lce_few_kernel<T, 4, 2, 2>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, scale, in.target, partial, zt);
     } else {
         Operand H, W;
         const Logits how = operands<T, PL, EL>(p, in, kept, true, stream, H, W);
         columns = ceil_div(in.V, kSizes[p.size_z]);
         with_tile<PL, EL>(p.size_z, [&](auto tile) {
             using TileT = decltype(tile);
-            LAUNCH_TILES((lce_forward_kernel<TileT>), (int)tiles_of(in.N, in.V, TileT::BM), H, W, (int)p.wd, how, in.target, partial, zt);
+            LAUNCH_TILES((lce_forward_kernel<TileT>), resident<TileT>(tiles_of(in.N, in.V, TileT::BM)), 2 * TileT::STAGE + TileT::WN * TileT::BM * (int)sizeof(float2), H, W, (int)p.wd, how, in.target, partial, zt);
         });
     }
     // (a workgroup for 16 rows reads their pairs in whole lines; few rows over many columns need more of them)
@@ -653,7 +690,7 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
         if (blocks_w + blocks_h) UNFLOW_LAUNCH((pack_transposes_kernel<T, PL, EL>), dim3(blocks_w + blocks_h), dim3(256), 0, stream, wc, hc, blocks_w, ex);
         with_tile<PL, EL>(p.size_g, [&](auto tile) {
             using TileT = decltype(tile);
-            LAUNCH_TILES((lce_gradient_kernel<TileT>), (int)tiles_of(in.N, vp, TileT::BM), H, W, (int)p.wd, how, (const Row*)stats, up, v0, vp, in.V, G, p.wvp, dw ? GT : nullptr, p.wn);
+            LAUNCH_TILES((lce_gradient_kernel<TileT>), (int)tiles_of(in.N, vp, TileT::BM), TileT::LDS, H, W, (int)p.wd, how, (const Row*)stats, up, v0, vp, in.V, G, p.wvp, dw ? GT : nullptr, p.wn);
         });
         Product a{}, b{};
         a.shares = b.shares = 1;
@@ -670,7 +707,7 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
             if (dh) a.tiles = (int)tiles_of(in.N, in.D, TileT::BM);
             if (dw) b.tiles = (int)tiles_of(vp, in.D, TileT::BM);
             const bool swap = dw && (!dh || b.width / b.shares > a.width / a.shares);        // the longer units first
-            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, swap ? b : a, swap ? a : b, (const Exponents*)ex, up);
+            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, 2 * TileT::STAGE, swap ? b : a, swap ? a : b, (const Exponents*)ex, up);
         });
         const bool last = v0 + vp >= in.V;
         const int finish_a = dh && last && a.sums ? blocks_for((long long)in.N * (p.ldc / 4)) : 0, finish_b = dw && b.sums ? blocks_for((long long)vp * (p.ldc / 4)) : 0;

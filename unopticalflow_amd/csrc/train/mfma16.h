@@ -96,6 +96,7 @@ struct Tile {
     static constexpr int STAGE = (BM + BN) * kStageBytes;
     static constexpr int PITCH = BM + 8;                                      // of a row of the transposed tile (store_transposed)
     static constexpr int LDS = 2 * STAGE > BN * PITCH * 2 ? 2 * STAGE : BN * PITCH * 2;
+    static constexpr int PER_CU = BM > 128 ? 1 : BM > 64 ? 2 : 4;             // workgroups that share a CU
     static constexpr int QA = BM / 8 / WAVES, QB = BN / 8 / WAVES;            // 1 KB copies (8 rows) of a wave per stage
     static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0, "a wave copies whole groups of 8 rows");
 
@@ -105,27 +106,49 @@ struct Tile {
     __device__ __forceinline__ static int row(int i) { return (wave() / WN) * TM + i * 16 + ((int)threadIdx.x & 15); }
     __device__ __forceinline__ static int col(int j) { return (wave() % WN) * TN + j * 16 + (((int)threadIdx.x & 63) >> 4) * 4; }
 
-    // k0, k1: the part of the packed width that is summed (k0 a multiple of 64); m0, n0: the tile's corner.  Every wave of the workgroup calls
-    // this with the same arguments; LDS bytes are free for other use after the barrier that ends it.
-    __device__ __forceinline__ void run(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
+    // What the copies need of the tile that is worked on.
+    byte_range range_a, range_b;
+    unsigned at_a, at_b, step_a, step_b;
+    int left;                                                                // packed elements behind the lane's piece of stage 0
+
+    // copy q (of QA + QB) of stage t; a stage behind the last one is all zeros
+    __device__ __forceinline__ void fetch(lds_address lds, int t, int q) const {
+        const lds_address to = lds + (t & 1) * STAGE;
+        const bool in = t * 64 < left;
+        const unsigned adv = (unsigned)t * kStageBytes;
+        const int w = wave();
+        if (q < QA) copy16_to_lds(range_a, to + (w + WAVES * q) * 1024, (in ? at_a : kOutside) + (adv + q * step_a));
+        else copy16_to_lds(range_b, to + BM * kStageBytes + (w + WAVES * (q - QA)) * 1024, (in ? at_b : kOutside) + (adv + (q - QA) * step_b));
+    }
+
+    // Sets the copies of the first two stages of a tile going.  k0, k1: the part of the packed width that is summed (k0 a multiple of 64); m0, n0: the
+    // tile's corner.  Every wave of the workgroup calls this with the same arguments, when nobody uses the stages' LDS any more.
+    __device__ __forceinline__ void start(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
         const int w = wave(), lane = (int)threadIdx.x & 63;
         const int piece = (lane & 7) ^ (((4 * (w & 1)) + (lane >> 4)) & 7);          // of the row 8 q + lane / 8, q = w + WAVES i
-        const int k_piece = piece * 8;
-        // The descriptors end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most 256
-        // rows of at most 2^21 numbers: its bytes stay below 2^31.)
+        // The ranges end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most 256 rows of
+        // at most 2^21 numbers: its bytes stay below 2^31.)
         const int ra = A.rows - m0 < BM ? A.rows - m0 : BM, rb = B.rows - n0 < BN ? B.rows - n0 : BN;
-        const byte_range da = range_of(A.p + (long long)m0 * A.ld, (int)(ra * A.ld * 2));
-        const byte_range db = range_of(B.p + (long long)n0 * B.ld, (int)(rb * B.ld * 2));
-        const unsigned step_a = (unsigned)(8 * WAVES * A.ld * 2), step_b = (unsigned)(8 * WAVES * B.ld * 2);
-        const unsigned at_a = (unsigned)(((8 * w + (lane >> 3)) * A.ld + k0 + k_piece) * 2), at_b = (unsigned)(((8 * w + (lane >> 3)) * B.ld + k0 + k_piece) * 2);
-        // copy q (of QA + QB) of stage t; a stage behind the last one is all zeros
-        auto fetch = [&](int t, int q) {
-            char* to = lds + (t & 1) * STAGE;
-            const bool in = k0 + t * 64 + k_piece < k1;
-            const unsigned adv = (unsigned)t * kStageBytes;
-            if (q < QA) copy16_to_lds(da, to + (w + WAVES * q) * 1024, (in ? at_a : kOutside) + (adv + q * step_a));
-            else copy16_to_lds(db, to + BM * kStageBytes + (w + WAVES * (q - QA)) * 1024, (in ? at_b : kOutside) + (adv + (q - QA) * step_b));
-        };
+        range_a = range_of(A.p + (long long)m0 * A.ld, (int)(ra * A.ld * 2));
+        range_b = range_of(B.p + (long long)n0 * B.ld, (int)(rb * B.ld * 2));
+        step_a = (unsigned)(8 * WAVES * A.ld * 2);
+        step_b = (unsigned)(8 * WAVES * B.ld * 2);
+        at_a = (unsigned)(((8 * w + (lane >> 3)) * A.ld + k0 + piece * 8) * 2);
+        at_b = (unsigned)(((8 * w + (lane >> 3)) * B.ld + k0 + piece * 8) * 2);
+        left = k1 - k0 - piece * 8;
+        stages = (k1 - k0 + 63) / 64;
+        const lds_address to = address_in_lds(lds);
+#pragma unroll
+        for (int q = 0; q < QA + QB; ++q) fetch(to, 0, q);
+#pragma unroll
+        for (int q = 0; q < QA + QB; ++q) fetch(to, 1, q);
+    }
+    int stages;
+
+    // The sums of the tile that was started.  The stages' LDS is free after the barrier that ends this.
+    __device__ __forceinline__ void finish(char* lds) {
+        const int w = wave(), lane = (int)threadIdx.x & 63;
+        const lds_address lds0 = address_in_lds(lds);
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -140,7 +163,6 @@ struct Tile {
         // row of the wave's part: issued together they would fill their queues and hold up the wave.  No wave waits for LDS or memory but at
         // the one barrier of a stage, by which its reads of stage t have arrived, its copies of stage t + 1 are in LDS (they had a whole stage),
         // and the buffer of stage t may be written again.
-        const int stages = (k1 - k0 + 63) / 64;
         uint4 a0[MI], b0[NI], a1[MI], b1[NI];
         constexpr int READS = MI + NI, EACH_READ = (READS + MI - 2) / (MI - 1), EACH_COPY = (QA + QB + MI - 1) / MI;
         auto read = [&](uint4* a, uint4* b, const char* s, int p, int r) {                      // read r of READS
@@ -151,12 +173,8 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(b[j], a[i], acc[i][j]);
         };
-#pragma unroll
-        for (int q = 0; q < QA + QB; ++q) fetch(0, q);
-        UNFLOW_WAIT_VMCNT0();
+        vm_wait<QA + QB>();                           // (what a wave issues arrives in order: all but the copies of stage 1, or what was issued behind them)
         __builtin_amdgcn_s_barrier();
-#pragma unroll
-        for (int q = 0; q < QA + QB; ++q) fetch(1, q);
 #pragma unroll
         for (int r = 0; r < READS; ++r) read(a0, b0, lds, p0, r);
         for (int t = 0; t < stages; ++t) {
@@ -182,7 +200,7 @@ struct Tile {
             for (int i = 0; i < MI; ++i) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int q = i * EACH_COPY; q < (i + 1) * EACH_COPY && q < QA + QB; ++q) fetch(t + 2, q);
+                for (int q = i * EACH_COPY; q < (i + 1) * EACH_COPY && q < QA + QB; ++q) fetch(lds0, t + 2, q);
 #pragma unroll
                 for (int r = i * EACH_READ; r < (i + 1) * EACH_READ && r < READS; ++r) read(a0, PL == TWO ? b1 : b0, next, p0, r);
                 multiply(a1, PL == TWO ? b0 : b1, i);
@@ -194,6 +212,10 @@ struct Tile {
         }
         UNFLOW_WAIT_VMCNT0();
         __syncthreads();
+    }
+    __device__ __forceinline__ void run(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
+        start(A, B, k0, k1, m0, n0, lds);
+        finish(lds);
     }
 
     // The transpose of the tile, value(i, j) being the four numbers that belong to acc[i][j], into packed rows: dst row n holds the numbers of

@@ -27,8 +27,8 @@ static int stages_of(long long packed_width_) { return (int)((packed_width_ + 63
 static long long tiles_of(long long m, long long n, int size) { return ((m + size - 1) / size) * ((n + size - 1) / size); }
 static long long lower_tiles_of(long long m, int size) { const long long t = (m + size - 1) / size; return t * (t + 1) / 2; }
 
-// Measured: microseconds of one stage of a unit on a full chip (of the units that share a CU, together) and on one that is not, and of a unit's
-// start and end.  (8192 x 8192 x 2048 and 1024 x 1024 x 4096, ONE and TWO planes)
+// Measured: microseconds of one stage of a unit on a full chip (of the units that share a CU, together) and on an empty one (a chip is as slow as a
+// full one from 60 % on), and of a unit's start and end.  (8192 x 8192 x 2048 and 1024 x 1024 x 4096, ONE and TWO planes)
 struct Cost { double full, alone, ends; int per_cu; };
 static const Cost kCost[2][4] = {{{1.43, 1.10, 10., 1}, {1.00, 0.75, 7., 1}, {1.00, 0.60, 6., 2}, {0.75, 0.46, 4., 4}},
                                  {{2.05, 1.45, 10., 1}, {1.17, 0.87, 7., 1}, {1.15, 0.56, 6., 2}, {0.80, 0.40, 4., 4}}};
@@ -47,23 +47,27 @@ static Choice choose(int planes, const Job* jobs, int count) {
         for (int s = 1; s <= 16; s = s < 4 ? s + 1 : s < 8 ? s + 2 : s + 4) {
             const int limit = (longest + s - 1) / s;
             if (s > 1 && (!any || limit < 4)) break;
-            double most = 0., least = 1e30, sum = 0., count_ = 0., joined = 0.;      // microseconds of a unit on a full chip, and of all of them
-            int stages = 1;                                                // of the longest
+            int most = 0, least = 1 << 30;                                 // stages of a unit
+            double sum = 0., joined = 0.;
             for (int i = 0; i < count; ++i) {
                 const int shares = jobs[i].cut ? shares_of(jobs[i].stages, limit) : 1, each = (jobs[i].stages + shares - 1) / shares;
-                const double tiles = (double)jobs[i].times * (jobs[i].lower ? lower_tiles_of(jobs[i].m, kSizes[z]) : tiles_of(jobs[i].m, jobs[i].n, kSizes[z]));
-                const double us = each * c.full + c.ends;
-                most = us > most ? us : most;
-                least = us < least ? us : least;
-                stages = each > stages ? each : stages;
-                sum += tiles * shares * us;
-                count_ += tiles * shares;
-                if (shares > 1) joined += tiles * shares * kSizes[z] * kSizes[z] * 8.;
+                const double units = (double)jobs[i].times * (jobs[i].lower ? lower_tiles_of(jobs[i].m, kSizes[z]) : tiles_of(jobs[i].m, jobs[i].n, kSizes[z])) * shares;
+                most = each > most ? each : most;
+                least = each < least ? each : least;
+                sum += units * (each * c.full + c.ends);
+                if (shares > 1) joined += units * kSizes[z] * kSizes[z] * 8.;
             }
-            // every CU busy to the end but for a part of the shortest unit; the longest are started first
-            double us = ceil(sum / (256. * c.per_cu) / least - 1e-9) * least;
-            us = us > most ? us : most;
-            if (count_ <= 256.) us = stages * c.alone + c.ends;
+            const double slots = 256. * c.per_cu, unit = most * c.full + c.ends, units = sum / unit;      // (in units of the longest)
+            auto last = [&](double n) {                                    // the longest unit among n that run together, n <= slots
+                const double busy = 1.6 * n / slots;
+                return most * (c.alone + (c.full - c.alone) * (busy < 1. ? busy : 1.)) + c.ends;
+            };
+            double us;
+            if (units <= slots) us = last(units);
+            else if (least == most) {
+                const double rounds = floor(units / slots), rest = units - rounds * slots;
+                us = rounds * unit + (rest > 0.5 ? last(rest) : 0.);
+            } else us = units / slots * unit + 0.5 * (least * c.full + c.ends);                          // the short ones fill up
             us += joined > 0. ? kLaunchUs + joined / kJoinBytesPerUs : 0.;
             if (best.us < 0. || us < best.us) best = Choice{z, limit, us};
         }
