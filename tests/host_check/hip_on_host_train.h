@@ -15,6 +15,16 @@ static inline unsigned long long __ballot(int p) {
     __syncthreads();
     return hip_on_host::ballots[wave];
 }
+static inline int hip_on_host_readlane(int v, int lane) {
+    static int values[1024];
+    __syncthreads();
+    values[hip_on_host::lane_id] = v;
+    __syncthreads();
+    const int r = values[(hip_on_host::lane_id & ~63u) + (unsigned)lane];
+    __syncthreads();
+    return r;
+}
+#define __builtin_amdgcn_readlane(v, lane) hip_on_host_readlane(v, lane)
 static inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 
 // v_mfma_f32_16x16x32_f16: the lane layouts of the bf16 form (hip_on_host.h)

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
                                                                                                     const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(W.rows, TileT::BN), total = mt * nt;
-    float2* rows = reinterpret_cast<float2*>(lds + 2 * TileT::STAGE);                    // [WN][BM]
+    float2* rows = reinterpret_cast<float2*>(lds + TileT::STAGES_LDS);                    // [WN][BM]
     const int wn = TileT::wave() % TileT::WN, group = ((int)threadIdx.x & 63) >> 4;
     int id = (int)blockIdx.x, tm, tn;
     tile_of(xcd_remap(id, total), mt, nt, tm, tn);
@@ -417,8 +417,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
 }
 
 template <class TileT> struct OutputOf { using type = __bf16; };
-template <int BM, int BN, int WM, int WN> struct OutputOf<Tile<BM, BN, WM, WN, ONE, FP16>> { using type = _Float16; };
-template <int BM, int BN, int WM, int WN> struct OutputOf<Tile<BM, BN, WM, WN, TWO, FP16>> { using type = float; };
+template <int BM, int BN, int WM, int WN, int DP> struct OutputOf<Tile<BM, BN, WM, WN, DP, ONE, FP16>> { using type = _Float16; };
+template <int BM, int BN, int WM, int WN, int DP> struct OutputOf<Tile<BM, BN, WM, WN, DP, TWO, FP16>> { using type = float; };
 
 // The two products of a piece, one launch: job 0 is dH += G W, job 1 dW = G^T H.  C = A B^T in `shares` shares of what is summed.  A job without
 // `sums` is one share and goes to the gradient as it is; else the shares' accumulators go to fp32 sums [shares][rows of A][ldc], added to what
@@ -512,10 +512,12 @@ __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, i
 // workgroups of a kernel that goes through its tiles itself
 template <class TileT> static int resident(long long units) { return (int)(units < 256 * TileT::PER_CU ? units : 256 * TileT::PER_CU); }
 template <int PL, int EL, class F> static void with_tile(int size, F&& f) {
-    if (size == 0) f(Tile<256, 256, 2, 4, PL, EL>{});
-    else if (size == 1) f(Tile<192, 192, 2, 4, PL, EL>{});
-    else if (size == 2) f(Tile<128, 128, 2, 2, PL, EL>{});
-    else f(Tile<64, 64, 2, 2, PL, EL>{});
+    if (size == 0) f(Tile<256, 256, 2, 4, 2, PL, EL>{});
+    else if (size == 1) f(Tile<192, 192, 2, 4, 3, PL, EL>{});
+    else if (size == 2) f(Tile<128, 128, 2, 2, 2, PL, EL>{});
+    else if (size == 3) f(Tile<64, 64, 2, 2, 2, PL, EL>{});
+    else if (size == 4) f(Tile<128, 128, 2, 2, 4, PL, EL>{});
+    else f(Tile<64, 64, 2, 2, 4, PL, EL>{});
 }
 
 // What a call needs of its buffers, and where.  `kept`: what the forward pass leaves for the backward pass.
@@ -563,7 +565,7 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
     const long long packed = at;
     p.kept_bytes = p.keeps ? packed : bare;
     at = 0;
-    const Job z{N, V, stages_of(p.wd), false, false};
+    const Job z{N, V, stages_of(p.wd), false, false, 0.};
     p.size_z = choose(p.planes, &z, 1).size;
     p.partial = take(8ll * ceil_div(V, p.few ? few_classes(N) : kSizes[p.size_z]) * N);
     p.ztarget = take(4ll * N);
@@ -582,12 +584,12 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
     vp = round_up((V + pieces - 1) / pieces, 256);                       // equal pieces
     p.vp = (int)(vp < V ? vp : V);
     p.wvp = packed_width(p.planes, p.vp);
-    const Job g{N, p.vp, stages_of(p.wd), false, false};
+    const Job g{N, p.vp, stages_of(p.wd), false, false, 4. * p.planes};
     p.size_g = choose(p.planes, &g, 1).size;
     Job both[2];
     int jobs = 0;
-    if (need_h) both[jobs++] = Job{N, D, stages_of(p.wvp), false, true};
-    if (need_w) both[jobs++] = Job{p.vp, D, stages_of(p.wn), false, true};
+    if (need_h) both[jobs++] = Job{N, D, stages_of(p.wvp), false, true, p.vp < V ? 8. : 2. * p.planes};
+    if (need_w) both[jobs++] = Job{p.vp, D, stages_of(p.wn), false, true, 2. * p.planes};
     if (jobs) {
         const Choice c = choose(p.planes, both, jobs);
         p.size_p = c.size;
@@ -653,7 +655,7 @@ static void forward(const Plan& p, const Inputs& in, int reduction, float* loss,
         columns = ceil_div(in.V, kSizes[p.size_z]);
         with_tile<PL, EL>(p.size_z, [&](auto tile) {
             using TileT = decltype(tile);
-            LAUNCH_TILES((lce_forward_kernel<TileT>), resident<TileT>(tiles_of(in.N, in.V, TileT::BM)), 2 * TileT::STAGE + TileT::WN * TileT::BM * (int)sizeof(float2), H, W, (int)p.wd, how, in.target, partial, zt);
+            LAUNCH_TILES((lce_forward_kernel<TileT>), resident<TileT>(tiles_of(in.N, in.V, TileT::BM)), TileT::STAGES_LDS + TileT::WN * TileT::BM * (int)sizeof(float2), H, W, (int)p.wd, how, in.target, partial, zt);
         });
     }
     // (a workgroup for 16 rows reads their pairs in whole lines; few rows over many columns need more of them)
@@ -707,7 +709,7 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
             if (dh) a.tiles = (int)tiles_of(in.N, in.D, TileT::BM);
             if (dw) b.tiles = (int)tiles_of(vp, in.D, TileT::BM);
             const bool swap = dw && (!dh || b.width / b.shares > a.width / a.shares);        // the longer units first
-            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, 2 * TileT::STAGE, swap ? b : a, swap ? a : b, (const Exponents*)ex, up);
+            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, TileT::STAGES_LDS, swap ? b : a, swap ? a : b, (const Exponents*)ex, up);
         });
         const bool last = v0 + vp >= in.V;
         const int finish_a = dh && last && a.sums ? blocks_for((long long)in.N * (p.ldc / 4)) : 0, finish_b = dw && b.sums ? blocks_for((long long)vp * (p.ldc / 4)) : 0;

@@ -89,14 +89,15 @@ constexpr unsigned kOutside = 0x80000000u;            // an offset outside every
 // A workgroup of WM x WN waves owns a BM x BN tile; a wave owns (BM / WM) x (BN / WN) of it.  acc[i][j] belongs to the wave's rows
 // 16 i .. and columns 16 j ..; a lane holds row m = 16 i + (lane & 15) and the four columns n = 16 j + 4 (lane >> 4) ..  (the operands go to
 // the instruction in the order B, A, so that the four values a lane holds are neighbours in a row of C).
-template <int BM_, int BN_, int WM_, int WN_, int PL_, int EL_>
+template <int BM_, int BN_, int WM_, int WN_, int DEPTH_, int PL_, int EL_>
 struct Tile {
+    static constexpr int DEPTH = DEPTH_;                                     // stages in LDS
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PL = PL_, EL = EL_;
     static constexpr int WAVES = WM * WN, THREADS = WAVES * 64, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
     static constexpr int STAGE = (BM + BN) * kStageBytes;
     static constexpr int PITCH = BM + 8;                                      // of a row of the transposed tile (store_transposed)
-    static constexpr int LDS = 2 * STAGE > BN * PITCH * 2 ? 2 * STAGE : BN * PITCH * 2;
-    static constexpr int PER_CU = BM > 128 ? 1 : BM > 64 ? 2 : 4;             // workgroups that share a CU
+    static constexpr int STAGES_LDS = DEPTH * STAGE, LDS = STAGES_LDS > BN * PITCH * 2 ? STAGES_LDS : BN * PITCH * 2;
+    static constexpr int PER_CU = STAGES_LDS > 80 * 1024 ? 1 : STAGES_LDS > 40 * 1024 ? 2 : 4;               // workgroups that share a CU
     static constexpr int QA = BM / 8 / WAVES, QB = BN / 8 / WAVES;            // 1 KB copies (8 rows) of a wave per stage
     static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0, "a wave copies whole groups of 8 rows");
 
@@ -111,9 +112,8 @@ struct Tile {
     unsigned at_a, at_b, step_a, step_b;
     int left;                                                                // packed elements behind the lane's piece of stage 0
 
-    // copy q (of QA + QB) of stage t; a stage behind the last one is all zeros
-    __device__ __forceinline__ void fetch(lds_address lds, int t, int q) const {
-        const lds_address to = lds + (t & 1) * STAGE;
+    // copy q (of QA + QB) of stage t to the buffer `to`; a stage behind the last one is all zeros
+    __device__ __forceinline__ void fetch(lds_address to, int t, int q) const {
         const bool in = t * 64 < left;
         const unsigned adv = (unsigned)t * kStageBytes;
         const int w = wave();
@@ -121,7 +121,7 @@ struct Tile {
         else copy16_to_lds(range_b, to + BM * kStageBytes + (w + WAVES * (q - QA)) * 1024, (in ? at_b : kOutside) + (adv + (q - QA) * step_b));
     }
 
-    // Sets the copies of the first two stages of a tile going.  k0, k1: the part of the packed width that is summed (k0 a multiple of 64); m0, n0: the
+    // Sets the copies of the first stages of a tile going.  k0, k1: the part of the packed width that is summed (k0 a multiple of 64); m0, n0: the
     // tile's corner.  Every wave of the workgroup calls this with the same arguments, when nobody uses the stages' LDS any more.
     __device__ __forceinline__ void start(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
         const int w = wave(), lane = (int)threadIdx.x & 63;
@@ -139,9 +139,9 @@ struct Tile {
         stages = (k1 - k0 + 63) / 64;
         const lds_address to = address_in_lds(lds);
 #pragma unroll
-        for (int q = 0; q < QA + QB; ++q) fetch(to, 0, q);
+        for (int t = 0; t < DEPTH; ++t)
 #pragma unroll
-        for (int q = 0; q < QA + QB; ++q) fetch(to, 1, q);
+            for (int q = 0; q < QA + QB; ++q) fetch(to + t * STAGE, t, q);
     }
     int stages;
 
@@ -161,7 +161,8 @@ struct Tile {
 
         // The operand reads of one half of a stage and the copies of the stage after the next run under the matrix instructions, a few behind every
         // row of the wave's part: issued together they would fill their queues and hold up the wave.  No wave waits for LDS or memory but at
-        // the one barrier of a stage, by which its reads of stage t have arrived, its copies of stage t + 1 are in LDS (they had a whole stage),
+        // the one barrier of a stage, by which its reads of stage t have arrived, its copies of stage t + 1 are in LDS (they had DEPTH - 1
+        // stages' time),
         // and the buffer of stage t may be written again.
         uint4 a0[MI], b0[NI], a1[MI], b1[NI];
         constexpr int READS = MI + NI, EACH_READ = (READS + MI - 2) / (MI - 1), EACH_COPY = (QA + QB + MI - 1) / MI;
@@ -173,13 +174,16 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<EL>(b[j], a[i], acc[i][j]);
         };
-        vm_wait<QA + QB>();                           // (what a wave issues arrives in order: all but the copies of stage 1, or what was issued behind them)
+        // (what a wave issues arrives in order: all but the copies of the stages behind this one, or what was issued behind them)
+        vm_wait<(DEPTH - 1) * (QA + QB)>();
         __builtin_amdgcn_s_barrier();
 #pragma unroll
         for (int r = 0; r < READS; ++r) read(a0, b0, lds, p0, r);
+        int here = 0;                                                        // the buffer of stage t
         for (int t = 0; t < stages; ++t) {
-            const char* s = lds + (t & 1) * STAGE;
-            const char* next = lds + (~t & 1) * STAGE;
+            const int there = here + STAGE == STAGES_LDS ? 0 : here + STAGE;
+            const char* s = lds + here;
+            const char* next = lds + there;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -194,13 +198,13 @@ struct Tile {
             }
             __builtin_amdgcn_sched_barrier(0);
             UNFLOW_WAIT_LGKMCNT0();
-            UNFLOW_WAIT_VMCNT0();
+            vm_wait<(DEPTH - 2) * (QA + QB)>();
             __builtin_amdgcn_s_barrier();
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int q = i * EACH_COPY; q < (i + 1) * EACH_COPY && q < QA + QB; ++q) fetch(lds0, t + 2, q);
+                for (int q = i * EACH_COPY; q < (i + 1) * EACH_COPY && q < QA + QB; ++q) fetch(lds0 + here, t + DEPTH, q);
 #pragma unroll
                 for (int r = i * EACH_READ; r < (i + 1) * EACH_READ && r < READS; ++r) read(a0, PL == TWO ? b1 : b0, next, p0, r);
                 multiply(a1, PL == TWO ? b0 : b1, i);
@@ -209,6 +213,7 @@ struct Tile {
 #pragma unroll
                 for (int j = 0; j < NI; ++j) b0[j] = b1[j];
             }
+            here = there;
         }
         UNFLOW_WAIT_VMCNT0();
         __syncthreads();

@@ -50,34 +50,38 @@ __global__ __launch_bounds__(256) void write_table_kernel(Words src, int count, 
     for (int i = threadIdx.x; i < count; i += 256) dst[i] = src.w[i];
 }
 
-// the problem that work item `id` of a phase belongs to, and the item's number within it; e: this lane's running count if one load holds them all
-__device__ __forceinline__ int count_before(const int* __restrict__ ends, int count, int e, int id) {
-    if (count <= 64) return __popcll(__ballot(e <= id));
+// How many of the first `count` running counts are at most id.
+__device__ __forceinline__ int counts_until(const int* __restrict__ ends, int count, int id) {
     int at = 0;
     for (int base = 0; base < count; base += 64) {
         const int lane = base + ((int)threadIdx.x & 63), before = __popcll(__ballot((lane < count ? ends[lane] : 0x7fffffff) <= id));
         at += before;
         if (before < 64) break;
     }
-    return at;
+    return __builtin_amdgcn_readfirstlane(at);
 }
-__device__ __forceinline__ int lane_end(const int* __restrict__ ends, int count) {
-    const int lane = (int)threadIdx.x & 63;
-    return lane < count ? ends[lane] : 0x7fffffff;
-}
+// the problem that work item `id` of a phase belongs to, and the item's number within it
 __device__ __forceinline__ int problem_of(const int* __restrict__ ends, int count, int id, int& local) {
-    const int at = __builtin_amdgcn_readfirstlane(count_before(ends, count, lane_end(ends, count), id));
+    const int at = counts_until(ends, count, id);
     local = id - (at > 0 ? ends[at - 1] : 0);
     return at;
 }
 // The same for the product phases.  Work items are sorted by length, the longest first; the matrices of one length are dealt over the XCDs by
-// themselves, so that every XCD has its share of the long ones and a matrix stays in one L2 as far as it goes.
+// themselves, so that every XCD has its share of the long ones and a matrix stays in one L2 as far as it goes.  Up to 64 matrices every lane holds
+// one's counts and the search waits for memory once (a launch over small matrices is all latency: 0.5 us for every load that waits for another).
 __device__ __forceinline__ int dealt_problem_of(const int* __restrict__ ends, int count, const int* __restrict__ classes, int& local) {
-    const int e = lane_end(ends, count), at = __builtin_amdgcn_readfirstlane(count_before(ends, count, e, (int)blockIdx.x));
-    const int first = classes[2 * at], end = classes[2 * at + 1], id = first + xcd_remap((int)blockIdx.x - first, end - first);
-    const int mine = __builtin_amdgcn_readfirstlane(count_before(ends, count, e, id));
-    local = id - (mine > 0 ? ends[mine - 1] : 0);
-    return mine;
+    if (count <= 64) {
+        const int lane = (int)threadIdx.x & 63, mine = lane < count ? lane : count - 1;
+        const int e = lane < count ? ends[mine] : 0x7fffffff, first = classes[2 * mine], end = classes[2 * mine + 1];
+        const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(e <= (int)blockIdx.x)));
+        const int f = __builtin_amdgcn_readlane(first, at), id = f + xcd_remap((int)blockIdx.x - f, __builtin_amdgcn_readlane(end, at) - f);
+        const int owner = __builtin_amdgcn_readfirstlane(__popcll(__ballot(e <= id)));
+        const int before = __builtin_amdgcn_readlane(e, owner > 0 ? owner - 1 : 0);
+        local = id - (owner > 0 ? before : 0);
+        return owner;
+    }
+    const int at = counts_until(ends, count, (int)blockIdx.x), first = classes[2 * at], end = classes[2 * at + 1];
+    return problem_of(ends, count, first + xcd_remap((int)blockIdx.x - first, end - first), local);
 }
 
 __device__ __forceinline__ float direction(float g, float m, float mu, int nesterov) { return nesterov ? g + mu * (m - g) : m; }
@@ -346,10 +350,12 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem*
 
 // ---- the host side
 template <class F> static void with_tile(int size, F&& f) {
-    if (size == 0) f(Tile<256, 256, 2, 4, TWO, FP16>{});
-    else if (size == 1) f(Tile<192, 192, 2, 4, TWO, FP16>{});
-    else if (size == 2) f(Tile<128, 128, 2, 2, TWO, FP16>{});
-    else f(Tile<64, 64, 2, 2, TWO, FP16>{});
+    if (size == 0) f(Tile<256, 256, 2, 4, 2, TWO, FP16>{});
+    else if (size == 1) f(Tile<192, 192, 2, 4, 3, TWO, FP16>{});
+    else if (size == 2) f(Tile<128, 128, 2, 2, 2, TWO, FP16>{});
+    else if (size == 3) f(Tile<64, 64, 2, 2, 2, TWO, FP16>{});
+    else if (size == 4) f(Tile<128, 128, 2, 2, 4, TWO, FP16>{});
+    else f(Tile<64, 64, 2, 2, 4, TWO, FP16>{});
 }
 
 // Bounds of |X|, |S|, |Q| (spectral norms: every singular value of X_0 is in [0, 1]) over all steps, as powers of two that keep the planes
@@ -417,8 +423,8 @@ static Group lay_out(const unflow_matrix* a, int first, int count, Problem* prob
     g.count = count;
     long long at = 0, chunks = 0;
     auto take = [&](long long bytes) { const long long p = at; at += round_up(bytes, 256); return p; };
-    g.table = take((long long)sizeof(Problem) * count);
-    g.ends = take(4ll * kTables * count);
+    g.table = take(((long long)sizeof(Problem) + 4 * kTables) * count);
+    g.ends = g.table + (long long)sizeof(Problem) * count;
     // matrices of one shape are one job of the model
     auto plan = [&](auto job_of) {
         int k = 0;
@@ -431,10 +437,10 @@ static Group lay_out(const unflow_matrix* a, int first, int count, Problem* prob
         }
         return choose(TWO, jobs, k);
     };
-    const Choice cs = plan([](long long m, long long n) { return Job{m, m, stages_of(packed_width(TWO, n)), true, true}; });
+    const Choice cs = plan([](long long m, long long n) { return Job{m, m, stages_of(packed_width(TWO, n)), true, true, 8.}; });
     g.size_s = cs.size;
-    g.size_q = plan([](long long m, long long n) { return Job{m, m, stages_of(packed_width(TWO, m)), true, false}; }).size;
-    g.size_x = plan([](long long m, long long n) { return Job{m, n, stages_of(packed_width(TWO, m)), false, false}; }).size;
+    g.size_q = plan([](long long m, long long n) { return Job{m, m, stages_of(packed_width(TWO, m)), true, false, 8.}; }).size;
+    g.size_x = plan([](long long m, long long n) { return Job{m, n, stages_of(packed_width(TWO, m)), false, false, 8.}; }).size;
     long long numbers = 0;
     for (int i = 0; i < count; ++i) numbers += (long long)order.m[i] * order.n[i];
     g.chunk = numbers < (16 << 20) ? 4096 : 16384;
@@ -572,11 +578,9 @@ static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca
     char* ws = (char*)workspace;
     for (int i = 0; i < count;) {
         const int e = group_end(a, count, i), n = e - i;
-        static thread_local Problem problems[kMost];
-        static thread_local int ends[kMost * kTables];
-        const Group g = lay_out(a, i, n, problems, ends);
-        write_table(problems, (long long)sizeof(Problem) * n, ws + g.table, stream);
-        write_table(ends, 4ll * kTables * n, ws + g.ends, stream);
+        static thread_local struct alignas(8) { char bytes[kMost * (sizeof(Problem) + 4 * kTables)]; } table;
+        const Group g = lay_out(a, i, n, (Problem*)table.bytes, (int*)(table.bytes + sizeof(Problem) * n));
+        write_table(table.bytes, (sizeof(Problem) + 4ll * kTables) * n, ws + g.table, stream);
         if (dtype == kFp32) iterate<float, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else if (dtype == kBf16) iterate<__bf16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else iterate<_Float16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
