@@ -536,6 +536,23 @@ def test_refusals_of_muon_step():
         assert all(torch.equal(a, b) for a, b in zip(params + momenta, kept))
     with pytest.raises(ValueError):
         optim.FlowMuon([])
+    opt = optim.FlowMuon([torch.nn.Parameter(torch.zeros(3, 4))])
+    with pytest.raises(ValueError):
+        opt.add_param_group({'params': [torch.nn.Parameter(torch.zeros(4))]})
+
+
+def test_flow_muon_groups(device):
+    """A group of its own step size, and a schedule on both: the weights move by lr sqrt(max(1, rows / cols)) times the same matrix."""
+    g = torch.Generator().manual_seed(0)
+    a, b = (torch.nn.Parameter(torch.randn(12, 20, generator=g).to(device)) for _ in range(2))
+    a.grad, b.grad = torch.randn(12, 20, generator=g).to(device), torch.randn(12, 20, generator=g).to(device)
+    opt = optim.FlowMuon([a], lr=0.25, momentum=0.0)
+    opt.add_param_group({'params': [b], 'lr': 0.5})
+    opt.param_groups[0]['lr'] = 0.125
+    before = [p.detach().clone() for p in (a, b)]
+    opt.step()
+    for p, old, lr in zip((a, b), before, (0.125, 0.5)):
+        assert torch.allclose((old - p.detach()) / lr, ops.orthogonalize(p.grad), rtol=0, atol=16 * 2**-24 * 4 / lr + 2**-20)
 
 
 class _Head(torch.nn.Module):
@@ -599,7 +616,7 @@ def test_loss_and_optimiser_together():
     for a, b in zip(losses[1:], want[1:]):
         assert abs(float(a - b)) <= 2**-9 * float(b)
     for p, q in zip(model.parameters(), exact.parameters()):
-        assert float((p.double() - q).norm()) <= 3 * 0.02 * 2**-9 * math.sqrt(p.numel()) + 2**-20 * float(q.norm())
+        assert float((p.detach().double() - q.detach()).norm()) <= 3 * 0.02 * 2**-9 * math.sqrt(p.numel()) + 2**-20 * float(q.detach().norm())
 
 
 @pytest.mark.gpu

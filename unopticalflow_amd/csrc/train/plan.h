@@ -34,7 +34,7 @@ static long long lower_tiles_of(long long m, int size) { const long long t = (m 
 // 1024 x 1024 x 4096; ONE and TWO planes)
 struct Cost { double full, alone, ends; int per_cu; };
 static const Cost kCost[2][kVariants] = {{{1.50, 1.10, 10., 1}, {0.97, 0.68, 7., 1}, {1.10, 0.62, 5., 2}, {0.80, 0.46, 4., 4}, {0.53, 0.45, 5., 1}, {0.35, 0.26, 4., 2}},
-                                         {{2.15, 1.50, 12., 1}, {1.28, 0.95, 9., 1}, {1.25, 0.60, 6., 2}, {0.83, 0.44, 4., 4}, {0.64, 0.54, 6., 1}, {0.44, 0.28, 4., 2}}};
+                                         {{2.15, 1.50, 18., 1}, {1.28, 0.95, 11., 1}, {1.25, 0.60, 7.5, 2}, {0.83, 0.44, 4.8, 4}, {0.64, 0.54, 7.5, 1}, {0.44, 0.28, 4.5, 2}}};
 constexpr double kJoinBytesPerUs = 3.0e6, kLaunchUs = 5.0, kStoreBytesPerUs = 4.5e6 / 256.;          // joining: the chip; stores: a CU's part of it
 
 static Choice choose(int planes, const Job* jobs, int count) {

@@ -1801,36 +1801,37 @@ def _rows_of(t):
     return t, t.shape[1]
 
 
+def _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, need_h, need_w):
+    """-> loss, and what the backward pass takes: (hidden, weight, kept) and (ldh, ldw, dtype, bytes of its workspace)."""
+    dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
+    (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
+    (N, D), V = hidden.shape, weight.shape[0]
+    loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
+    if N == 0:
+        return loss.zero_(), (hidden, weight, None), (ldh, ldw, dtype, 0)
+    with _on(dev):
+        sizes = (ctypes.c_longlong * 3)()                # bytes kept for the backward pass, of the forward's workspace, of the backward's
+        at, ph, pw = ctypes.addressof(sizes), hidden.data_ptr(), weight.data_ptr()
+        _call('unflow_linear_ce_workspace', ph, ldh, pw, ldw, N, V, D, dtype, need_h, need_w, at, at + 8, at + 16)
+        kept = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
+        ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
+        _call('unflow_linear_ce_fwd', ph, ldh, pw, ldw, target.data_ptr(), N, V, D, dtype, scale, ignore_index, reduction,
+              loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), sizes[1], _stream_of(dev), nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+    return loss, (hidden, weight, kept), (ldh, ldw, dtype, sizes[2])
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, scale, reduction):
-        dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
-        (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
-        (N, D), V = hidden.shape, weight.shape[0]
-        loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
-        need_h, need_w = ctx.needs_input_grad[:2]
-        if N == 0:
-            ctx.how = (ignore_index, scale, reduction, ldh, ldw, dtype, 0)
-            ctx.save_for_backward(hidden, weight, target, None)
-            return loss.zero_()
-        with _on(dev):
-            sizes = (ctypes.c_longlong * 3)()            # bytes kept for the backward pass, of the forward's workspace, of the backward's
-            at = ctypes.addressof(sizes)
-            _call('unflow_linear_ce_workspace', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, N, V, D, dtype, need_h, need_w, at, at + 8, at + 16)
-            kept = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
-            ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
-            _call('unflow_linear_ce_fwd', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), N, V, D, dtype, scale, ignore_index,
-                  reduction, loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), sizes[1], _stream_of(dev),
-                  nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
-        if need_h or need_w:
-            ctx.how = (ignore_index, scale, reduction, ldh, ldw, dtype, sizes[2])
-            ctx.save_for_backward(hidden, weight, target, kept)
+        loss, (hidden, weight, kept), ctx.how = _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, *ctx.needs_input_grad[:2])
+        ctx.options = (ignore_index, scale, reduction)
+        ctx.save_for_backward(hidden, weight, target, kept)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         hidden, weight, target, kept = ctx.saved_tensors
-        ignore_index, scale, reduction, ldh, ldw, dtype, need = ctx.how
+        (ignore_index, scale, reduction), (ldh, ldw, dtype, need) = ctx.options, ctx.how
         need_h, need_w = ctx.needs_input_grad[:2]
         (N, D), V, dev = hidden.shape, weight.shape[0], hidden.device
         dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if need_h else None
@@ -1860,18 +1861,26 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
     Between the passes 16 bytes per row are kept, and for fp32 inputs (or rows that are not multiples of 16 bytes) a packed copy of both."""
     if reduction not in _REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got {!r}".format(reduction))
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
-        raise ValueError('linear_cross_entropy: hidden [..., D] and weight [V, D] do not fit: {} vs {}'.format(tuple(hidden.shape), tuple(weight.shape)))
-    if target.shape != hidden.shape[:-1] or target.dtype != torch.int64:
-        raise ValueError('linear_cross_entropy: target must be int64 of shape {}, got {} {}'.format(tuple(hidden.shape[:-1]), target.dtype, tuple(target.shape)))
+    shape, wshape = hidden.shape, weight.shape
+    if len(shape) < 1 or len(wshape) != 2 or shape[-1] != wshape[1]:
+        raise ValueError('linear_cross_entropy: hidden [..., D] and weight [V, D] do not fit: {} vs {}'.format(tuple(shape), tuple(wshape)))
+    if target.shape != shape[:-1] or target.dtype != torch.int64:
+        raise ValueError('linear_cross_entropy: target must be int64 of shape {}, got {} {}'.format(tuple(shape[:-1]), target.dtype, tuple(target.shape)))
     if target.device != hidden.device:
         raise RuntimeError('operands on different devices: %s vs %s' % (hidden.device, target.device))
-    if weight.shape[0] < 1 or not 1 <= weight.shape[1] <= _LCE_MAX_DIM or target.numel() > _LCE_MAX_ROWS or weight.shape[0] >= 1 << 31:
+    if wshape[0] < 1 or not 1 <= wshape[1] <= _LCE_MAX_DIM or target.numel() > _LCE_MAX_ROWS or wshape[0] >= 1 << 31:
         raise ValueError('linear_cross_entropy: at least one class, 1 to {} dimensions and at most {} rows; got {} rows, weight {}'.format(
-            _LCE_MAX_DIM, _LCE_MAX_ROWS, target.numel(), tuple(weight.shape)))
-    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]) if hidden.dim() != 2 else hidden, weight, target.reshape(-1).contiguous(),
-                                     int(ignore_index), float(scale), _REDUCTIONS[reduction])
-    return loss.view(target.shape) if reduction == 'none' else loss
+            _LCE_MAX_DIM, _LCE_MAX_ROWS, target.numel(), tuple(wshape)))
+    if len(shape) != 2:
+        hidden, flat = hidden.reshape(-1, shape[-1]), target.reshape(-1)
+    else:
+        flat = target
+    args = (hidden, weight, flat.contiguous(), int(ignore_index), float(scale), _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(*args)
+    else:
+        loss = _linear_ce_forward(*args, False, False)[0]
+    return loss.view(shape[:-1]) if reduction == 'none' and len(shape) != 2 else loss
 
 
 class _Matrix(ctypes.Structure):

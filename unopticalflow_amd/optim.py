@@ -212,7 +212,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
 class FlowMuon(torch.optim.Optimizer):
     """Muon for the weights of two or more dimensions (``muon_step_``), Adam (``FlowAdam``) for everything else.
 
-    Two parameter groups: 'matrices' (``lr``, ``momentum``, ``nesterov``, ``weight_decay``) and 'others' (``adam_lr``, betas, eps).  Momentum
+    ``params`` is a list of parameters; it becomes two groups: 'matrices' (``lr``, ``momentum``, ``nesterov``, ``weight_decay``) and 'others' (``adam_lr``, betas, eps).  Momentum
     is kept in fp32 whatever the parameters' type.  Like FlowAdam it can be captured into a hipGraph once ``prepare()`` has created its state."""
 
     def __init__(self, params, lr=0.02, adam_lr=1e-4, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
@@ -227,8 +227,15 @@ class FlowMuon(torch.optim.Optimizer):
         self._adam = FlowAdam(others, lr=adam_lr) if others else None
         self._share()
 
-    def _group(self, kind):
-        return next((g for g in self.param_groups if g['kind'] == kind), None)
+    def add_param_group(self, group):
+        """Further groups hold matrices."""
+        group.setdefault('kind', 'matrices')
+        if group['kind'] == 'matrices' and any(p.dim() < 2 for p in ([group['params']] if torch.is_tensor(group['params']) else group['params'])):
+            raise ValueError('FlowMuon: a further parameter group holds weights of two or more dimensions')
+        super().add_param_group(group)
+
+    def _matrices(self):
+        return [p for g in self.param_groups if g['kind'] == 'matrices' for p in g['params']]
 
     def _share(self):
         """One state for both: the inner Adam keeps its moments in this optimizer's ``state``."""
@@ -237,8 +244,7 @@ class FlowMuon(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
-        group = self._group('matrices')
-        for p in group['params'] if group else ():
+        for p in self._matrices():
             if p in self.state:                # Optimizer.load_state_dict casts to the parameter's type
                 m = self.state[p]['momentum_buffer']
                 self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(m)
@@ -256,8 +262,7 @@ class FlowMuon(torch.optim.Optimizer):
 
     def prepare(self):
         """Create the state of all parameters now (before a capture)."""
-        group = self._group('matrices')
-        for p in group['params'] if group else ():
+        for p in self._matrices():
             self._momentum(p)
         return self._adam.prepare() if self._adam is not None else True
 
@@ -267,12 +272,13 @@ class FlowMuon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        g = self._group('matrices')
-        if g is not None:
+        for g in self.param_groups:
+            if g['kind'] != 'matrices':
+                continue
             params = [p for p in g['params'] if p.grad is not None]
             muon_step_(params, [p.grad for p in params], [self._momentum(p) for p in params], lr=g['lr'], momentum=g['momentum'], weight_decay=g['weight_decay'],
                        nesterov=g['nesterov'], steps=g['steps'], coefficients=g['coefficients'], eps=g['eps'])
         if self._adam is not None:
-            self._adam.param_groups[0]['lr'] = self._group('others')['lr']
+            self._adam.param_groups[0]['lr'] = next(g['lr'] for g in self.param_groups if g['kind'] == 'others')
             self._adam.step()
         return loss
