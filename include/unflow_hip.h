@@ -432,6 +432,7 @@ int unflow_prepare_triplets(const uint8_t* src, const long long* offsets, const 
  * unflow_linear_ce_workspace() says how many bytes are kept and how many each pass needs as workspace (256-byte aligned; its contents mean nothing
  * between calls).  The alignment of hidden and weight is part of the question: ask with the pointers of the call. */
 #define UNFLOW_LCE_MAX_ROWS (1 << 20)      /* N; split longer batches */
+#define UNFLOW_LCE_MAX_CLASSES (1 << 30)   /* V */
 #define UNFLOW_LCE_MAX_DIM (1 << 20)       /* D, ldh, ldw */
 int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_dhidden, int need_dweight,
                                long long* kept_bytes, long long* forward_bytes, long long* backward_bytes);

@@ -109,6 +109,13 @@ def test_loss_and_gradients(device, dtype, rows, vocab, dim, reduction, scale):
     _check_lce(h, w, t, dtype, reduction, scale)
 
 
+@pytest.mark.parametrize('rows,vocab,reduction', [(1024, 40, 'mean'), (1025, 40, 'mean'), (5, 2200, 'sum'), (300, 2200, 'mean'), (40, 2048, 'sum')])
+def test_rows_and_tiles_joined_in_one_launch_or_two(device, rows, vocab, reduction):
+    """Up to 1024 rows of up to 32 tiles, and more of either."""
+    h, w, t = _inputs(rows, vocab, 8, torch.bfloat16, device)
+    _check_lce(h, w, t, torch.bfloat16, reduction)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('rows,vocab,dim', [(1, 32000, 2048), (7, 50257, 129), (513, 3001, 777), (832, 832, 96), (2100, 2200, 200), (3700, 4000, 264),
@@ -338,7 +345,7 @@ def test_entry_points_check_their_arguments():
     ok, k, a, b = 4096, ctypes.c_longlong(), ctypes.c_longlong(), ctypes.c_longlong()
     size = lambda *v: lib.unflow_linear_ce_workspace(ok, v[2], ok, v[2], *v, 1, 1, ctypes.byref(k), ctypes.byref(a), ctypes.byref(b))  # noqa: E731
     assert size(5, 7, 8, 0) == 0 and a.value > 0 and b.value > 0 and k.value > 0
-    for bad in ((0, 7, 8, 0), (5, 0, 8, 0), (5, 7, 0, 0), (5, 7, 8, 3), (5, 7, 8, -1), ((1 << 20) + 1, 7, 8, 0), (5, 7, (1 << 20) + 1, 0)):
+    for bad in ((0, 7, 8, 0), (5, 0, 8, 0), (5, 7, 0, 0), (5, 7, 8, 3), (5, 7, 8, -1), ((1 << 20) + 1, 7, 8, 0), (5, (1 << 30) + 1, 8, 0), (5, 7, (1 << 20) + 1, 0)):
         assert size(*bad) == -22, bad
     fwd = lambda ws, n, red=0, loss=ok, kept=ok: lib.unflow_linear_ce_fwd(ok, 8, ok, 8, ok, 5, 7, 8, 0, 1.0, -100, red, loss, kept, ws, n, None)  # noqa: E731
     assert fwd(ok, 16) == -22 and fwd(None, 1 << 30) == -22 and fwd(ok, 1 << 30, 3) == -22 and fwd(ok, 1 << 30, 0, None) == -22 and fwd(ok, 1 << 30, 0, ok, None) == -22

@@ -28,7 +28,8 @@ constexpr int kMaxima = 1024;                                      // workgroups
 // fp32 rows are packed with a power of two of their own that brings the row's largest magnitude to [2^14, 2^15), their transposes (where rows are
 // what is summed over) with one for the whole matrix.
 struct Exponents { int h, w; };      // of the transposes
-struct Row { float top, inverse, others, unused; };                // of a row: log2(e) max z, 1 / sum exp(z - max z), sum over all classes but the target times that
+// of a row: log2(e) max z, 1 / sum exp(z - max z), sum over all classes but the target times that
+struct Row { float top, inverse, others, unused; };
 
 __device__ __forceinline__ float finite_magnitude(float m, f32x4 v) {
 #pragma unroll
@@ -95,7 +96,7 @@ template <int PL> __device__ __forceinline__ f32x4 logits_of(const Logits& l, f3
 // are not the row's target, and the target's z.  partial [tile column][N]
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand H, Operand W, int width, Logits how,
-                                                                                                    const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
+        const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(W.rows, TileT::BN), total = mt * nt;
     float2* rows = reinterpret_cast<float2*>(lds + TileT::STAGES_LDS);                    // [WN][BM]
@@ -106,70 +107,73 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
     T.start(H, W, 0, width, tm * TileT::BM, tn * TileT::BN, lds);
     // a workgroup goes through tiles a grid apart: the copies of the next one are under way while this one's sums are dealt with
     for (bool more = true; more;) {
-    T.finish(lds);
-    const int m0 = tm * TileT::BM, n0 = tn * TileT::BN, column = tn;
-    id += (int)gridDim.x;
-    more = id < total;
-    if (more) {
-        tile_of(xcd_remap(id, total), mt, nt, tm, tn);
-        T.start(H, W, 0, width, tm * TileT::BM, tn * TileT::BN, lds);
-    }
-    const bool edge = n0 + TileT::BN > W.rows;
-#pragma unroll
-    for (int i = 0; i < TileT::MI; ++i) {
-        const int m = m0 + TileT::row(i);
-        const long long t = m < H.rows ? target[m] - n0 : -1;                            // the target's place in this tile
-        const int own = t >= 0 && t < TileT::BN && t + n0 < W.rows ? (int)t : -1, eh = TileT::PL == TWO && m < H.rows ? how.eh[m] : 0;
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < TileT::NI; ++j) {
-            f32x4 z = logits_of<TileT::PL>(how, T.acc[i][j], eh, n0 + TileT::col(j), W.rows - 1);
-            if (edge)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) z[r] = n0 + TileT::col(j) + r < W.rows ? z[r] : -INFINITY;
-            T.acc[i][j] = z;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, z[r]);
+        T.finish(lds);
+        const int m0 = tm * TileT::BM, n0 = tn * TileT::BN, column = tn;
+        id += (int)gridDim.x;
+        more = id < total;
+        if (more) {
+            tile_of(xcd_remap(id, total), mt, nt, tm, tn);
+            T.start(H, W, 0, width, tm * TileT::BM, tn * TileT::BN, lds);
         }
-        if (__ballot(own >= 0))                                                          // (few of a wave's rows have their target among its columns)
+        const bool edge = n0 + TileT::BN > W.rows;
+#pragma unroll
+        for (int i = 0; i < TileT::MI; ++i) {
+            const int m = m0 + TileT::row(i);
+            const long long t = m < H.rows ? target[m] - n0 : -1;                            // the target's place in this tile
+            const int own = t >= 0 && t < TileT::BN && t + n0 < W.rows ? (int)t : -1, eh = TileT::PL == TWO && m < H.rows ? how.eh[m] : 0;
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < TileT::NI; ++j) {
+                f32x4 z = logits_of<TileT::PL>(how, T.acc[i][j], eh, n0 + TileT::col(j), W.rows - 1);
+                if (edge)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[r] = n0 + TileT::col(j) + r < W.rows ? z[r] : -INFINITY;
+                T.acc[i][j] = z;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, z[r]);
+            }
+            // (few of a wave's rows have their target among its columns)
+            if (__ballot(own >= 0))
+#pragma unroll
+                for (int j = 0; j < TileT::NI; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (TileT::col(j) + r == own) {
+                            ztarget[m] = T.acc[i][j][r];
+                            T.acc[i][j][r] = -INFINITY;
+                        }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float base = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < TileT::NI; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (TileT::col(j) + r == own) {
-                        ztarget[m] = T.acc[i][j][r];
-                        T.acc[i][j][r] = -INFINITY;
-                    }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < TileT::NI; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum += exp2_of(T.acc[i][j][r] - base);
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (group == 0) rows[wn * TileT::BM + TileT::row(i)] = make_float2(top, sum);
-    }
-    __syncthreads();
-    for (int r = (int)threadIdx.x; r < TileT::BM && m0 + r < H.rows; r += TileT::THREADS) {
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int q = 0; q < TileT::WN; ++q) top = fmaxf(top, rows[q * TileT::BM + r].x);
-#pragma unroll
-        for (int q = 0; q < TileT::WN; ++q) {
-            const float2 v = rows[q * TileT::BM + r];
-            sum += v.x != -INFINITY ? v.y * exp2_of(v.x - top) : v.y;                      // (without a maximum: 0, or NaN from NaNs, which fmaxf passes over)
+                for (int r = 0; r < 4; ++r) sum += exp2_of(T.acc[i][j][r] - base);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (group == 0) rows[wn * TileT::BM + TileT::row(i)] = make_float2(top, sum);
         }
-        partial[(long long)column * H.rows + m0 + r] = make_float2(top, sum);
-    }
+        __syncthreads();
+        for (int r = (int)threadIdx.x; r < TileT::BM && m0 + r < H.rows; r += TileT::THREADS) {
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < TileT::WN; ++q) top = fmaxf(top, rows[q * TileT::BM + r].x);
+#pragma unroll
+            for (int q = 0; q < TileT::WN; ++q) {
+                const float2 v = rows[q * TileT::BM + r];
+                // (without a maximum: 0, or NaN from NaNs, which fmaxf passes over)
+                sum += v.x != -INFINITY ? v.y * exp2_of(v.x - top) : v.y;
+            }
+            partial[(long long)column * H.rows + m0 + r] = make_float2(top, sum);
+        }
     }
 }
 
 // ---- forward of few rows (at most 16 NF): reading W is all there is to it.  16-bit inputs of more than 16 rows are better served by the tiles
-// above, where the four waves share the rows of H (61 rows against 50257 classes of 1024 fp16: 28 us against 36); fp32 inputs stay here up to 64
-// rows, for packing W would read and write all of it once more.  A workgroup takes 16 CF classes, its four waves a quarter of D each, AHEAD
+// above, where the four waves share the rows of H (61 rows against 50257 classes of 1024 fp16: 20 us against 36); fp32 inputs stay here up to 64
+// rows, for packing W would read and write all of it once more (50257 classes of 1024 dimensions, whole calls: 16 rows 58 us against 200 through
+// the tiles, 33 rows 112 against 204, 64 rows 126 against 212; 5000 of 256: 15 against 18).  A workgroup takes 16 CF classes, its four waves a quarter of D each, AHEAD
 // steps of loads in flight; the rows of W go from memory to the matrix instruction as they lie there.  16-bit numbers: 32 k a step, lane l holds
 // k = 8 (l >> 4) .. of row l & 15.  fp32: 16 k a step as four v_mfma_f32_16x16x4_f32, the e-th taking k = 4 (l >> 4) + e -- fp32 arithmetic
 // throughout, and no packing.
@@ -183,7 +187,8 @@ template <class T> __device__ __forceinline__ f32x4 few_product(uint4 a, uint4 b
     } else return mfma16<__is_same(T, __bf16) ? BF16 : FP16>(a, b, c);
 }
 template <class T, int NF, int CF, int AHEAD>
-__global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, long long ldh, const T* __restrict__ W, long long ldw, int N, int V, int D, float scale, const long long* __restrict__ target,
+__global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, long long ldh, const T* __restrict__ W, long long ldw, int N, int V,
+        int D, float scale, const long long* __restrict__ target,
                                                       float2* __restrict__ partial, float* __restrict__ ztarget) {
     constexpr int ROWS = 16 * NF, PER = 256 / ROWS, CLASSES = 16 * CF / PER, PITCH = 16 * CF + 2;
     __shared__ float sums[4][ROWS][PITCH];
@@ -192,7 +197,8 @@ __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, l
     const T* wrow[CF];
     const T* hrow[NF];
 #pragma unroll
-    for (int c = 0; c < CF; ++c) wrow[c] = W + (long long)(v0 + 16 * c + r_lane < V ? v0 + 16 * c + r_lane : V - 1) * ldw;          // (classes behind the last repeat it, unused)
+    // (classes behind the last repeat it, unused)
+    for (int c = 0; c < CF; ++c) wrow[c] = W + (long long)(v0 + 16 * c + r_lane < V ? v0 + 16 * c + r_lane : V - 1) * ldw;
 #pragma unroll
     for (int i = 0; i < NF; ++i) hrow[i] = H + (long long)(16 * i + r_lane < N ? 16 * i + r_lane : N - 1) * ldh;
     f32x4 acc[CF][NF];
@@ -205,7 +211,8 @@ __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, l
         uint4 a[AHEAD][CF], b[AHEAD][NF];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int k = (first + (u / 2) * 8 + w * 2 + u % 2) * Few<T>::STEP + k_lane;              // (a wave takes two steps in a row: whole lines of W)
+            // (a wave takes two steps in a row: whole lines of W)
+            const int k = (first + (u / 2) * 8 + w * 2 + u % 2) * Few<T>::STEP + k_lane;
             const bool in = k < D;                                                         // (D is a multiple of what a lane loads)
 #pragma unroll
             for (int c = 0; c < CF; ++c) a[u][c] = in ? *reinterpret_cast<const uint4*>(wrow[c] + k) : uint4{0, 0, 0, 0};
@@ -250,55 +257,44 @@ __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, l
     if (part == 0 && m < N) partial[(long long)blockIdx.x * N + m] = make_float2(top, sum);
 }
 
-// the tiles' (maximum, sum) pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup.  The target's own term joins
-// here: where it outweighs the others, loss = log1p(others / own) and others / all = 1 - p keep the digits that 1 - p would lose.
+// two (maximum, sum) pairs as one
+__device__ __forceinline__ float2 joined(float2 x, float2 y) {
+    const float both = fmaxf(x.x, y.x), base = both == -INFINITY ? 0.f : both;
+    return make_float2(both, x.y * (x.x == -INFINITY ? 1.f : exp2_of(x.x - base)) + y.y * (y.x == -INFINITY ? 1.f : exp2_of(y.x - base)));
+}
+// A row's statistics and loss from its joined pair.  The target's own term joins here: where it outweighs the others, loss = log1p(others / own)
+// and others / all = 1 - p keep the digits that 1 - p would lose.
+__device__ __forceinline__ float row_of(float2 pair, long long t, long long ignore, int V, const float* __restrict__ ztarget, Row* __restrict__ stats) {
+    const float base = pair.x == -INFINITY ? 0.f : pair.x, others = pair.y;
+    const bool known = t >= 0 && t < V;
+    const float zt = known ? *ztarget : -INFINITY, own = known ? exp2_of(zt - base) : 0.f, all = others + own;
+    *stats = Row{base, 1.f / all, others / all, 0.f};
+    return t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) * kLn2 + logf(all);
+}
+
+// the tiles' pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup
 template <int R>
-__global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict__ partial, int tiles, int N, int V, const long long* __restrict__ target, long long ignore,
-                                                       const float* __restrict__ ztarget, Row* __restrict__ stats, float* __restrict__ losses) {
+__global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict__ partial, int tiles, int N, int V, const long long* __restrict__ target,
+        long long ignore, const float* __restrict__ ztarget, Row* __restrict__ stats, float* __restrict__ losses) {
     constexpr int SHARES = 256 / R;
     __shared__ float2 part[SHARES][R + 1];
     const int r = threadIdx.x % R, share = threadIdx.x / R, m = blockIdx.x * R + r;
-    float top = -INFINITY, sum = 0.f;
+    float2 pair = make_float2(-INFINITY, 0.f);
     if (m < N)
-        for (int t = share; t < tiles; t += SHARES) {
-            const float2 v = partial[(long long)t * N + m];
-            const float both = fmaxf(top, v.x);
-            const float base = both == -INFINITY ? 0.f : both;
-            sum = sum * (top == -INFINITY ? 1.f : exp2_of(top - base)) + v.y * (v.x == -INFINITY ? 1.f : exp2_of(v.x - base));
-            top = both;
-        }
-    part[share][r] = make_float2(top, sum);
+        for (int t = share; t < tiles; t += SHARES) pair = joined(pair, partial[(long long)t * N + m]);
+    part[share][r] = pair;
     __syncthreads();
     for (int half = SHARES / 2; half > 0; half /= 2) {
-        if (share < half) {
-            const float2 x = part[share][r], y = part[share + half][r];
-            const float both = fmaxf(x.x, y.x);
-            const float base = both == -INFINITY ? 0.f : both;
-            part[share][r] = make_float2(both, x.y * (x.x == -INFINITY ? 1.f : exp2_of(x.x - base)) + y.y * (y.x == -INFINITY ? 1.f : exp2_of(y.x - base)));
-        }
+        if (share < half) part[share][r] = joined(part[share][r], part[share + half][r]);
         __syncthreads();
     }
-    if (share == 0 && m < N) {
-        top = part[0][r].x;
-        const float others = part[0][r].y, base = top == -INFINITY ? 0.f : top;
-        const long long t = target[m];
-        const bool known = t >= 0 && t < V;
-        const float zt = known ? ztarget[m] : -INFINITY, own = known ? exp2_of(zt - base) : 0.f, all = others + own;
-        stats[m] = Row{base, 1.f / all, others / all, 0.f};
-        losses[m] = t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) * kLn2 + logf(all);
-    }
+    if (share == 0 && m < N) losses[m] = row_of(part[0][r], target[m], ignore, V, ztarget + m, stats + m);
 }
 
-// loss = sum of the rows' losses (mean: divided by the number of rows that are not ignored, at least 1, which is left for the backward pass); one
-// workgroup, fixed order
-__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restrict__ losses, const long long* __restrict__ target, long long ignore, int N, int mean, float* __restrict__ loss,
-                                                          float* __restrict__ count) {
+// loss = sum of a thread's losses over the workgroup (mean: divided by the number of rows that are not ignored, at least 1, which is left for the
+// backward pass); fixed order
+__device__ __forceinline__ void reduce_losses(float s, float c, int mean, float* __restrict__ loss, float* __restrict__ count) {
     __shared__ float red[16], cnt[16];
-    float s = 0.f, c = 0.f;
-    for (int i = threadIdx.x; i < N; i += 1024) {
-        s += losses[i];
-        c += target[i] != ignore ? 1.f : 0.f;
-    }
     s = wave_sum(s);
     c = wave_sum(c);
     if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = s; cnt[threadIdx.x >> 6] = c; }
@@ -310,9 +306,34 @@ __global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restric
         loss[0] = mean ? s / fmaxf(c, 1.f) : s;
     }
 }
+__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restrict__ losses, const long long* __restrict__ target, long long ignore, int N,
+        int mean, float* __restrict__ loss, float* __restrict__ count) {
+    float s = 0.f, c = 0.f;
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        s += losses[i];
+        c += target[i] != ignore ? 1.f : 0.f;
+    }
+    reduce_losses(s, c, mean, loss, count);
+}
+// both at once for up to 1024 rows of few tiles: a launch less where launches are what a pass costs
+__global__ __launch_bounds__(1024) void lce_join_reduce_kernel(const float2* __restrict__ partial, int tiles, int N, int V,
+        const long long* __restrict__ target, long long ignore, const float* __restrict__ ztarget, Row* __restrict__ stats, int mean,
+        float* __restrict__ loss, float* __restrict__ count) {
+    const int m = threadIdx.x;
+    float s = 0.f, c = 0.f;
+    if (m < N) {
+        float2 pair = make_float2(-INFINITY, 0.f);
+        for (int t = 0; t < tiles; ++t) pair = joined(pair, partial[(long long)t * N + m]);
+        const long long t = target[m];
+        s = row_of(pair, t, ignore, V, ztarget + m, stats + m);
+        c = t != ignore ? 1.f : 0.f;
+    }
+    reduce_losses(s, c, mean, loss, count);
+}
 
 // ---- backward
-// The upstream gradient: one number for a reduced loss, one per row for reduction none (these relative to the largest, so that fp16 planes hold them).
+// The upstream gradient: one number for a reduced loss, one per row for reduction none (these relative to the largest, so that fp16 planes hold
+// them).
 struct Upstream { const float* g; const float* largest; const float* count; const long long* target; long long ignore; int reduction; float scale; };
 __device__ __forceinline__ float uniform_factor(const Upstream& u) {
     return u.reduction == 0 ? u.scale : u.reduction == 1 ? u.scale * u.g[0] / u.count[0] : u.scale * u.g[0];
@@ -365,7 +386,7 @@ template <int EL> __host__ __device__ constexpr int probability_exponent() { ret
 // same times the row's upstream gradient relative to the largest; columns behind N and vp up to the packed width are zero
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand H, Operand W, int width, Logits how,
-                                                                                                     const Row* __restrict__ stats, Upstream up, int v0, int vp, int V, u16* __restrict__ G, long long ldg,
+        const Row* __restrict__ stats, Upstream up, int v0, int vp, int V, u16* __restrict__ G, long long ldg,
                                                                                                      u16* __restrict__ GT, long long ldgt) {
     constexpr int PL = TileT::PL, EL = TileT::EL;
     UNFLOW_DYNAMIC_LDS(char, lds);
@@ -407,7 +428,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (TileT::col(j) + r == own) T.acc[i][j][r] = -s.others * unit;
-        if (there)
+        if (G && there)
 #pragma unroll
             for (int j = 0; j < TileT::NI; ++j)
                 if (n0 + TileT::col(j) < wide_n) pack4<PL, EL>(G + (long long)m * ldg, n0 + TileT::col(j), T.acc[i][j]);
@@ -460,13 +481,17 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product
             if (!p.first) {                                            // (all of a row's loads before its sums: one wait, not one per load)
                 f32x4 old[TileT::NI];
 #pragma unroll
-                for (int j = 0; j < TileT::NI; ++j) old[j] = n0 + TileT::col(j) < p.ldc ? *reinterpret_cast<const f32x4*>(row + n0 + TileT::col(j)) : f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < TileT::NI; ++j) {
+                    const int n = n0 + TileT::col(j);
+                    old[j] = n < p.ldc ? *reinterpret_cast<const f32x4*>(row + n) : f32x4{0.f, 0.f, 0.f, 0.f};
+                }
 #pragma unroll
                 for (int j = 0; j < TileT::NI; ++j) T.acc[i][j] += old[j];
             }
 #pragma unroll
             for (int j = 0; j < TileT::NI; ++j)
-                if (n0 + TileT::col(j) < p.ldc) *reinterpret_cast<f32x4*>(row + n0 + TileT::col(j)) = T.acc[i][j];   // (ldc: the columns rounded up to 4)
+                // (ldc: the columns rounded up to 4)
+                if (n0 + TileT::col(j) < p.ldc) *reinterpret_cast<f32x4*>(row + n0 + TileT::col(j)) = T.acc[i][j];
         }
         return;
     }
@@ -542,7 +567,8 @@ static bool aligned(const void* p, long long ld, int D, int dtype) {
     return D % each == 0 && ld % each == 0 && ((size_t)p & 15) == 0;
 }
 
-static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, bool train, bool need_h, bool need_w) {
+static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, bool train, bool need_h,
+        bool need_w) {
     Plan p{};
     p.planes = dtype == kFp32 ? TWO : ONE;
     p.few = N <= (dtype == kFp32 ? 64 : 16) && aligned(h, ldh, D, dtype) && aligned(w, ldw, D, dtype);
@@ -627,8 +653,9 @@ static Logits operands(const Plan& p, const Inputs& in, char* to, bool pack, hip
     const Packed at{(u16*)(to + p.hp), (u16*)(to + p.wp), (int*)(to + p.eh), (int*)(to + p.ew), (float*)(to + p.maxima)};
     if (pack && (p.pack_h || p.pack_w)) {
         const int blocks_h = p.pack_h ? pack_blocks(in.N) : 0, blocks_w = p.pack_w ? pack_blocks(in.V) : 0;
-        UNFLOW_LAUNCH((pack_inputs_kernel<T, PL, EL>), dim3(blocks_h + blocks_w), dim3(256), 0, stream, Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, Source{in.w, in.ldw, in.V, in.D}, blocks_h,
-                      at, p.wd, (int)(PL == TWO ? p.wd / 2 : p.wd));
+        UNFLOW_LAUNCH((pack_inputs_kernel<T, PL, EL>), dim3(blocks_h + blocks_w), dim3(256), 0, stream,
+            Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, Source{in.w, in.ldw, in.V, in.D}, blocks_h, at, p.wd,
+            (int)(PL == TWO ? p.wd / 2 : p.wd));
     }
     return Logits{in.scale * kLog2E, at.eh, at.ew};
 }
@@ -642,30 +669,47 @@ static void forward(const Plan& p, const Inputs& in, int reduction, float* loss,
     int columns;
     if (p.few) {
         columns = ceil_div(in.V, few_classes(in.N));
-        const T *h = (const T*)in.h, *w = (const T*)in.w;
-        const float scale = in.scale * kLog2E;
-        // (beyond 16 rows a wave holds fewer classes, so that more waves fit a CU: 61 rows against 50257 classes of 1024 fp16)
-        if (in.N <= 16) UNFLOW_LAUNCH((lce_few_kernel<T, 1, 4, 4>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, scale, in.target, partial, zt);
-        else if constexpr (sizeof(T) < 4) return;
-        else if (in.N <= 32) UNFLOW_LAUNCH((lce_few_kernel<T, 2, 2, 4>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, scale, in.target, partial, zt);
-        else UNFLOW_LAUNCH((lce_few_kernel<T, 4, 2, 2>), dim3(columns), dim3(256), 0, stream, h, in.ldh, w, in.ldw, in.N, in.V, in.D, scale, in.target, partial, zt);
+        auto launch = [&](auto kernel) {
+            UNFLOW_LAUNCH(kernel, dim3(columns), dim3(256), 0, stream, (const T*)in.h, in.ldh, (const T*)in.w, in.ldw, in.N, in.V, in.D,
+                in.scale * kLog2E, in.target, partial, zt);
+        };
+        if (in.N <= 16) launch(lce_few_kernel<T, 1, 4, 4>);
+        else if constexpr (PL == TWO) {
+            // (beyond 16 rows a wave holds fewer classes and steps, so that more waves fit a CU)
+            if (in.N <= 32) launch(lce_few_kernel<T, 2, 2, 4>);
+            else launch(lce_few_kernel<T, 4, 2, 2>);
+        }
     } else {
         Operand H, W;
         const Logits how = operands<T, PL, EL>(p, in, kept, true, stream, H, W);
         columns = ceil_div(in.V, kSizes[p.size_z]);
         with_tile<PL, EL>(p.size_z, [&](auto tile) {
             using TileT = decltype(tile);
-            LAUNCH_TILES((lce_forward_kernel<TileT>), resident<TileT>(tiles_of(in.N, in.V, TileT::BM)), TileT::STAGES_LDS + TileT::WN * TileT::BM * (int)sizeof(float2), H, W, (int)p.wd, how, in.target, partial, zt);
+            LAUNCH_TILES((lce_forward_kernel<TileT>), resident<TileT>(tiles_of(in.N, in.V, TileT::BM)),
+                TileT::STAGES_LDS + TileT::WN * TileT::BM * (int)sizeof(float2), H, W, (int)p.wd, how, in.target, partial, zt);
         });
     }
+    const float2* pairs = partial;
+    const float* own = zt;
+    Row* rows = (Row*)stats;
+    float* count = stats + 4ll * in.N;
+    if (reduction != 0 && in.N <= 1024 && columns <= 32) {
+        UNFLOW_LAUNCH(lce_join_reduce_kernel, dim3(1), dim3(1024), 0, stream, pairs, columns, in.N, in.V, in.target, in.ignore, own, rows,
+            reduction == 1 ? 1 : 0, loss, count);
+        return;
+    }
     // (a workgroup for 16 rows reads their pairs in whole lines; few rows over many columns need more of them)
-    if (in.N <= 256) UNFLOW_LAUNCH((lce_join_kernel<1>), dim3(in.N), dim3(256), 0, stream, (const float2*)partial, columns, in.N, in.V, in.target, in.ignore, (const float*)zt, (Row*)stats, losses);
-    else UNFLOW_LAUNCH((lce_join_kernel<16>), dim3(ceil_div(in.N, 16)), dim3(256), 0, stream, (const float2*)partial, columns, in.N, in.V, in.target, in.ignore, (const float*)zt, (Row*)stats, losses);
-    if (reduction != 0) UNFLOW_LAUNCH(lce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)losses, in.target, in.ignore, in.N, reduction == 1 ? 1 : 0, loss, stats + 4ll * in.N);
+    if (in.N <= 256) UNFLOW_LAUNCH((lce_join_kernel<1>), dim3(in.N), dim3(256), 0, stream, pairs, columns, in.N, in.V, in.target, in.ignore, own,
+        rows, losses);
+    else UNFLOW_LAUNCH((lce_join_kernel<16>), dim3(ceil_div(in.N, 16)), dim3(256), 0, stream, pairs, columns, in.N, in.V, in.target, in.ignore, own,
+        rows, losses);
+    if (reduction != 0) UNFLOW_LAUNCH(lce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)losses, in.target, in.ignore, in.N,
+        reduction == 1 ? 1 : 0, loss, count);
 }
 
 template <class T, int PL, int EL>
-static void backward(const Plan& p, const Inputs& in, int reduction, const float* gout, void* dh, void* dw, char* kept, char* ws, hipStream_t stream) {
+static void backward(const Plan& p, const Inputs& in, int reduction, const float* gout, void* dh, void* dw, char* kept, char* ws,
+        hipStream_t stream) {
     const float* stats = (const float*)(kept + p.stats);
     char* to = p.keeps ? kept : ws + p.repacked;
     Operand H, W;
@@ -682,26 +726,32 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
         Columns wc{}, hc{};
         int blocks_w = 0, blocks_h = 0;
         if (dh) {
-            wc = Columns{Source{(const T*)in.w + (long long)v0 * in.ldw, in.ldw, vp, in.D}, (u16*)(ws + p.wt), wvp, (int)(PL == TWO ? wvp / 2 : wvp), maxima + kMaxima, pack_blocks(in.V)};
+            wc = Columns{Source{(const T*)in.w + (long long)v0 * in.ldw, in.ldw, vp, in.D}, (u16*)(ws + p.wt), wvp,
+                (int)(PL == TWO ? wvp / 2 : wvp), maxima + kMaxima, pack_blocks(in.V)};
             blocks_w = ceil_div(wc.width, 64) * ceil_div(in.D, 64);
         }
         if (dw && v0 == 0) {
-            hc = Columns{Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, (u16*)(ws + p.ht), p.wn, (int)(PL == TWO ? p.wn / 2 : p.wn), maxima, pack_blocks(in.N)};
+            hc = Columns{Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, (u16*)(ws + p.ht), p.wn, (int)(PL == TWO ? p.wn / 2 : p.wn),
+                maxima, pack_blocks(in.N)};
             blocks_h = ceil_div(hc.width, 64) * ceil_div(in.D, 64);
         }
-        if (blocks_w + blocks_h) UNFLOW_LAUNCH((pack_transposes_kernel<T, PL, EL>), dim3(blocks_w + blocks_h), dim3(256), 0, stream, wc, hc, blocks_w, ex);
+        if (blocks_w + blocks_h) UNFLOW_LAUNCH((pack_transposes_kernel<T, PL, EL>), dim3(blocks_w + blocks_h), dim3(256), 0, stream, wc, hc,
+            blocks_w, ex);
         with_tile<PL, EL>(p.size_g, [&](auto tile) {
             using TileT = decltype(tile);
-            LAUNCH_TILES((lce_gradient_kernel<TileT>), (int)tiles_of(in.N, vp, TileT::BM), TileT::LDS, H, W, (int)p.wd, how, (const Row*)stats, up, v0, vp, in.V, G, p.wvp, dw ? GT : nullptr, p.wn);
+            LAUNCH_TILES((lce_gradient_kernel<TileT>), (int)tiles_of(in.N, vp, TileT::BM), TileT::LDS, H, W, (int)p.wd, how, (const Row*)stats, up,
+                v0, vp, in.V, dh ? G : nullptr, p.wvp, dw ? GT : nullptr, p.wn);
         });
         Product a{}, b{};
         a.shares = b.shares = 1;
         if (dh) {
-            a = Product{Operand{G, p.wvp, in.N}, Operand{(const u16*)(ws + p.wt), wvp, in.D}, (int)wvp, shares_of(stages_of(p.wvp), p.limit), 0, (float*)(ws + p.sum_h), p.ldc, v0 == 0 ? 1 : 0, dh, 0};
+            a = Product{Operand{G, p.wvp, in.N}, Operand{(const u16*)(ws + p.wt), wvp, in.D}, (int)wvp, shares_of(stages_of(p.wvp), p.limit), 0,
+                (float*)(ws + p.sum_h), p.ldc, v0 == 0 ? 1 : 0, dh, 0};
             if (single && a.shares == 1) a.sums = nullptr;
         }
         if (dw) {
-            b = Product{Operand{GT, p.wn, vp}, Operand{(const u16*)(ws + p.ht), p.wn, in.D}, (int)p.wn, shares_of(stages_of(p.wn), p.limit), 0, (float*)(ws + p.sum_w), p.ldc, 1, (T*)dw + (long long)v0 * in.D, 1};
+            b = Product{Operand{GT, p.wn, vp}, Operand{(const u16*)(ws + p.ht), p.wn, in.D}, (int)p.wn, shares_of(stages_of(p.wn), p.limit), 0,
+                (float*)(ws + p.sum_w), p.ldc, 1, (T*)dw + (long long)v0 * in.D, 1};
             if (b.shares == 1) b.sums = nullptr;
         }
         with_tile<PL, EL>(p.size_p, [&](auto tile) {
@@ -709,22 +759,27 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
             if (dh) a.tiles = (int)tiles_of(in.N, in.D, TileT::BM);
             if (dw) b.tiles = (int)tiles_of(vp, in.D, TileT::BM);
             const bool swap = dw && (!dh || b.width / b.shares > a.width / a.shares);        // the longer units first
-            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, TileT::STAGES_LDS, swap ? b : a, swap ? a : b, (const Exponents*)ex, up);
+            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, TileT::STAGES_LDS, swap ? b : a, swap ? a : b,
+                (const Exponents*)ex, up);
         });
         const bool last = v0 + vp >= in.V;
-        const int finish_a = dh && last && a.sums ? blocks_for((long long)in.N * (p.ldc / 4)) : 0, finish_b = dw && b.sums ? blocks_for((long long)vp * (p.ldc / 4)) : 0;
-        if (finish_a + finish_b) UNFLOW_LAUNCH((lce_finish_kernel<T, PL, EL>), dim3(finish_a + finish_b), dim3(256), 0, stream, a, b, finish_a, (const Exponents*)ex, up);
+        const int finish_a = dh && last && a.sums ? blocks_for((long long)in.N * (p.ldc / 4)) : 0,
+            finish_b = dw && b.sums ? blocks_for((long long)vp * (p.ldc / 4)) : 0;
+        if (finish_a + finish_b) UNFLOW_LAUNCH((lce_finish_kernel<T, PL, EL>), dim3(finish_a + finish_b), dim3(256), 0, stream, a, b, finish_a,
+            (const Exponents*)ex, up);
     }
 }
 
 static bool sizes_ok(long long ldh, long long ldw, int N, int V, int D, int dtype, int reduction) {
-    return N > 0 && V > 0 && D > 0 && N <= UNFLOW_LCE_MAX_ROWS && D <= UNFLOW_LCE_MAX_DIM && ldh >= D && ldw >= D && ldh <= UNFLOW_LCE_MAX_DIM && ldw <= UNFLOW_LCE_MAX_DIM &&
+    return N > 0 && V > 0 && D > 0 && N <= UNFLOW_LCE_MAX_ROWS && V <= UNFLOW_LCE_MAX_CLASSES && D <= UNFLOW_LCE_MAX_DIM &&
+           ldh >= D && ldw >= D && ldh <= UNFLOW_LCE_MAX_DIM && ldw <= UNFLOW_LCE_MAX_DIM &&
            dtype >= kFp32 && dtype <= kFp16 && reduction >= 0 && reduction <= 2;
 }
 
 }  // namespace
 
-extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_dhidden, int need_dweight,
+extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype,
+        int need_dhidden, int need_dweight,
                                           long long* kept_bytes, long long* forward_bytes, long long* backward_bytes) {
     UNFLOW_REQUIRE(kept_bytes && forward_bytes && backward_bytes && sizes_ok(ldh, ldw, N, V, D, dtype, 0));
     const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, need_dhidden || need_dweight, need_dhidden != 0, need_dweight != 0);
@@ -734,8 +789,10 @@ extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, con
     return 0;
 }
 
-extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V, int D, int dtype, float scale,
-                                    long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes, void* stream) {
+extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V,
+        int D, int dtype, float scale,
+                                    long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes,
+                                        void* stream) {
     UNFLOW_REQUIRE(hidden && weight && target && loss && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
     const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, false, false, false);
     UNFLOW_REQUIRE(workspace_bytes >= p.forward_bytes);
@@ -747,8 +804,10 @@ extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const voi
     return unflow_launch_status();
 }
 
-extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* gout, int N, int V, int D,
-                                    int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept, void* workspace, long long workspace_bytes, void* stream) {
+extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
+        const float* gout, int N, int V, int D,
+                                    int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept,
+                                        void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(hidden && weight && target && gout && (dhidden || dweight) && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
     const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, true, dhidden != nullptr, dweight != nullptr);
     UNFLOW_REQUIRE(workspace_bytes >= p.backward_bytes);

@@ -73,7 +73,8 @@ template <int PL, int EL> __device__ __forceinline__ f32x4 unpack4(const u16* p,
 }
 
 template <int EL> __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
-    if constexpr (EL == BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    if constexpr (EL == BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+        0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
@@ -126,7 +127,8 @@ struct Tile {
     __device__ __forceinline__ void start(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
         const int w = wave(), lane = (int)threadIdx.x & 63;
         const int piece = (lane & 7) ^ (((4 * (w & 1)) + (lane >> 4)) & 7);          // of the row 8 q + lane / 8, q = w + WAVES i
-        // The ranges end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most 256 rows of
+        // The ranges end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most 256 rows
+        // of
         // at most 2^21 numbers: its bytes stay below 2^31.)
         const int ra = A.rows - m0 < BM ? A.rows - m0 : BM, rb = B.rows - n0 < BN ? B.rows - n0 : BN;
         range_a = range_of(A.p + (long long)m0 * A.ld, (int)(ra * A.ld * 2));
@@ -227,7 +229,8 @@ struct Tile {
     // column n at k = m.  A lane's four numbers lie in four dst rows; through LDS (half of m at a time for TWO planes) the rows leave in 16-byte
     // pieces.  `width`: elements of a dst row; LDS is free when this is called and not when it returns.
     template <class F>
-    __device__ __forceinline__ void store_transposed(char* lds, u16* __restrict__ dst, long long ld, int rows, long long width, int m0, int n0, F&& value) {
+    __device__ __forceinline__ void store_transposed(char* lds, u16* __restrict__ dst, long long ld, int rows, long long width, int m0, int n0,
+        F&& value) {
         static_assert(WM == 2, "the halves of m are the wave rows");
         constexpr int R = BM / PL;
         u16* s = reinterpret_cast<u16*>(lds);
@@ -247,7 +250,8 @@ struct Tile {
             const long long first = packed_at(PL, m0 + pass * R);
             for (int c = (int)threadIdx.x; c < BN * BM / 8; c += THREADS) {
                 const int n = c / (BM / 8), e = c % (BM / 8) * 8;
-                if (n0 + n < rows && first + e < width) *reinterpret_cast<uint4*>(dst + (long long)(n0 + n) * ld + first + e) = *reinterpret_cast<const uint4*>(s + n * PITCH + e);
+                u16* to = dst + (long long)(n0 + n) * ld + first + e;
+                if (n0 + n < rows && first + e < width) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(s + n * PITCH + e);
             }
             if (pass + 1 < PL) __syncthreads();
         }

@@ -10,7 +10,8 @@
 //
 // Numbers (mfma16.h): every type is iterated on as two fp16 planes (22 bits, products and sums as in fp32).  One plane would take a third of
 // the products, and its 2^-12 looks small beside the 2^-9 of a bf16 result, but the iteration multiplies small singular values by a^5 = 485 and
-// what rounding spreads over their directions with them: a bf16 matrix of low rank comes out several percent off that way.  The Frobenius norm is summed in 64 bits.  |X|, |S|, |Q| are bounded by the polynomial over [0, 1], which gives the powers of two that
+// what rounding spreads over their directions with them: a bf16 matrix of low rank comes out several percent off that way.  The Frobenius norm is
+// summed in 64 bits.  |X|, |S|, |Q| are bounded by the polynomial over [0, 1], which gives the powers of two that
 // the planes are scaled by.  A matrix whose norm is far below eps comes out as nearly zero, as the definition has it, but without relative
 // accuracy.
 #include "pack.h"
@@ -88,7 +89,8 @@ __device__ __forceinline__ float direction(float g, float m, float mu, int neste
 
 // ---- sum of squares of a chunk of `size` numbers (after the momentum's update)
 template <class T, bool STEP>
-__global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size, float mu, int nesterov, double* __restrict__ parts) {
+__global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size, float mu,
+        int nesterov, double* __restrict__ parts) {
     int chunk;
     const Problem p = table[problem_of(ends, count, (int)blockIdx.x, chunk)];
     const long long total = (long long)p.rows * p.cols, e0 = (long long)chunk * size;
@@ -128,7 +130,8 @@ __global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ t
 
 // ---- X_0 and its transpose, as planes: a 64 x 64 tile of the matrix per workgroup, both ways
 template <class T, bool STEP>
-__global__ __launch_bounds__(256) void start_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const double* __restrict__ parts, float mu, int nesterov, float eps,
+__global__ __launch_bounds__(256) void start_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
+        const double* __restrict__ parts, float mu, int nesterov, float eps,
                                                     Exponents ex, char* __restrict__ ws) {
     __shared__ float tile[64][65];
     __shared__ double red[256];
@@ -209,7 +212,8 @@ __device__ __forceinline__ void symmetric_store(TileT& T, char* lds, u16* __rest
 
 // ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves fp32 tiles for join_kernel
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const int* __restrict__ classes, Exponents ex, char* __restrict__ ws) {
+__global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
+        const int* __restrict__ classes, Exponents ex, char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
     const Problem p = table[dealt_problem_of(ends, count, classes, id)];
@@ -233,7 +237,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem
     symmetric_store(T, lds, (u16*)(ws + p.S), lds_, p.m, tm, tn, [&](int i, int j) { return T.acc[i][j] * f; });
 }
 // (64 x 64 of a tile of side `size` per workgroup)
-__global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size, Exponents ex, char* __restrict__ ws) {
+__global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size,
+        Exponents ex, char* __restrict__ ws) {
     __shared__ float tile[64][65];
     int id, tm, tn;
     const Problem p = table[problem_of(ends, count, (int)blockIdx.x, id)];
@@ -275,7 +280,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ t
 
 // ---- Q = a I + b S + c S S: lower tiles
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const int* __restrict__ classes, float a, float b, float c, Exponents ex,
+__global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
+        const int* __restrict__ classes, float a, float b, float c, Exponents ex,
                                                                                              char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
@@ -304,7 +310,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* 
 // ---- X <- Q X.  LAST: the output, or the parameter's update
 struct Update { float keep, lr; };                                   // 1 - lr wd, lr
 template <class TileT, bool LAST, bool STEP, class T>
-__global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, const int* __restrict__ classes, int odd, Exponents ex, Update up,
+__global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
+        const int* __restrict__ classes, int odd, Exponents ex, Update up,
                                                                                               char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
@@ -384,13 +391,15 @@ constexpr long long kGroupBytes = 4ll << 30;                         // matrices
 struct Group {
     int first, count;
     int size_s, size_q, size_x;                                      // indices into kSizes
-    int chunk;                                                       // numbers a workgroup of the norm takes: few of a small list, so that it fills the chip
+    // numbers a workgroup of the norm takes: few of a small list, so that it fills the chip
+    int chunk;
     int total[kPhases];
     long long table, ends, parts, bytes;
 };
 
 static long long plane_bytes(long long m, long long n) {
-    return round_up(2 * packed_width(TWO, n) * m, 256) + 2 * round_up(2 * packed_width(TWO, m) * n, 256) + 2 * round_up(2 * packed_width(TWO, m) * m, 256);
+    return round_up(2 * packed_width(TWO, n) * m, 256) + 2 * round_up(2 * packed_width(TWO, m) * n, 256) + 2 * round_up(2 * packed_width(TWO,
+        m) * m, 256);
 }
 
 constexpr int kMost = 1024;                                          // matrices of one group
@@ -530,27 +539,32 @@ static void write_table(const void* src, long long bytes, char* dst, hipStream_t
 }
 
 template <class T, bool STEP>
-static void iterate(const Group& g, int steps, float a, float b, float c, float eps, float mu, int nesterov, Update up, Exponents ex, char* ws, hipStream_t stream) {
+static void iterate(const Group& g, int steps, float a, float b, float c, float eps, float mu, int nesterov, Update up, Exponents ex, char* ws,
+        hipStream_t stream) {
     const Problem* table = (const Problem*)(ws + g.table);
     const int* ends = (const int*)(ws + g.ends);
     double* parts = (double*)(ws + g.parts);
     const int n = g.count;
     UNFLOW_LAUNCH((norm_kernel<T, STEP>), dim3(g.total[kNorm]), dim3(256), 0, stream, table, ends + kNorm * n, n, g.chunk, mu, nesterov, parts);
-    UNFLOW_LAUNCH((start_kernel<T, STEP>), dim3(g.total[kPack]), dim3(256), 0, stream, table, ends + kPack * n, n, (const double*)parts, mu, nesterov, eps, ex, ws);
+    UNFLOW_LAUNCH((start_kernel<T, STEP>), dim3(g.total[kPack]), dim3(256), 0, stream, table, ends + kPack * n, n, (const double*)parts, mu,
+        nesterov, eps, ex, ws);
     for (int k = 0; k < steps; ++k) {
         with_tile(g.size_s, [&](auto tile) {
             using TileT = decltype(tile);
             LAUNCH_TILES((square_kernel<TileT>), g.total[kSquare], table, ends + kSquare * n, n, ends + kSquareClass * n, ex, ws);
         });
-        if (g.total[kJoin]) UNFLOW_LAUNCH(join_kernel, dim3(g.total[kJoin]), dim3(256), 0, stream, table, ends + kJoin * n, n, kSizes[g.size_s], ex, ws);
+        if (g.total[kJoin]) UNFLOW_LAUNCH(join_kernel, dim3(g.total[kJoin]), dim3(256), 0, stream, table, ends + kJoin * n, n, kSizes[g.size_s], ex,
+            ws);
         with_tile(g.size_q, [&](auto tile) {
             using TileT = decltype(tile);
             LAUNCH_TILES((poly_kernel<TileT>), g.total[kPoly], table, ends + kPoly * n, n, ends + kPolyClass * n, a, b, c, ex, ws);
         });
         with_tile(g.size_x, [&](auto tile) {
             using TileT = decltype(tile);
-            if (k + 1 < steps) LAUNCH_TILES((apply_kernel<TileT, false, false, float>), g.total[kApply], table, ends + kApply * n, n, ends + kApplyClass * n, k & 1, ex, up, ws);
-            else LAUNCH_TILES((apply_kernel<TileT, true, STEP, T>), g.total[kApply], table, ends + kApply * n, n, ends + kApplyClass * n, k & 1, ex, up, ws);
+            if (k + 1 < steps) LAUNCH_TILES((apply_kernel<TileT, false, false, float>), g.total[kApply], table, ends + kApply * n, n,
+                ends + kApplyClass * n, k & 1, ex, up, ws);
+            else LAUNCH_TILES((apply_kernel<TileT, true, STEP, T>), g.total[kApply], table, ends + kApply * n, n, ends + kApplyClass * n, k & 1, ex,
+                up, ws);
         });
     }
 }
@@ -568,7 +582,8 @@ static int workspace_of(const unflow_matrix* a, int count, int dtype, long long*
 }
 
 template <bool STEP>
-static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca, float cb, float cc, float eps, float mu, int nesterov, Update up, void* workspace, long long workspace_bytes, void* stream_) {
+static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca, float cb, float cc, float eps, float mu, int nesterov, Update up,
+        void* workspace, long long workspace_bytes, void* stream_) {
     Exponents ex;
     UNFLOW_REQUIRE(exponents_of(steps, ca, cb, cc, ex));
     long long need = 0;
@@ -596,15 +611,18 @@ extern "C" int unflow_orthogonalize_workspace(const unflow_matrix* matrices, int
     return workspace_of(matrices, count, dtype, bytes);
 }
 
-extern "C" int unflow_orthogonalize(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace, long long workspace_bytes, void* stream) {
+extern "C" int unflow_orthogonalize(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, float eps,
+        void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(matrices_ok(matrices, count, dtype) && workspace && steps >= 1 && steps <= 64 && eps >= 0.f);
     for (int i = 0; i < count; ++i) UNFLOW_REQUIRE(matrices[i].x && matrices[i].out);
     return run<false>(matrices, count, dtype, steps, a, b, c, eps, 0.f, 0, Update{1.f, 0.f}, workspace, workspace_bytes, stream);
 }
 
-extern "C" int unflow_muon_step(const unflow_matrix* matrices, int count, int dtype, float lr, float momentum, float weight_decay, int nesterov, int steps, float a, float b, float c, float eps,
+extern "C" int unflow_muon_step(const unflow_matrix* matrices, int count, int dtype, float lr, float momentum, float weight_decay, int nesterov,
+        int steps, float a, float b, float c, float eps,
                                 void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(matrices_ok(matrices, count, dtype) && workspace && steps >= 1 && steps <= 64 && eps >= 0.f);
     for (int i = 0; i < count; ++i) UNFLOW_REQUIRE(matrices[i].x && matrices[i].out && matrices[i].momentum);
-    return run<true>(matrices, count, dtype, steps, a, b, c, eps, momentum, nesterov, Update{1.f - lr * weight_decay, lr}, workspace, workspace_bytes, stream);
+    return run<true>(matrices, count, dtype, steps, a, b, c, eps, momentum, nesterov, Update{1.f - lr * weight_decay, lr}, workspace,
+        workspace_bytes, stream);
 }

@@ -8,7 +8,8 @@ namespace {
 // What is read: rows x cols, `ld` elements from row to row.  A row r with label[r] == skip does not count (label == nullptr: every row does).
 struct Source { const void* p; long long ld; int rows, cols; const long long* label = nullptr; long long skip = 0; };
 
-template <class T> __device__ __forceinline__ f32x4 load4(const T* p, int n) {               // the first n = 0 .. 4 of four numbers, zeros behind them
+// the first n = 0 .. 4 of four numbers, zeros behind them
+template <class T> __device__ __forceinline__ f32x4 load4(const T* p, int n) {
     f32x4 v{0.f, 0.f, 0.f, 0.f};
     if (n >= 4 && ((size_t)p & (4 * sizeof(T) - 1)) == 0) {
         if constexpr (sizeof(T) == 4) return *reinterpret_cast<const f32x4*>(p);

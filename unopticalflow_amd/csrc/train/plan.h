@@ -11,7 +11,8 @@
 namespace {
 
 constexpr int kVariants = 6;
-constexpr int kSizes[kVariants] = {256, 192, 128, 64, 128, 64};             // of the variants of with_tile(): the last two with more stages in LDS, fewer on a CU
+// of the variants of with_tile(): the last two with more stages in LDS, fewer on a CU
+constexpr int kSizes[kVariants] = {256, 192, 128, 64, 128, 64};
 
 // m x n outputs (lower: the lower triangle of m x m) of `times` matrices, `out` bytes written for each; cut: may be cut into shares
 struct Job { long long m, n; int stages; bool lower, cut; double out; int times = 1; };
@@ -33,8 +34,10 @@ static long long lower_tiles_of(long long m, int size) { const long long t = (m 
 // full one from 60 % on), and of a unit's start and end.  (8192 x 8192 x 2048 against x 512, and
 // 1024 x 1024 x 4096; ONE and TWO planes)
 struct Cost { double full, alone, ends; int per_cu; };
-static const Cost kCost[2][kVariants] = {{{1.50, 1.10, 10., 1}, {0.97, 0.68, 7., 1}, {1.10, 0.62, 5., 2}, {0.80, 0.46, 4., 4}, {0.53, 0.45, 5., 1}, {0.35, 0.26, 4., 2}},
-                                         {{2.15, 1.50, 18., 1}, {1.28, 0.95, 11., 1}, {1.25, 0.60, 7.5, 2}, {0.83, 0.44, 4.8, 4}, {0.64, 0.54, 7.5, 1}, {0.44, 0.28, 4.5, 2}}};
+static const Cost kCost[2][kVariants] = {{{1.50, 1.10, 10., 1}, {0.97, 0.68, 7., 1}, {1.10, 0.62, 5., 2}, {0.80, 0.46, 4., 4}, {0.53, 0.45, 5., 1},
+        {0.35, 0.26, 4., 2}},
+                                         {{2.15, 1.50, 18., 1}, {1.28, 0.95, 11., 1}, {1.25, 0.60, 7.5, 2}, {0.83, 0.44, 4.8, 4}, {0.64, 0.54, 7.5,
+                                             1}, {0.44, 0.28, 4.5, 2}}};
 constexpr double kJoinBytesPerUs = 3.0e6, kLaunchUs = 5.0, kStoreBytesPerUs = 4.5e6 / 256.;          // joining: the chip; stores: a CU's part of it
 
 static Choice choose(int planes, const Job* jobs, int count) {
@@ -54,8 +57,10 @@ static Choice choose(int planes, const Job* jobs, int count) {
             double sum = 0., joined = 0., all = 0., longest_us = 0., least_us = 1e30, ends = 0.;
             for (int i = 0; i < count; ++i) {
                 const int shares = jobs[i].cut ? shares_of(jobs[i].stages, limit) : 1, each = (jobs[i].stages + shares - 1) / shares;
-                const double units = (double)jobs[i].times * (jobs[i].lower ? lower_tiles_of(jobs[i].m, kSizes[z]) : tiles_of(jobs[i].m, jobs[i].n, kSizes[z])) * shares;
-                const double area = (double)kSizes[z] * kSizes[z], end = c.ends + c.per_cu * area * (shares > 1 ? 4. : jobs[i].out) / kStoreBytesPerUs, us = each * c.full + end;
+                const double units = (double)jobs[i].times * (jobs[i].lower ? lower_tiles_of(jobs[i].m, kSizes[z]) : tiles_of(jobs[i].m, jobs[i].n,
+                    kSizes[z])) * shares;
+                const double area = (double)kSizes[z] * kSizes[z],
+                    end = c.ends + c.per_cu * area * (shares > 1 ? 4. : jobs[i].out) / kStoreBytesPerUs, us = each * c.full + end;
                 if (us > longest_us) { longest_us = us; most = each; ends = end; }
                 least = each < least ? each : least;
                 least_us = us < least_us ? us : least_us;

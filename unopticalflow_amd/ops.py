@@ -1770,6 +1770,7 @@ def prepare_triplets(images, img_hw, flips=None, device=None, src_is_rgb=True, s
 # ------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}            # UNFLOW_DTYPE_*
 _LCE_MAX_ROWS = _LCE_MAX_DIM = 1 << 20
+_LCE_MAX_CLASSES = 1 << 30
 _MATRIX_MAX_SIDE = 1 << 18
 _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
 
@@ -1868,9 +1869,9 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
         raise ValueError('linear_cross_entropy: target must be int64 of shape {}, got {} {}'.format(tuple(shape[:-1]), target.dtype, tuple(target.shape)))
     if target.device != hidden.device:
         raise RuntimeError('operands on different devices: %s vs %s' % (hidden.device, target.device))
-    if wshape[0] < 1 or not 1 <= wshape[1] <= _LCE_MAX_DIM or target.numel() > _LCE_MAX_ROWS or wshape[0] >= 1 << 31:
-        raise ValueError('linear_cross_entropy: at least one class, 1 to {} dimensions and at most {} rows; got {} rows, weight {}'.format(
-            _LCE_MAX_DIM, _LCE_MAX_ROWS, target.numel(), tuple(wshape)))
+    if not 1 <= wshape[0] <= _LCE_MAX_CLASSES or not 1 <= wshape[1] <= _LCE_MAX_DIM or target.numel() > _LCE_MAX_ROWS:
+        raise ValueError('linear_cross_entropy: 1 to {} classes, 1 to {} dimensions and at most {} rows; got {} rows, weight {}'.format(
+            _LCE_MAX_CLASSES, _LCE_MAX_DIM, _LCE_MAX_ROWS, target.numel(), tuple(wshape)))
     if len(shape) != 2:
         hidden, flat = hidden.reshape(-1, shape[-1]), target.reshape(-1)
     else:
