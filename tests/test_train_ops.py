@@ -270,6 +270,16 @@ def test_offsets_beyond_32_bits():
     assert bool(((dh.double() - p @ w.detach()[-2:].double()).abs() <= 2 * 2**-8 * (p.abs() @ w.detach()[-2:].double().abs()) + 2**-30).all())
 
 
+def test_no_second_derivative(device):
+    """The gradients are values: asking for theirs is an error, not a zero."""
+    h, w, t = _inputs(4, 7, 8, torch.float32, device)
+    h.requires_grad_()
+    loss = ops.linear_cross_entropy(h, w, t)
+    g, = torch.autograd.grad(loss, h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.square().sum().backward()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_captured_and_replayed(dtype):
@@ -668,6 +678,34 @@ def test_flow_muon_state_capture_and_checkpoint():
     part.proj.weight.grad = None
     popt.step()
     assert torch.equal(part.proj.weight, base.proj.weight) and not torch.equal(part.classes, base.classes)
+
+
+def test_flow_muon_checkpoint_of_bf16_weights(device):
+    """The momentum of a bf16 weight goes through a checkpoint in its 32 bits."""
+    g = torch.Generator().manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(9, 14, generator=g).bfloat16().to(device))
+    p.grad = torch.randn(9, 14, generator=g).bfloat16().to(device)
+    opt = optim.FlowMuon([p], lr=0.02)
+    opt.step()
+    q = torch.nn.Parameter(p.detach().clone())
+    resumed = optim.FlowMuon([q], lr=0.02)
+    resumed.load_state_dict(copy.deepcopy(opt.state_dict()))
+    momentum = opt.state[p]['momentum_buffer']
+    assert momentum.dtype == torch.float32 and not torch.equal(momentum, momentum.bfloat16().float())
+    assert torch.equal(resumed.state[q]['momentum_buffer'], momentum)
+    q.grad = p.grad.clone()
+    opt.step()
+    resumed.step()
+    assert torch.equal(p, q)
+
+
+def test_a_momentum_is_not_its_parameter():
+    import train_on_host
+    with train_on_host.patched():
+        p, g = torch.ones(3, 4), torch.ones(3, 4)
+        with pytest.raises(ValueError):
+            optim.muon_step_([p], [g], [p], lr=0.1)
+        assert torch.equal(p, torch.ones(3, 4))
 
 
 @pytest.mark.gpu

@@ -47,7 +47,8 @@ __device__ __forceinline__ float wave_largest(float m) {
 __device__ __forceinline__ int exponent_for(float largest) { return largest > 0.f ? 14 - ilogbf(largest) : 0; }
 
 // H and W into packed rows, one launch: the first `blocks_h` workgroups take H (0: H needs no packing), the rest W; a wave takes a row at a time.
-// fp32: the rows' exponents, and the workgroups' largest finite magnitudes of the rows that count (maxima [2][kMaxima]).
+// fp32: the rows' exponents, and the workgroups' largest finite magnitudes of the rows that count (maxima [2][kMaxima]).  Bound by bytes: 11020 rows
+// of 777 fp32 numbers 24 us (34 MB read, 35 written).
 struct Packed { u16 *h, *w; int *eh, *ew; float* maxima; };
 template <class T, int PL, int EL>
 __global__ __launch_bounds__(256) void pack_inputs_kernel(Source h, Source w, int blocks_h, Packed to, long long ldd, int width) {
@@ -93,7 +94,8 @@ template <int PL> __device__ __forceinline__ f32x4 logits_of(const Logits& l, f3
 }
 
 // ---- forward: of each row of a tile of z the maximum (times log2(e), as all that follows) and the sum of exp(z - maximum) over the classes that
-// are not the row's target, and the target's z.  partial [tile column][N]
+// are not the row's target, and the target's z.  partial [tile column][N].  Bound by the matrix instructions, and for short rows by what a tile's
+// end costs: 8192 rows, 131072 classes of 4096 bf16 6.70 ms = 1313 TFLOP/s; 4096, 32000 of 2048 518 us = 1036; fp32 1013, 10007 of 777 57 us = 276.
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand H, Operand W, int width, Logits how,
         const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
@@ -105,7 +107,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
     tile_of(xcd_remap(id, total), mt, nt, tm, tn);
     TileT T;
     T.start(H, W, 0, width, tm * TileT::BM, tn * TileT::BN, lds);
-    // a workgroup goes through tiles a grid apart: the copies of the next one are under way while this one's sums are dealt with
+    // A workgroup goes through tiles a grid apart: the copies of the next one are under way while this one's sums are dealt with (4 % of 4096 rows,
+    // 32000 classes of 2048).
     for (bool more = true; more;) {
         T.finish(lds);
         const int m0 = tm * TileT::BM, n0 = tn * TileT::BN, column = tn;
@@ -119,7 +122,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
 #pragma unroll
         for (int i = 0; i < TileT::MI; ++i) {
             const int m = m0 + TileT::row(i);
-            const long long t = m < H.rows ? target[m] - n0 : -1;                            // the target's place in this tile
+            const long long t = m < H.rows ? target[m] - n0 : -1;                        // the target's place in this tile
             const int own = t >= 0 && t < TileT::BN && t + n0 < W.rows ? (int)t : -1, eh = TileT::PL == TWO && m < H.rows ? how.eh[m] : 0;
             float top = -INFINITY;
 #pragma unroll
@@ -173,7 +176,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
 // ---- forward of few rows (at most 16 NF): reading W is all there is to it.  16-bit inputs of more than 16 rows are better served by the tiles
 // above, where the four waves share the rows of H (61 rows against 50257 classes of 1024 fp16: 20 us against 36); fp32 inputs stay here up to 64
 // rows, for packing W would read and write all of it once more (50257 classes of 1024 dimensions, whole calls: 16 rows 58 us against 200 through
-// the tiles, 33 rows 112 against 204, 64 rows 126 against 212; 5000 of 256: 15 against 18).  A workgroup takes 16 CF classes, its four waves a quarter of D each, AHEAD
+// the tiles, 33 rows 112 against 204, 64 rows 126 against 212; 5000 of 256: 15 against 18).  One row, 32000 classes of 2048 bf16: 23 us =
+// 5.7 TB/s.  A workgroup takes 16 CF classes, its four waves a quarter of D each, AHEAD
 // steps of loads in flight; the rows of W go from memory to the matrix instruction as they lie there.  16-bit numbers: 32 k a step, lane l holds
 // k = 8 (l >> 4) .. of row l & 15.  fp32: 16 k a step as four v_mfma_f32_16x16x4_f32, the e-th taking k = 4 (l >> 4) + e -- fp32 arithmetic
 // throughout, and no packing.
@@ -189,7 +193,7 @@ template <class T> __device__ __forceinline__ f32x4 few_product(uint4 a, uint4 b
 template <class T, int NF, int CF, int AHEAD>
 __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, long long ldh, const T* __restrict__ W, long long ldw, int N, int V,
         int D, float scale, const long long* __restrict__ target,
-                                                      float2* __restrict__ partial, float* __restrict__ ztarget) {
+        float2* __restrict__ partial, float* __restrict__ ztarget) {
     constexpr int ROWS = 16 * NF, PER = 256 / ROWS, CLASSES = 16 * CF / PER, PITCH = 16 * CF + 2;
     __shared__ float sums[4][ROWS][PITCH];
     const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -262,9 +266,22 @@ __device__ __forceinline__ float2 joined(float2 x, float2 y) {
     const float both = fmaxf(x.x, y.x), base = both == -INFINITY ? 0.f : both;
     return make_float2(both, x.y * (x.x == -INFINITY ? 1.f : exp2_of(x.x - base)) + y.y * (y.x == -INFINITY ? 1.f : exp2_of(y.x - base)));
 }
+// the pairs of row m of the tiles first, first + step, ..; the loads of eight are under way together
+__device__ __forceinline__ float2 joined_tiles(const float2* __restrict__ partial, int first, int step, int tiles, int N, int m) {
+    float2 pair = make_float2(-INFINITY, 0.f);
+    for (int t = first; t < tiles; t += 8 * step) {
+        float2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = t + k * step < tiles ? partial[(long long)(t + k * step) * N + m] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) pair = joined(pair, v[k]);
+    }
+    return pair;
+}
 // A row's statistics and loss from its joined pair.  The target's own term joins here: where it outweighs the others, loss = log1p(others / own)
 // and others / all = 1 - p keep the digits that 1 - p would lose.
-__device__ __forceinline__ float row_of(float2 pair, long long t, long long ignore, int V, const float* __restrict__ ztarget, Row* __restrict__ stats) {
+__device__ __forceinline__ float row_of(float2 pair, long long t, long long ignore, int V, const float* __restrict__ ztarget,
+        Row* __restrict__ stats) {
     const float base = pair.x == -INFINITY ? 0.f : pair.x, others = pair.y;
     const bool known = t >= 0 && t < V;
     const float zt = known ? *ztarget : -INFINITY, own = known ? exp2_of(zt - base) : 0.f, all = others + own;
@@ -272,17 +289,15 @@ __device__ __forceinline__ float row_of(float2 pair, long long t, long long igno
     return t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) * kLn2 + logf(all);
 }
 
-// the tiles' pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup
+// the tiles' pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup.  4 to 6 us: the latency of a launch and of
+// its loads
 template <int R>
-__global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict__ partial, int tiles, int N, int V, const long long* __restrict__ target,
-        long long ignore, const float* __restrict__ ztarget, Row* __restrict__ stats, float* __restrict__ losses) {
+__global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict__ partial, int tiles, int N, int V,
+        const long long* __restrict__ target, long long ignore, const float* __restrict__ ztarget, Row* __restrict__ stats, float* __restrict__ losses) {
     constexpr int SHARES = 256 / R;
     __shared__ float2 part[SHARES][R + 1];
     const int r = threadIdx.x % R, share = threadIdx.x / R, m = blockIdx.x * R + r;
-    float2 pair = make_float2(-INFINITY, 0.f);
-    if (m < N)
-        for (int t = share; t < tiles; t += SHARES) pair = joined(pair, partial[(long long)t * N + m]);
-    part[share][r] = pair;
+    part[share][r] = m < N ? joined_tiles(partial, share, SHARES, tiles, N, m) : make_float2(-INFINITY, 0.f);
     __syncthreads();
     for (int half = SHARES / 2; half > 0; half /= 2) {
         if (share < half) part[share][r] = joined(part[share][r], part[share + half][r]);
@@ -306,8 +321,8 @@ __device__ __forceinline__ void reduce_losses(float s, float c, int mean, float*
         loss[0] = mean ? s / fmaxf(c, 1.f) : s;
     }
 }
-__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restrict__ losses, const long long* __restrict__ target, long long ignore, int N,
-        int mean, float* __restrict__ loss, float* __restrict__ count) {
+__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* __restrict__ losses, const long long* __restrict__ target, long long ignore,
+        int N, int mean, float* __restrict__ loss, float* __restrict__ count) {
     float s = 0.f, c = 0.f;
     for (int i = threadIdx.x; i < N; i += 1024) {
         s += losses[i];
@@ -322,10 +337,8 @@ __global__ __launch_bounds__(1024) void lce_join_reduce_kernel(const float2* __r
     const int m = threadIdx.x;
     float s = 0.f, c = 0.f;
     if (m < N) {
-        float2 pair = make_float2(-INFINITY, 0.f);
-        for (int t = 0; t < tiles; ++t) pair = joined(pair, partial[(long long)t * N + m]);
         const long long t = target[m];
-        s = row_of(pair, t, ignore, V, ztarget + m, stats + m);
+        s = row_of(joined_tiles(partial, 0, 1, tiles, N, m), t, ignore, V, ztarget + m, stats + m);
         c = t != ignore ? 1.f : 0.f;
     }
     reduce_losses(s, c, mean, loss, count);
@@ -358,7 +371,7 @@ __global__ __launch_bounds__(1024) void lce_largest_upstream_kernel(Upstream u, 
 }
 
 // Transposes of a piece of W and (with the first piece) of H, one launch: the first `blocks_w` workgroups take W.  fp32: with the exponent of the
-// largest of the `counts` magnitudes that packing noted, left in `ex`.
+// largest of the `counts` magnitudes that packing noted, left in `ex`.  Bound by bytes: 8192 classes of 4096 bf16 31 us = 4.3 TB/s.
 struct Columns { Source s; u16* dst; long long ldd; int width; const float* maxima; int counts; };
 template <class T, int PL, int EL>
 __global__ __launch_bounds__(256) void pack_transposes_kernel(Columns w, Columns h, int blocks_w, Exponents* __restrict__ ex) {
@@ -383,11 +396,12 @@ __global__ __launch_bounds__(256) void pack_transposes_kernel(Columns w, Columns
 template <int EL> __host__ __device__ constexpr int probability_exponent() { return EL == FP16 ? 14 : 0; }
 
 // a piece of G and of its transpose: classes [v0, v0 + vp).  G [N][packed vp] holds p - [v = t] (0 where the row is ignored), GT [vp][packed N] the
-// same times the row's upstream gradient relative to the largest; columns behind N and vp up to the packed width are zero
+// same times the row's upstream gradient relative to the largest; columns behind N and vp up to the packed width are zero.  Bound by the matrix
+// instructions, and then by its stores: 8192 rows, 8192 classes of 4096 bf16 460 us = 1195 TFLOP/s, 268 MB of it written.
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand H, Operand W, int width, Logits how,
         const Row* __restrict__ stats, Upstream up, int v0, int vp, int V, u16* __restrict__ G, long long ldg,
-                                                                                                     u16* __restrict__ GT, long long ldgt) {
+        u16* __restrict__ GT, long long ldgt) {
     constexpr int PL = TileT::PL, EL = TileT::EL;
     UNFLOW_DYNAMIC_LDS(char, lds);
     const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(vp, TileT::BN);
@@ -443,7 +457,7 @@ template <int BM, int BN, int WM, int WN, int DP> struct OutputOf<Tile<BM, BN, W
 
 // The two products of a piece, one launch: job 0 is dH += G W, job 1 dW = G^T H.  C = A B^T in `shares` shares of what is summed.  A job without
 // `sums` is one share and goes to the gradient as it is; else the shares' accumulators go to fp32 sums [shares][rows of A][ldc], added to what
-// is there unless it is the first piece.
+// is there unless it is the first piece.  Bound by the matrix instructions: both products of that piece 875 us = 1257 TFLOP/s.
 struct Product { Operand A, B; int width, shares, tiles; float* sums; long long ldc; int first; void* out; int by_h; };
 
 // what turns a job's sums into gradients: the uniform factor, and the row's own (dH; for dW it is in GT, relative to the largest)
@@ -509,7 +523,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product
     }
 }
 
-// gradients = sums over the shares, in order, times the factors; one launch for the jobs that have sums (blocks of the first, then of the second)
+// gradients = sums over the shares, in order, times the factors; one launch for the jobs that have sums (blocks of the first, then of the second).
+// Bound by bytes: 4096 x 2048 to bf16 10.5 us = 4.8 TB/s.
 template <class T_, int PL, int EL>
 __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, int blocks_a, const Exponents* __restrict__ ex, Upstream up) {
     const bool second = (int)blockIdx.x >= blocks_a;
@@ -779,8 +794,7 @@ static bool sizes_ok(long long ldh, long long ldw, int N, int V, int D, int dtyp
 }  // namespace
 
 extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype,
-        int need_dhidden, int need_dweight,
-                                          long long* kept_bytes, long long* forward_bytes, long long* backward_bytes) {
+        int need_dhidden, int need_dweight, long long* kept_bytes, long long* forward_bytes, long long* backward_bytes) {
     UNFLOW_REQUIRE(kept_bytes && forward_bytes && backward_bytes && sizes_ok(ldh, ldw, N, V, D, dtype, 0));
     const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, need_dhidden || need_dweight, need_dhidden != 0, need_dweight != 0);
     *kept_bytes = p.kept_bytes;
@@ -790,9 +804,8 @@ extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, con
 }
 
 extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V,
-        int D, int dtype, float scale,
-                                    long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes,
-                                        void* stream) {
+        int D, int dtype, float scale, long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes,
+        void* stream) {
     UNFLOW_REQUIRE(hidden && weight && target && loss && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
     const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, false, false, false);
     UNFLOW_REQUIRE(workspace_bytes >= p.forward_bytes);
@@ -805,9 +818,8 @@ extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const voi
 }
 
 extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
-        const float* gout, int N, int V, int D,
-                                    int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept,
-                                        void* workspace, long long workspace_bytes, void* stream) {
+        const float* gout, int N, int V, int D, int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight,
+        const void* kept, void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(hidden && weight && target && gout && (dhidden || dweight) && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
     const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, true, dhidden != nullptr, dweight != nullptr);
     UNFLOW_REQUIRE(workspace_bytes >= p.backward_bytes);

@@ -73,8 +73,8 @@ template <int PL, int EL> __device__ __forceinline__ f32x4 unpack4(const u16* p,
 }
 
 template <int EL> __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
-    if constexpr (EL == BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-        0);
+    if constexpr (EL == BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+        0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
@@ -127,9 +127,8 @@ struct Tile {
     __device__ __forceinline__ void start(const Operand& A, const Operand& B, int k0, int k1, int m0, int n0, char* lds) {
         const int w = wave(), lane = (int)threadIdx.x & 63;
         const int piece = (lane & 7) ^ (((4 * (w & 1)) + (lane >> 4)) & 7);          // of the row 8 q + lane / 8, q = w + WAVES i
-        // The ranges end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most 256 rows
-        // of
-        // at most 2^21 numbers: its bytes stay below 2^31.)
+        // The ranges end with the operand's (or the tile's) last row, so rows behind it read as zero by themselves.  (A tile spans at most
+        // 256 rows of at most 2^21 numbers: its bytes stay below 2^31.)
         const int ra = A.rows - m0 < BM ? A.rows - m0 : BM, rb = B.rows - n0 < BN ? B.rows - n0 : BN;
         range_a = range_of(A.p + (long long)m0 * A.ld, (int)(ra * A.ld * 2));
         range_b = range_of(B.p + (long long)n0 * B.ld, (int)(rb * B.ld * 2));
@@ -164,8 +163,7 @@ struct Tile {
         // The operand reads of one half of a stage and the copies of the stage after the next run under the matrix instructions, a few behind every
         // row of the wave's part: issued together they would fill their queues and hold up the wave.  No wave waits for LDS or memory but at
         // the one barrier of a stage, by which its reads of stage t have arrived, its copies of stage t + 1 are in LDS (they had DEPTH - 1
-        // stages' time),
-        // and the buffer of stage t may be written again.
+        // stages' time), and the buffer of stage t may be written again.
         uint4 a0[MI], b0[NI], a1[MI], b1[NI];
         constexpr int READS = MI + NI, EACH_READ = (READS + MI - 2) / (MI - 1), EACH_COPY = (QA + QB + MI - 1) / MI;
         auto read = [&](uint4* a, uint4* b, const char* s, int p, int r) {                      // read r of READS

@@ -87,7 +87,8 @@ __device__ __forceinline__ int dealt_problem_of(const int* __restrict__ ends, in
 
 __device__ __forceinline__ float direction(float g, float m, float mu, int nesterov) { return nesterov ? g + mu * (m - g) : m; }
 
-// ---- sum of squares of a chunk of `size` numbers (after the momentum's update)
+// ---- sum of squares of a chunk of `size` numbers (after the momentum's update).  Bound by bytes: 16 bf16 weights
+// of 1024 x 1024, four of 4096 x 1024 and four of 1024 x 4096 (50 million numbers) with their momenta 91 us = 5.5 TB/s
 template <class T, bool STEP>
 __global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size, float mu,
         int nesterov, double* __restrict__ parts) {
@@ -128,11 +129,11 @@ __global__ __launch_bounds__(256) void norm_kernel(const Problem* __restrict__ t
     if (threadIdx.x == 0) parts[p.part0 + chunk] = red[0];
 }
 
-// ---- X_0 and its transpose, as planes: a 64 x 64 tile of the matrix per workgroup, both ways
+// ---- X_0 and its transpose, as planes: a 64 x 64 tile of the matrix per workgroup, both ways.  Bound by bytes: the same weights 148 us = 4.8 TB/s
 template <class T, bool STEP>
 __global__ __launch_bounds__(256) void start_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
         const double* __restrict__ parts, float mu, int nesterov, float eps,
-                                                    Exponents ex, char* __restrict__ ws) {
+        Exponents ex, char* __restrict__ ws) {
     __shared__ float tile[64][65];
     __shared__ double red[256];
     int id;
@@ -210,7 +211,8 @@ __device__ __forceinline__ void symmetric_store(TileT& T, char* lds, u16* __rest
     if (tm != tn) T.store_transposed(lds, p, ld, m, ld, tm * TileT::BM, tn * TileT::BN, value);
 }
 
-// ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves fp32 tiles for join_kernel
+// ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves fp32 tiles for join_kernel.  Bound by the matrix
+// instructions: 4096 x 4096 192 us = 1120 TFLOP/s of fp16 products (three for one of fp32)
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
         const int* __restrict__ classes, Exponents ex, char* __restrict__ ws) {
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem
     const float f = ldexpf(1.f, ex.s - 2 * ex.x);
     symmetric_store(T, lds, (u16*)(ws + p.S), lds_, p.m, tm, tn, [&](int i, int j) { return T.acc[i][j] * f; });
 }
-// (64 x 64 of a tile of side `size` per workgroup)
+// (64 x 64 of a tile of side `size` per workgroup; 5 to 7 us, the latency of a launch and of its loads)
 __global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, int size,
         Exponents ex, char* __restrict__ ws) {
     __shared__ float tile[64][65];
@@ -278,11 +280,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ t
     }
 }
 
-// ---- Q = a I + b S + c S S: lower tiles
+// ---- Q = a I + b S + c S S: lower tiles.  Bound by the matrix instructions: 4096 x 4096 200 us
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
         const int* __restrict__ classes, float a, float b, float c, Exponents ex,
-                                                                                             char* __restrict__ ws) {
+        char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
     const Problem p = table[dealt_problem_of(ends, count, classes, id)];
@@ -307,12 +309,14 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* 
     symmetric_store(T, lds, (u16*)(ws + p.Q), ld, p.m, tm, tn, [&](int i, int j) { return T.acc[i][j]; });
 }
 
-// ---- X <- Q X.  LAST: the output, or the parameter's update
+// ---- X <- Q X.  LAST: the output, or the parameter's update.  Bound by the matrix instructions (4096 x 4096 335 us = 1230 TFLOP/s of fp16
+// products), for the weights above as much by writing X both ways (343 us = 900 TFLOP/s, 400 MB written): S sums over the columns of X and the next
+// X over its rows, and both operands of a product lie along what is summed
 struct Update { float keep, lr; };                                   // 1 - lr wd, lr
 template <class TileT, bool LAST, bool STEP, class T>
 __global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
         const int* __restrict__ classes, int odd, Exponents ex, Update up,
-                                                                                              char* __restrict__ ws) {
+        char* __restrict__ ws) {
     UNFLOW_DYNAMIC_LDS(char, lds);
     int id, tm, tn;
     const Problem p = table[dealt_problem_of(ends, count, classes, id)];
@@ -398,8 +402,8 @@ struct Group {
 };
 
 static long long plane_bytes(long long m, long long n) {
-    return round_up(2 * packed_width(TWO, n) * m, 256) + 2 * round_up(2 * packed_width(TWO, m) * n, 256) + 2 * round_up(2 * packed_width(TWO,
-        m) * m, 256);
+    const long long wm = packed_width(TWO, m), wn = packed_width(TWO, n);
+    return round_up(2 * wn * m, 256) + 2 * round_up(2 * wm * n, 256) + 2 * round_up(2 * wm * m, 256);
 }
 
 constexpr int kMost = 1024;                                          // matrices of one group
@@ -620,7 +624,7 @@ extern "C" int unflow_orthogonalize(const unflow_matrix* matrices, int count, in
 
 extern "C" int unflow_muon_step(const unflow_matrix* matrices, int count, int dtype, float lr, float momentum, float weight_decay, int nesterov,
         int steps, float a, float b, float c, float eps,
-                                void* workspace, long long workspace_bytes, void* stream) {
+        void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(matrices_ok(matrices, count, dtype) && workspace && steps >= 1 && steps <= 64 && eps >= 0.f);
     for (int i = 0; i < count; ++i) UNFLOW_REQUIRE(matrices[i].x && matrices[i].out && matrices[i].momentum);
     return run<true>(matrices, count, dtype, steps, a, b, c, eps, momentum, nesterov, Update{1.f - lr * weight_decay, lr}, workspace,

@@ -29,8 +29,7 @@ template <class T> __device__ __forceinline__ f32x4 load4(const T* p, int n) {
 __device__ __forceinline__ f32x4 scaled(f32x4 v, int e) { return f32x4{ldexpf(v[0], e), ldexpf(v[1], e), ldexpf(v[2], e), ldexpf(v[3], e)}; }
 
 // dst row c = source column c times 2^e, for the `cols` columns; `width` >= rows numbers a dst row holds, zeros behind rows and for rows that do
-// not count.  The 64 x 64 tile (bx, by) of
-// ceil(width / 64) x ceil(cols / 64)
+// not count.  The 64 x 64 tile (bx, by) of ceil(width / 64) x ceil(cols / 64)
 template <class T, int PL, int EL>
 __device__ __forceinline__ void pack_columns_tile(const Source& s, int e, u16* __restrict__ dst, long long ldd, int width, int bx, int by) {
     __shared__ float tile[64][65];

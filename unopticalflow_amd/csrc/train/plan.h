@@ -31,13 +31,11 @@ static long long tiles_of(long long m, long long n, int size) { return ((m + siz
 static long long lower_tiles_of(long long m, int size) { const long long t = (m + size - 1) / size; return t * (t + 1) / 2; }
 
 // Measured: microseconds of one stage of a unit on a full chip (of the units that share a CU, together) and on an empty one (a chip is as slow as a
-// full one from 60 % on), and of a unit's start and end.  (8192 x 8192 x 2048 against x 512, and
-// 1024 x 1024 x 4096; ONE and TWO planes)
+// full one from 60 % on), and of a unit's start and end.  (8192 x 8192 x 2048 against x 512, and 1024 x 1024 x 4096; ONE and TWO planes)
 struct Cost { double full, alone, ends; int per_cu; };
-static const Cost kCost[2][kVariants] = {{{1.50, 1.10, 10., 1}, {0.97, 0.68, 7., 1}, {1.10, 0.62, 5., 2}, {0.80, 0.46, 4., 4}, {0.53, 0.45, 5., 1},
-        {0.35, 0.26, 4., 2}},
-                                         {{2.15, 1.50, 18., 1}, {1.28, 0.95, 11., 1}, {1.25, 0.60, 7.5, 2}, {0.83, 0.44, 4.8, 4}, {0.64, 0.54, 7.5,
-                                             1}, {0.44, 0.28, 4.5, 2}}};
+static const Cost kCost[2][kVariants] = {
+    {{1.50, 1.10, 10., 1}, {0.97, 0.68, 7., 1}, {1.10, 0.62, 5., 2}, {0.80, 0.46, 4., 4}, {0.53, 0.45, 5., 1}, {0.35, 0.26, 4., 2}},
+    {{2.15, 1.50, 18., 1}, {1.28, 0.95, 11., 1}, {1.25, 0.60, 7.5, 2}, {0.83, 0.44, 4.8, 4}, {0.64, 0.54, 7.5, 1}, {0.44, 0.28, 4.5, 2}}};
 constexpr double kJoinBytesPerUs = 3.0e6, kLaunchUs = 5.0, kStoreBytesPerUs = 4.5e6 / 256.;          // joining: the chip; stores: a CU's part of it
 
 static Choice choose(int planes, const Job* jobs, int count) {

@@ -1830,6 +1830,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         hidden, weight, target, kept = ctx.saved_tensors
         (ignore_index, scale, reduction), (ldh, ldw, dtype, need) = ctx.options, ctx.how

@@ -203,7 +203,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
             g = torch.empty_like(p).copy_(g)
             copied.append(g)
         items.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), rows, cols))
-    if len({x[1] for x in items}) < len(items) or len({x[2] for x in items}) < len(items):
+    if len({x[1] for x in items} | {x[2] for x in items}) < 2 * len(items):
         raise ValueError('muon_step_: a parameter or momentum appears twice')
     ops._newton_schulz('unflow_muon_step', dev, dtype, (ops._Matrix * len(items))(*items), len(items),
                        (float(lr), float(momentum), float(weight_decay), int(bool(nesterov)), steps, *coefficients, float(eps)))
@@ -212,8 +212,8 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
 class FlowMuon(torch.optim.Optimizer):
     """Muon for the weights of two or more dimensions (``muon_step_``), Adam (``FlowAdam``) for everything else.
 
-    ``params`` is a list of parameters; it becomes two groups: 'matrices' (``lr``, ``momentum``, ``nesterov``, ``weight_decay``) and 'others' (``adam_lr``, betas, eps).  Momentum
-    is kept in fp32 whatever the parameters' type.  Like FlowAdam it can be captured into a hipGraph once ``prepare()`` has created its state."""
+    ``params`` is a list of parameters; it becomes two groups: 'matrices' (``lr``, ``momentum``, ``nesterov``, ``weight_decay``) and 'others'
+    (``adam_lr`` as their ``lr``; betas and eps are FlowAdam's own).  Momentum is kept in fp32 whatever the parameters' type.  Like FlowAdam it can be captured into a hipGraph once ``prepare()`` has created its state."""
 
     def __init__(self, params, lr=0.02, adam_lr=1e-4, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
         params = [p for p in params]
@@ -244,10 +244,12 @@ class FlowMuon(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
-        for p in self._matrices():
-            if p in self.state:                # Optimizer.load_state_dict casts to the parameter's type
-                m = self.state[p]['momentum_buffer']
-                self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(m)
+        # (Optimizer.load_state_dict has cast the momentum to the parameter's type: taken again from what was given)
+        given = [i for g in state_dict['param_groups'] for i in g['params']]
+        kept = [p for g in self.param_groups for p in g['params']]
+        for i, p in zip(given, kept):
+            if p.dim() >= 2 and p in self.state:
+                self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(state_dict['state'][i]['momentum_buffer'])
         self._share()
         if self._adam is not None:
             self._adam._tables = None
