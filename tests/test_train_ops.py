@@ -109,6 +109,30 @@ def test_loss_and_gradients(device, dtype, rows, vocab, dim, reduction, scale):
     _check_lce(h, w, t, dtype, reduction, scale)
 
 
+@pytest.mark.parametrize('rows,vocab,dim,scale', [(60, 90, 16, 14.0), (33, 200, 100, 1.0), (3, 40, 8, 2.0), (20, 50, 33, -3.0)])
+@pytest.mark.parametrize('spread', [1.0, 2.0**-60, 2.0**60])
+def test_gradients_of_bf16_inputs_are_rounded_to_bf16_once(device, rows, vocab, dim, scale, spread):
+    """What is summed holds 11 bits (two factors: 2^-11 of a term each at most, and 2^-39 of the largest), whatever the inputs' magnitudes: the
+    output's own eps / 2 = 2^-8 is the only rounding to bf16."""
+    h, w, t = _inputs(rows, vocab, dim, torch.bfloat16, device, ignored=0.2 if rows > 4 else 0.0)
+    h, w = h * spread, w / spread
+    h[t < 0] = 3e38                                       # (an ignored row has no part in any scale)
+    h.requires_grad_()
+    w.requires_grad_()
+    dh, dw = torch.autograd.grad(ops.linear_cross_entropy(h, w, t, scale=scale, reduction='sum'), (h, w))
+    hd, wd, used = h.detach().double().where((t >= 0)[:, None], 0), w.detach().double(), t >= 0
+    z = scale * (hd @ wd.T)
+    dz = abs(scale) * (dim * 2**-24 + 2**-20) * float((hd.abs() @ wd.abs().T).max())
+    loose = 2 * dz + (2 * float(z.abs().max()) + 128) * 2**-23
+    p = z.softmax(1)
+    g = (p - torch.zeros_like(p).scatter_(1, t.where(used, 0)[:, None], 1.0)) * used[:, None] * scale
+    off = ((p * loose + 2**-23) * abs(scale) + g.abs() * _u(torch.float16) + 2**-39 * abs(scale)) * used[:, None]
+    for got, a, b, error in ((dh, g, wd, off), (dw, g.T, hd, off.T)):
+        exact, size = a @ b, a.abs() @ b.abs()
+        bound = error @ b.abs() + size * (a.shape[1] * 2**-24 + _u(torch.float16)) + a.abs().sum(1, keepdim=True) * float(b.abs().max()) * 2**-38 + _u(torch.bfloat16) * exact.abs()
+        assert bool(((got.double() - exact).abs() <= bound).all()), float(((got.double() - exact).abs() / (bound + 2.0**-200)).max())
+
+
 @pytest.mark.parametrize('rows,vocab,reduction', [(1024, 40, 'mean'), (1025, 40, 'mean'), (5, 2200, 'sum'), (300, 2200, 'mean'), (40, 2048, 'sum')])
 def test_rows_and_tiles_joined_in_one_launch_or_two(device, rows, vocab, reduction):
     """Up to 1024 rows of up to 32 tiles, and more of either."""

@@ -9,9 +9,12 @@
 //
 // What bounds it: the matrix products, 2 N V D operations forward and 8 N V D for the three of the backward pass with z recomputed (6 N V D
 // where z could be kept); reading W bounds the forward pass of few rows.  Numbers: 16-bit inputs go to the matrix instructions as they are;
-// fp32 inputs as two fp16 planes scaled by the largest magnitude (mfma16.h).  G keeps the type of the products: for bf16 inputs its rounding
-// (2^-9 of every element, at random) is of the size of the gradients' own rounding; the uniform factors of G (scale, the upstream gradient of a
-// reduced loss) are applied to the sums, so that -1 at the target stays exact.
+// fp32 inputs as two fp16 planes scaled by the largest magnitude (mfma16.h).  G is held in fp16 (two planes for fp32) times 2^14: 11 (22) bits of
+// every probability down to 2^-28 (2^-17).  For bf16 inputs its own 8 bits would do as far as the products go, but where a gradient's sum cancels
+// they show: 9246 rows against 9246 classes of 32, scale 14, came out 1.6 times as far off as the rounding of the gradients to bf16 alone.  The
+// other operands of these products, transposes that are written anyhow, are then fp16 as well, times the power of two that brings the largest
+// magnitude to [2^14, 2^15); to find it bf16 inputs are read once more.  The uniform factors of G (scale, the upstream gradient of a reduced loss)
+// are applied to the sums.
 //
 // A row whose target is `ignore_index` has loss 0 and no gradient, whatever its hidden row holds (it is left out of the largest magnitude, and
 // enters the transposed H as zeros: 0 * NaN never meets a sum).  Any other target outside [0, V) makes its row's loss and gradients NaN.
@@ -345,6 +348,44 @@ __global__ __launch_bounds__(1024) void lce_join_reduce_kernel(const float2* __r
 }
 
 // ---- backward
+// The largest finite magnitudes that workgroups meet in bf16 inputs as pack_inputs_kernel notes them for fp32 ones (rows of 16-byte pieces, zeros
+// behind the last number).  A wave takes a row at a time, four pieces a lane under way together.  Bound by bytes.
+__global__ __launch_bounds__(256) void lce_magnitudes_kernel(Operand h, Operand w, int pieces, int blocks_h, const long long* __restrict__ target,
+        long long ignore, float* __restrict__ maxima) {
+    __shared__ unsigned red[4];
+    const bool second = (int)blockIdx.x >= blocks_h;
+    const Operand s = second ? w : h;
+    const int block = (int)blockIdx.x - (second ? blocks_h : 0), blocks = second ? (int)gridDim.x - blocks_h : blocks_h;
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    unsigned top = 0;                                                    // magnitudes of bf16 numbers order as their bits
+    auto meet = [&](unsigned bits) { top = bits < 0x7f80u && bits > top ? bits : top; };
+    for (int r = block * 4 + wave; r < s.rows; r += blocks * 4) {
+        if (!second && target[r] == ignore) continue;
+        const uint4* row = reinterpret_cast<const uint4*>(s.p + (long long)r * s.ld);
+        for (int k = lane; k < pieces; k += 256) {
+            uint4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = k + 64 * u < pieces ? row[k + 64 * u] : uint4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const unsigned e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    meet(e[i] & 0x7fffu);
+                    meet(e[i] >> 16 & 0x7fffu);
+                }
+            }
+        }
+    }
+    const float all = wave_largest(__builtin_bit_cast(float, top << 16));
+    if (lane == 0) red[wave] = __builtin_bit_cast(unsigned, all);        // (positive floats order as their bits)
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int q = 1; q < 4; ++q) red[0] = red[q] > red[0] ? red[q] : red[0];
+        maxima[(second ? kMaxima : 0) + block] = __builtin_bit_cast(float, red[0]);
+    }
+}
+
 // The upstream gradient: one number for a reduced loss, one per row for reduction none (these relative to the largest, so that fp16 planes hold
 // them).
 struct Upstream { const float* g; const float* largest; const float* count; const long long* target; long long ignore; int reduction; float scale; };
@@ -370,17 +411,18 @@ __global__ __launch_bounds__(1024) void lce_largest_upstream_kernel(Upstream u, 
     }
 }
 
-// Transposes of a piece of W and (with the first piece) of H, one launch: the first `blocks_w` workgroups take W.  fp32: with the exponent of the
-// largest of the `counts` magnitudes that packing noted, left in `ex`.  Bound by bytes: 8192 classes of 4096 bf16 31 us = 4.3 TB/s.
+// Transposes of a piece of W and (with the first piece) of H, one launch: the first `blocks_w` workgroups take W.  All but fp16, which goes as it
+// is: with the exponent of the largest of the `counts` magnitudes that were noted, left in `ex`.  Bound by bytes: 8192 classes of 4096 bf16 31 us = 4.3 TB/s.
 struct Columns { Source s; u16* dst; long long ldd; int width; const float* maxima; int counts; };
-template <class T, int PL, int EL>
+template <class T> constexpr bool kScaled = !__is_same(T, _Float16);
+template <class T, int PL>
 __global__ __launch_bounds__(256) void pack_transposes_kernel(Columns w, Columns h, int blocks_w, Exponents* __restrict__ ex) {
     __shared__ float red[4];
     const bool second = (int)blockIdx.x >= blocks_w;
     const Columns c = second ? h : w;
     const int id = (int)blockIdx.x - (second ? blocks_w : 0), across = ceil_div(c.width, 64);
     int e = 0;
-    if constexpr (PL == TWO) {
+    if constexpr (kScaled<T>) {
         float m = 0.f;
         for (int i = threadIdx.x; i < c.counts; i += 256) m = fmaxf(m, c.maxima[i]);
         m = wave_largest(m);
@@ -389,11 +431,10 @@ __global__ __launch_bounds__(256) void pack_transposes_kernel(Columns w, Columns
         e = exponent_for(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
         if (threadIdx.x == 0 && id == 0) (second ? ex->h : ex->w) = e;
     }
-    pack_columns_tile<T, PL, EL>(c.s, e, c.dst, c.ldd, c.width, id % across, id / across);
+    pack_columns_tile<T, PL, FP16>(c.s, e, c.dst, c.ldd, c.width, id % across, id / across);
 }
 
-// fp16 planes hold probabilities times 2^14: 11 (22) bits of every probability down to 2^-28 (2^-17)
-template <int EL> __host__ __device__ constexpr int probability_exponent() { return EL == FP16 ? 14 : 0; }
+constexpr int kProbabilityExponent = 14;
 
 // a piece of G and of its transpose: classes [v0, v0 + vp).  G [N][packed vp] holds p - [v = t] (0 where the row is ignored), GT [vp][packed N] the
 // same times the row's upstream gradient relative to the largest; columns behind N and vp up to the packed width are zero.  Bound by the matrix
@@ -402,7 +443,7 @@ template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand H, Operand W, int width, Logits how,
         const Row* __restrict__ stats, Upstream up, int v0, int vp, int V, u16* __restrict__ G, long long ldg,
         u16* __restrict__ GT, long long ldgt) {
-    constexpr int PL = TileT::PL, EL = TileT::EL;
+    constexpr int PL = TileT::PL;
     UNFLOW_DYNAMIC_LDS(char, lds);
     const int mt = ceil_div(H.rows, TileT::BM), nt = ceil_div(vp, TileT::BN);
     int tm, tn;
@@ -412,7 +453,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
     const Operand piece{W.p + (long long)v0 * W.ld, W.ld, vp};
     T.run(H, piece, 0, width, m0, n0, lds);
     how.ew += PL == TWO ? v0 : 0;
-    const float unit = (float)(1 << probability_exponent<EL>());
+    const float unit = (float)(1 << kProbabilityExponent);
     const int wide_n = (int)round_up(vp, PL == TWO ? 32 : 8);
     const bool edge = n0 + TileT::BN > vp;
     float weights[TileT::MI];
@@ -445,15 +486,11 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
         if (G && there)
 #pragma unroll
             for (int j = 0; j < TileT::NI; ++j)
-                if (n0 + TileT::col(j) < wide_n) pack4<PL, EL>(G + (long long)m * ldg, n0 + TileT::col(j), T.acc[i][j]);
+                if (n0 + TileT::col(j) < wide_n) pack4<PL, FP16>(G + (long long)m * ldg, n0 + TileT::col(j), T.acc[i][j]);
     }
     // (a row that is not used, or behind the last, is zeros already: 0 times its weight)
-    if (GT) T.store_transposed(lds, GT, ldgt, vp, ldgt, m0, n0, [&](int i, int j) { return T.acc[i][j] * weights[i]; });
+    if (GT) T.template store_transposed<FP16>(lds, GT, ldgt, vp, ldgt, m0, n0, [&](int i, int j) { return T.acc[i][j] * weights[i]; });
 }
-
-template <class TileT> struct OutputOf { using type = __bf16; };
-template <int BM, int BN, int WM, int WN, int DP> struct OutputOf<Tile<BM, BN, WM, WN, DP, ONE, FP16>> { using type = _Float16; };
-template <int BM, int BN, int WM, int WN, int DP> struct OutputOf<Tile<BM, BN, WM, WN, DP, TWO, FP16>> { using type = float; };
 
 // The two products of a piece, one launch: job 0 is dH += G W, job 1 dW = G^T H.  C = A B^T in `shares` shares of what is summed.  A job without
 // `sums` is one share and goes to the gradient as it is; else the shares' accumulators go to fp32 sums [shares][rows of A][ldc], added to what
@@ -461,15 +498,14 @@ template <int BM, int BN, int WM, int WN, int DP> struct OutputOf<Tile<BM, BN, W
 struct Product { Operand A, B; int width, shares, tiles; float* sums; long long ldc; int first; void* out; int by_h; };
 
 // what turns a job's sums into gradients: the uniform factor, and the row's own (dH; for dW it is in GT, relative to the largest)
-template <int PL, int EL> __device__ __forceinline__ float product_factor(const Exponents* ex, const Upstream& up, int by_h) {
+template <class T> __device__ __forceinline__ float product_factor(const Exponents* ex, const Upstream& up, int by_h) {
     float f = uniform_factor(up) * (by_h && up.reduction == 0 ? up.largest[0] : 1.f);
-    if constexpr (PL == TWO) f = ldexpf(f, -(by_h ? ex->h : ex->w));
-    return ldexpf(f, -probability_exponent<EL>());
+    if constexpr (kScaled<T>) f = ldexpf(f, -(by_h ? ex->h : ex->w));
+    return ldexpf(f, -kProbabilityExponent);
 }
 
-template <class TileT>
+template <class T_, class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product a, Product b, const Exponents* __restrict__ ex, Upstream up) {
-    using T_ = typename OutputOf<TileT>::type;
     UNFLOW_DYNAMIC_LDS(char, lds);
     // Each job is dealt over the XCDs by itself: their units differ in length.  (A workgroup that goes through units of its own, as in the forward
     // pass, gains nothing where they are alike and loses a third where they are not.)
@@ -509,7 +545,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product
         }
         return;
     }
-    const float f = product_factor<TileT::PL, TileT::EL>(ex, up, p.by_h);
+    const float f = product_factor<T_>(ex, up, p.by_h);
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
@@ -525,12 +561,12 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product
 
 // gradients = sums over the shares, in order, times the factors; one launch for the jobs that have sums (blocks of the first, then of the second).
 // Bound by bytes: 4096 x 2048 to bf16 10.5 us = 4.8 TB/s.
-template <class T_, int PL, int EL>
+template <class T_>
 __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, int blocks_a, const Exponents* __restrict__ ex, Upstream up) {
     const bool second = (int)blockIdx.x >= blocks_a;
     const Product p = second ? b : a;
     const int block = (int)blockIdx.x - (second ? blocks_a : 0), blocks = second ? (int)gridDim.x - blocks_a : blocks_a;
-    const float f = product_factor<PL, EL>(ex, up, p.by_h);
+    const float f = product_factor<T_>(ex, up, p.by_h);
     const int rows = p.A.rows, cols = p.B.rows;
     const long long per = p.ldc / 4, total = per * rows;
     for (long long g = block * 256ll + threadIdx.x; g < total; g += blocks * 256ll) {
@@ -570,7 +606,7 @@ struct Plan {
     long long partial, ztarget, losses, forward_bytes;
     int vp, size_g, size_p, limit;
     long long wvp, ldc;
-    long long repacked, exponents, largest, g, gt, ht, wt, sum_h, sum_w, backward_bytes;
+    long long repacked, magnitudes, exponents, largest, g, gt, ht, wt, sum_h, sum_w, backward_bytes;
 };
 
 // classes a workgroup of lce_few_kernel takes
@@ -636,6 +672,7 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
         p.size_p = c.size;
         p.limit = c.limit;
     }
+    if (dtype == kBf16) p.magnitudes = take(2 * kMaxima * 4);
     p.exponents = take(sizeof(Exponents));
     p.largest = take(4);
     p.g = take(2 * p.wvp * N);
@@ -730,7 +767,12 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
     Operand H, W;
     const Logits how = operands<T, PL, EL>(p, in, to, !p.keeps, stream, H, W);
     Exponents* ex = (Exponents*)(ws + p.exponents);
-    const float* maxima = (const float*)(to + p.maxima);
+    float* maxima = (float*)(PL == TWO ? to + p.maxima : ws + p.magnitudes);
+    if constexpr (kScaled<T> && PL == ONE) {
+        const int blocks_h = dw ? pack_blocks(in.N) : 0, blocks_w = dh ? pack_blocks(in.V) : 0;
+        UNFLOW_LAUNCH(lce_magnitudes_kernel, dim3(blocks_h + blocks_w), dim3(256), 0, stream, H, W, (int)(p.wd / 8), blocks_h, in.target, in.ignore,
+            maxima);
+    }
     const Upstream up{gout, (const float*)(ws + p.largest), stats + 4ll * in.N, in.target, in.ignore, reduction, in.scale};
     if (reduction == 0) UNFLOW_LAUNCH(lce_largest_upstream_kernel, dim3(1), dim3(1024), 0, stream, up, in.N, (float*)(ws + p.largest));
     u16 *G = (u16*)(ws + p.g), *GT = (u16*)(ws + p.gt);
@@ -750,7 +792,7 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
                 maxima, pack_blocks(in.N)};
             blocks_h = ceil_div(hc.width, 64) * ceil_div(in.D, 64);
         }
-        if (blocks_w + blocks_h) UNFLOW_LAUNCH((pack_transposes_kernel<T, PL, EL>), dim3(blocks_w + blocks_h), dim3(256), 0, stream, wc, hc,
+        if (blocks_w + blocks_h) UNFLOW_LAUNCH((pack_transposes_kernel<T, PL>), dim3(blocks_w + blocks_h), dim3(256), 0, stream, wc, hc,
             blocks_w, ex);
         with_tile<PL, EL>(p.size_g, [&](auto tile) {
             using TileT = decltype(tile);
@@ -769,18 +811,18 @@ static void backward(const Plan& p, const Inputs& in, int reduction, const float
                 (float*)(ws + p.sum_w), p.ldc, 1, (T*)dw + (long long)v0 * in.D, 1};
             if (b.shares == 1) b.sums = nullptr;
         }
-        with_tile<PL, EL>(p.size_p, [&](auto tile) {
+        with_tile<PL, FP16>(p.size_p, [&](auto tile) {
             using TileT = decltype(tile);
             if (dh) a.tiles = (int)tiles_of(in.N, in.D, TileT::BM);
             if (dw) b.tiles = (int)tiles_of(vp, in.D, TileT::BM);
             const bool swap = dw && (!dh || b.width / b.shares > a.width / a.shares);        // the longer units first
-            LAUNCH_TILES((lce_products_kernel<TileT>), a.tiles * a.shares + b.tiles * b.shares, TileT::STAGES_LDS, swap ? b : a, swap ? a : b,
+            LAUNCH_TILES((lce_products_kernel<T, TileT>), a.tiles * a.shares + b.tiles * b.shares, TileT::STAGES_LDS, swap ? b : a, swap ? a : b,
                 (const Exponents*)ex, up);
         });
         const bool last = v0 + vp >= in.V;
         const int finish_a = dh && last && a.sums ? blocks_for((long long)in.N * (p.ldc / 4)) : 0,
             finish_b = dw && b.sums ? blocks_for((long long)vp * (p.ldc / 4)) : 0;
-        if (finish_a + finish_b) UNFLOW_LAUNCH((lce_finish_kernel<T, PL, EL>), dim3(finish_a + finish_b), dim3(256), 0, stream, a, b, finish_a,
+        if (finish_a + finish_b) UNFLOW_LAUNCH((lce_finish_kernel<T>), dim3(finish_a + finish_b), dim3(256), 0, stream, a, b, finish_a,
             (const Exponents*)ex, up);
     }
 }

@@ -225,8 +225,8 @@ struct Tile {
 
     // The transpose of the tile, value(i, j) being the four numbers that belong to acc[i][j], into packed rows: dst row n holds the numbers of
     // column n at k = m.  A lane's four numbers lie in four dst rows; through LDS (half of m at a time for TWO planes) the rows leave in 16-byte
-    // pieces.  `width`: elements of a dst row; LDS is free when this is called and not when it returns.
-    template <class F>
+    // pieces.  `width`: elements of a dst row; LDS is free when this is called and not when it returns.  AS: what the numbers become.
+    template <int AS = EL, class F>
     __device__ __forceinline__ void store_transposed(char* lds, u16* __restrict__ dst, long long ld, int rows, long long width, int m0, int n0,
         F&& value) {
         static_assert(WM == 2, "the halves of m are the wave rows");
@@ -241,7 +241,7 @@ struct Tile {
                     for (int j = 0; j < NI; ++j) {
                         const f32x4 v = value(i, j);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) pack1<PL, EL>(s + (col(j) + r) * PITCH, row(i) - pass * R, v[r]);
+                        for (int r = 0; r < 4; ++r) pack1<PL, AS>(s + (col(j) + r) * PITCH, row(i) - pass * R, v[r]);
                     }
             }
             __syncthreads();
