@@ -442,6 +442,26 @@ def test_orthogonalize_at_size(dtype, shape):
     _check_orthogonal(ops.orthogonalize(x), x)
 
 
+@pytest.mark.parametrize('shape,rank', [((1, 1), None), ((1, 300), None), ((300, 1), None), ((2, 8), None), ((4, 512), None), ((15, 175), None), ((175, 15), None),
+                                        ((31, 129), None), ((32, 32), None), ((3, 32, 127), None), ((257, 32), None), ((20, 60), 3), ((13, 8400), None), ((8400, 7), 2)])
+def test_few_rows(device, shape, rank):
+    """Up to 32 rows or columns: all sums in 64 bits (n 2^-53, times a^10 = 2^18, and the steps' rounding), one rounding of the result to 2^-24."""
+    x = _matrix(*shape, dtype=torch.float32, device=device, rank=rank)
+    got = ops.orthogonalize(x)
+    g = x.double().mT if shape[-2] > shape[-1] else x.double()
+    m, n = g.shape[-2:]
+    g = g / (g.norm(dim=(-2, -1), keepdim=True) + 1e-7)
+    a, b, c = COEFFICIENTS
+    s, p = g @ g.mT.contiguous(), torch.eye(m, dtype=torch.float64, device=x.device)
+    for _ in range(5):
+        q = a * torch.eye(m, dtype=torch.float64, device=x.device) + b * s + c * (s @ s)
+        p, s = q @ p, q @ s @ q
+    exact = p @ g
+    bound = exact.abs() * 2**-24 + (n + 1000) * 2**-53 * 2**18 * float(g.abs().max()) * m + 2**-149
+    got = got.double().mT if shape[-2] > shape[-1] else got.double()
+    assert bool(((got - exact).abs() <= bound).all()), float(((got - exact).abs() / bound).max())
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_orthogonalize_low_rank(device, dtype):
     """Rank 3 of 60: the directions that only rounding fills are multiplied by 485 and must be the input's, not the kernel's."""

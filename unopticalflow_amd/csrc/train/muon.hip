@@ -7,8 +7,9 @@
 // S and Q are symmetric: their tiles above the diagonal are not computed but written as the mirror of those below, so a step costs
 // m^2 n + m^3 + 2 m^2 n operations instead of 4 m^2 n + 2 m^3.  The products bound large matrices; a list of small ones is bound by launches,
 // so every phase is one launch over the tiles of all matrices (a wave finds its matrix in a table of running tile counts), 3 launches a step.
+// Matrices of up to 32 rows or columns, where nothing larger is in the list, have kernels of their own (in the middle of this file).
 //
-// Numbers (mfma16.h): every type is iterated on as two fp16 planes (22 bits, products and sums as in fp32).  One plane would take a third of
+// Numbers of the tiles (mfma16.h): every type is iterated on as two fp16 planes (22 bits, products and sums as in fp32).  One plane would take a third of
 // the products, and its 2^-12 looks small beside the 2^-9 of a bf16 result, but the iteration multiplies small singular values by a^5 = 485 and
 // what rounding spreads over their directions with them: a bf16 matrix of low rank comes out several percent off that way.  The Frobenius norm is
 // summed in 64 bits.  |X|, |S|, |Q| are bounded by the polynomial over [0, 1], which gives the powers of two that
@@ -359,6 +360,225 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem*
     if constexpr (!LAST) T_.store_transposed(lds, next, ldm, p.n, ldm, tm * TileT::BM, tn * TileT::BN, [&](int i, int j) { return T_.acc[i][j]; });
 }
 
+// ---- matrices of up to 32 rows (or columns).  All X of the iteration are polynomials in S_0 = X_0 X_0^T times X_0, so it can run on m x m matrices:
+//   P <- Q P,  S <- Q S Q,  Q = a I + b S + c S S;   X = P X_0 at the end
+// one read of the matrix for S_0, whose trace is the squared norm, and one for the result: 3 launches instead of 22.  Squaring the singular values
+// needs twice the digits (what rounding adds to S_0 is multiplied by a^10), so all sums are 64 bits, and that is what bounds m: the 17 products
+// of one workgroup take 17 m^3 fused operations at 64 a cycle (18 us for m = 32).  8 x 500: 30 us against 50 by the tiles, 8 of 32 x 1152 44 against
+// 98, 32 x 100000 122 against 382; and nearer to the formula than the tiles' planes, whose two roundings a step show where sums are short (4 x 512:
+// 3.5e-6 by the tiles, 1.5e-6 in fp32).  A list that has larger matrices goes by the tiles as a whole, whose launches are there anyhow (the flow
+// network's weights: 252 us, 299 where those of few rows have their own kernels).
+constexpr int kNarrow = 32, kColumns = 128, kGramParts = 64;         // a workgroup takes 128 columns at a time; S_0 is summed in at most 64 parts
+constexpr int kNarrowNumbers = kNarrow * kColumns / 256;             // of a thread
+
+// the columns j0 .. of a matrix as they lie in memory: number q of a thread is (i, j), j < width where there is one
+struct Columns {
+    int m, n, j0, width;
+    bool tall;
+    __device__ __forceinline__ Columns(const Problem& p, int chunk)
+        : m(p.m), n(p.n), j0(chunk * kColumns), width(p.n - chunk * kColumns < kColumns ? p.n - chunk * kColumns : kColumns), tall(p.rows > p.cols) {}
+    __device__ __forceinline__ void place(int q, int& i, int& j) const {
+        const int e = q * 256 + (int)threadIdx.x;
+        const bool in_rows = tall && e < kColumns * m;               // (behind the last number both give rows m ..)
+        i = in_rows ? e % m : e / kColumns;
+        j = in_rows ? e / m : e % kColumns;
+    }
+    __device__ __forceinline__ bool there(int i, int j) const { return i < m && j < width; }
+    __device__ __forceinline__ long long at(int i, int j) const { return tall ? (long long)(j0 + j) * m + i : (long long)i * n + j0 + j; }
+};
+typedef float NarrowTile[kColumns + 4] __attribute__((aligned(16)));
+
+// the update's direction (or the matrix) into x [32][128]; zeros where nothing is.  FIRST: the momentum is brought up to date
+template <class T, bool STEP, bool FIRST>
+__device__ __forceinline__ void load_columns(const Problem& p, const Columns& c, float mu, int nesterov, NarrowTile* x) {
+    float v[kNarrowNumbers], m[kNarrowNumbers];
+#pragma unroll
+    for (int q = 0; q < kNarrowNumbers; ++q) {
+        int i, j;
+        c.place(q, i, j);
+        v[q] = c.there(i, j) ? load1((const T*)p.x + c.at(i, j)) : 0.f;
+        m[q] = STEP && c.there(i, j) ? p.momentum[c.at(i, j)] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < kNarrowNumbers; ++q) {
+        int i, j;
+        c.place(q, i, j);
+        if constexpr (STEP) {
+            if constexpr (FIRST) {
+                m[q] = m[q] + (1.f - mu) * (v[q] - m[q]);
+                if (c.there(i, j)) p.momentum[c.at(i, j)] = m[q];
+            }
+            v[q] = direction(v[q], m[q], mu, nesterov);
+        }
+        x[i][j] = v[q];
+    }
+}
+
+// a part of S_0 |G|^2: a thread sums 2 x 2 numbers in 64 bits (products of 32-bit numbers are exact)
+template <class T, bool STEP>
+__global__ __launch_bounds__(256) void narrow_gram_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, float mu,
+        int nesterov, char* __restrict__ ws) {
+    __shared__ NarrowTile x[kNarrow];
+    int part;
+    const Problem p = table[problem_of(ends, count, (int)blockIdx.x, part)];
+    const int chunks = ceil_div(p.n, kColumns), per = ceil_div(chunks, p.parts), last = (part + 1) * per < chunks ? (part + 1) * per : chunks;
+    const int i = 2 * ((int)threadIdx.x >> 4), k = 2 * ((int)threadIdx.x & 15);
+    double s[2][2] = {};
+    for (int c = part * per; c < last; ++c) {
+        load_columns<T, STEP, true>(p, Columns(p, c), mu, nesterov, x);
+        __syncthreads();
+        if (i < p.m && k < p.m)
+#pragma unroll 4
+            for (int j = 0; j < kColumns; j += 4) {
+                const f32x4 a[2] = {*reinterpret_cast<const f32x4*>(&x[i][j]), *reinterpret_cast<const f32x4*>(&x[i + 1][j])};
+                const f32x4 b[2] = {*reinterpret_cast<const f32x4*>(&x[k][j]), *reinterpret_cast<const f32x4*>(&x[k + 1][j])};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) s[u][w] = fma((double)a[u][q], (double)b[w][q], s[u][w]);
+            }
+        __syncthreads();
+    }
+    double* to = (double*)(ws + p.S) + (long long)part * kNarrow * kNarrow;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) to[(i + u) * kNarrow + k + w] = s[u][w];
+}
+
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef double NarrowMatrix[kNarrow + 2] __attribute__((aligned(16)));
+// a thread's 2 x 2 numbers of A B for symmetric matrices (B's columns are its rows), zeros behind m
+__device__ __forceinline__ void narrow_product(const NarrowMatrix* A, const NarrowMatrix* B, int m, int i, int k, double (&c)[2][2]) {
+    double s[2][2] = {};
+    for (int q = 0; q < m; q += 2) {
+        const f64x2 a[2] = {*reinterpret_cast<const f64x2*>(&A[i][q]), *reinterpret_cast<const f64x2*>(&A[i + 1][q])};
+        const f64x2 b[2] = {*reinterpret_cast<const f64x2*>(&B[k][q]), *reinterpret_cast<const f64x2*>(&B[k + 1][q])};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) s[u][w] = fma(a[u].y, b[w].y, fma(a[u].x, b[w].x, s[u][w]));
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) c[u][w] = s[u][w];
+}
+
+// S_0 from its parts, in order, and P / (norm + eps), 1024 numbers at p.Q.  A workgroup per matrix
+__global__ __launch_bounds__(256) void narrow_iterate_kernel(const Problem* __restrict__ table, int steps, double a, double b, double c, float eps,
+        char* __restrict__ ws) {
+    __shared__ NarrowMatrix S[kNarrow], Q[kNarrow], P[kNarrow];
+    const Problem p = table[blockIdx.x];
+    const int i = 2 * ((int)threadIdx.x >> 4), k = 2 * ((int)threadIdx.x & 15), m = p.m;
+    const bool in = i < m && k < m;
+    double v[2][2] = {}, mine[2][2];
+    auto put = [&](NarrowMatrix* to, double scale) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) to[i + u][k + w] = v[u][w] * scale;
+    };
+    const double* parts = (const double*)(ws + p.S) + i * kNarrow + k;
+#pragma unroll 4
+    for (int q = 0; q < p.parts; ++q) {
+        const f64x2 x = *reinterpret_cast<const f64x2*>(parts + (long long)q * kNarrow * kNarrow);
+        const f64x2 y = *reinterpret_cast<const f64x2*>(parts + (long long)q * kNarrow * kNarrow + kNarrow);
+        v[0][0] += x.x; v[0][1] += x.y; v[1][0] += y.x; v[1][1] += y.y;
+    }
+    put(S, 1.);
+    __syncthreads();
+    double trace = 0.;
+    for (int q = 0; q < m; ++q) trace += S[q][q];
+    const double factor = 1. / (sqrt(trace) + (double)eps);
+    __syncthreads();
+    put(S, factor * factor);
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        if (in) {
+            narrow_product(S, S, m, i, k, v);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) v[u][w] = c * v[u][w] + b * S[i + u][k + w] + (i + u == k + w && i + u < m ? a : 0.);
+        }
+        put(Q, 1.);
+        __syncthreads();
+        if (step == 0) put(P, 1.);
+        else {
+            if (in) narrow_product(Q, P, m, i, k, v);
+            __syncthreads();
+            put(P, 1.);
+        }
+        if (step + 1 < steps) {
+            if (in) narrow_product(Q, S, m, i, k, v);
+            __syncthreads();
+            put(S, 1.);
+            __syncthreads();
+            if (in) narrow_product(Q, S, m, i, k, mine);
+            __syncthreads();
+            if (in)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) S[i + u][k + w] = mine[u][w];
+        }
+        __syncthreads();
+    }
+    double* to = (double*)(ws + p.Q);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) to[(i + u) * kNarrow + k + w] = P[i + u][k + w] * factor;
+}
+
+// X = P X_0 of 128 columns: a thread has one column and half of the rows.  The output, or the parameter's update
+template <class T, bool STEP>
+__global__ __launch_bounds__(256) void narrow_apply_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count, float mu,
+        int nesterov, Update up, const char* __restrict__ ws) {
+    __shared__ NarrowTile x[kNarrow];
+    __shared__ NarrowMatrix P[kNarrow];
+    int chunk;
+    const Problem p = table[problem_of(ends, count, (int)blockIdx.x, chunk)];
+    const double* from = (const double*)(ws + p.Q);
+    for (int e = (int)threadIdx.x; e < kNarrow * kNarrow; e += 256) P[e / kNarrow][e % kNarrow] = from[e];
+    const Columns c(p, chunk);
+    load_columns<T, STEP, false>(p, c, mu, nesterov, x);
+    __syncthreads();
+    const int j = (int)threadIdx.x & (kColumns - 1), r0 = (int)threadIdx.x / kColumns * 16;
+    f64x2 v[8] = {};
+    if (r0 < p.m)
+        for (int k = 0; k < p.m; ++k) {
+            const double xk = (double)x[k][j];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const f64x2 pk = *reinterpret_cast<const f64x2*>(&P[k][r0 + 2 * r]);
+                v[r] = f64x2{fma(pk.x, xk, v[r].x), fma(pk.y, xk, v[r].y)};
+            }
+        }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r0 + r][j] = (float)v[r / 2][r % 2];
+    __syncthreads();
+    const float lr = up.lr * p.boost;
+    T* out = (T*)p.out;
+    float old[kNarrowNumbers];
+#pragma unroll
+    for (int q = 0; q < kNarrowNumbers; ++q) {
+        int i, k;
+        c.place(q, i, k);
+        old[q] = STEP && c.there(i, k) ? load1(out + c.at(i, k)) : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < kNarrowNumbers; ++q) {
+        int i, k;
+        c.place(q, i, k);
+        if (c.there(i, k)) out[c.at(i, k)] = (T)(STEP ? old[q] * up.keep - x[i][k] * lr : x[i][k]);
+    }
+}
+
 // ---- the host side
 template <class F> static void with_tile(int size, F&& f) {
     if (size == 0) f(Tile<256, 256, 2, 4, 2, TWO, FP16>{});
@@ -393,12 +613,14 @@ static bool exponents_of(int steps, float a, float b, float c, Exponents& ex) {
 constexpr long long kGroupBytes = 4ll << 30;                         // matrices are taken together as long as their planes fit in this
 
 struct Group {
-    int first, count;
+    int first, count;                                                // of the list
+    bool narrow;                                                     // all of few rows
+    int grams, columns;                                              // the work items of the kernels for these
     int size_s, size_q, size_x;                                      // indices into kSizes
     // numbers a workgroup of the norm takes: few of a small list, so that it fills the chip
     int chunk;
     int total[kPhases];
-    long long table, ends, parts, bytes;
+    long long table, ends, parts, table_bytes, bytes;
 };
 
 static long long plane_bytes(long long m, long long n) {
@@ -426,18 +648,49 @@ static void sort_of(const unflow_matrix* a, int first, int count, Sorted& s) {
     }
 }
 
-// lays out a group: problems and running counts on the host, offsets into the workspace
-static Group lay_out(const unflow_matrix* a, int first, int count, Problem* problems, int* ends) {
+static Problem problem_for(const unflow_matrix& q, int m, int n) {
+    Problem p{};
+    p.x = q.x; p.out = q.out; p.momentum = q.momentum;
+    p.rows = q.rows; p.cols = q.cols;
+    p.m = m; p.n = n;
+    p.boost = q.rows > q.cols ? sqrtf((float)q.rows / (float)q.cols) : 1.f;
+    return p;
+}
+
+// lays out a group: problems and running counts on the host (`table`: what g.table_bytes of the workspace will hold), offsets into the workspace
+static Group lay_out(const unflow_matrix* a, int first, int count, char* table) {
     static thread_local Sorted order;
     static thread_local Job jobs[kMost];
     sort_of(a, first, count, order);
     Group g{};
     g.first = first;
     g.count = count;
+    g.narrow = *std::max_element(order.m, order.m + count) <= kNarrow;
     long long at = 0, chunks = 0;
     auto take = [&](long long bytes) { const long long p = at; at += round_up(bytes, 256); return p; };
-    g.table = take(((long long)sizeof(Problem) + 4 * kTables) * count);
-    g.ends = g.table + (long long)sizeof(Problem) * count;
+    g.ends = (long long)sizeof(Problem) * count;                     // (of the table)
+    g.table_bytes = g.ends + 4ll * (g.narrow ? 2 : kTables) * count;
+    g.table = take(g.table_bytes);
+    Problem* problems = (Problem*)table;
+    int* ends = (int*)(table ? table + g.ends : nullptr);
+    if (g.narrow) {
+        for (int i = 0; i < count; ++i) {
+            Problem p = problem_for(a[order.at[i]], order.m[i], order.n[i]);
+            const int columns = ceil_div(p.n, kColumns);
+            p.parts = columns < kGramParts ? columns : kGramParts;
+            p.S = take(8ll * kNarrow * kNarrow * p.parts);
+            p.Q = take(8ll * kNarrow * kNarrow);
+            g.grams += p.parts;
+            g.columns += columns;
+            if (table) {
+                problems[i] = p;
+                ends[i] = g.grams;
+                ends[count + i] = g.columns;
+            }
+        }
+        g.bytes = at;
+        return g;
+    }
     // matrices of one shape are one job of the model
     auto plan = [&](auto job_of) {
         int k = 0;
@@ -461,12 +714,7 @@ static Group lay_out(const unflow_matrix* a, int first, int count, Problem* prob
     g.parts = take(8 * chunks);
     int part0 = 0, run[kPhases] = {};
     for (int i = 0; i < count; ++i) {
-        const unflow_matrix& q = a[order.at[i]];
-        Problem p{};
-        p.x = q.x; p.out = q.out; p.momentum = q.momentum;
-        p.rows = q.rows; p.cols = q.cols;
-        p.m = order.m[i]; p.n = order.n[i];
-        p.boost = q.rows > q.cols ? sqrtf((float)q.rows / (float)q.cols) : 1.f;
+        Problem p = problem_for(a[order.at[i]], order.m[i], order.n[i]);
         p.X = take(2 * packed_width(TWO, p.n) * p.m);
         p.XT0 = take(2 * packed_width(TWO, p.m) * p.n);
         p.XT1 = take(2 * packed_width(TWO, p.m) * p.n);
@@ -484,12 +732,12 @@ static Group lay_out(const unflow_matrix* a, int first, int count, Problem* prob
         run[kJoin] += p.shares > 1 ? low * (kSizes[g.size_s] / 64) * (kSizes[g.size_s] / 64) : 0;
         run[kPoly] += (int)lower_tiles_of(p.m, kSizes[g.size_q]);
         run[kApply] += (int)tiles_of(p.m, p.n, kSizes[g.size_x]);
-        if (problems) {
+        if (table) {
             problems[i] = p;
             for (int k = 0; k < kPhases; ++k) ends[k * count + i] = run[k];
         }
     }
-    if (problems) {
+    if (table) {
         // matrices whose work items of a phase are equally long are dealt out together (they are neighbours for S, which sums over n; the other two
         // sum over m, which need not be in order: as far as neighbours are alike)
         const int phases[3] = {kSquare, kPoly, kApply}, tables[3] = {kSquareClass, kPolyClass, kApplyClass};
@@ -546,9 +794,15 @@ template <class T, bool STEP>
 static void iterate(const Group& g, int steps, float a, float b, float c, float eps, float mu, int nesterov, Update up, Exponents ex, char* ws,
         hipStream_t stream) {
     const Problem* table = (const Problem*)(ws + g.table);
-    const int* ends = (const int*)(ws + g.ends);
-    double* parts = (double*)(ws + g.parts);
+    const int* ends = (const int*)(ws + g.table + g.ends);
     const int n = g.count;
+    if (g.narrow) {
+        UNFLOW_LAUNCH((narrow_gram_kernel<T, STEP>), dim3(g.grams), dim3(256), 0, stream, table, ends, n, mu, nesterov, ws);
+        UNFLOW_LAUNCH(narrow_iterate_kernel, dim3(n), dim3(256), 0, stream, table, steps, (double)a, (double)b, (double)c, eps, ws);
+        UNFLOW_LAUNCH((narrow_apply_kernel<T, STEP>), dim3(g.columns), dim3(256), 0, stream, table, ends + n, n, mu, nesterov, up, (const char*)ws);
+        return;
+    }
+    double* parts = (double*)(ws + g.parts);
     UNFLOW_LAUNCH((norm_kernel<T, STEP>), dim3(g.total[kNorm]), dim3(256), 0, stream, table, ends + kNorm * n, n, g.chunk, mu, nesterov, parts);
     UNFLOW_LAUNCH((start_kernel<T, STEP>), dim3(g.total[kPack]), dim3(256), 0, stream, table, ends + kPack * n, n, (const double*)parts, mu,
         nesterov, eps, ex, ws);
@@ -577,7 +831,7 @@ static int workspace_of(const unflow_matrix* a, int count, int dtype, long long*
     long long most = 0;
     for (int i = 0; i < count;) {
         const int e = group_end(a, count, i);
-        const long long b = lay_out(a, i, e - i, nullptr, nullptr).bytes;
+        const long long b = lay_out(a, i, e - i, nullptr).bytes;
         most = most > b ? most : b;
         i = e;
     }
@@ -598,8 +852,8 @@ static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca
     for (int i = 0; i < count;) {
         const int e = group_end(a, count, i), n = e - i;
         static thread_local struct alignas(8) { char bytes[kMost * (sizeof(Problem) + 4 * kTables)]; } table;
-        const Group g = lay_out(a, i, n, (Problem*)table.bytes, (int*)(table.bytes + sizeof(Problem) * n));
-        write_table(table.bytes, (sizeof(Problem) + 4ll * kTables) * n, ws + g.table, stream);
+        const Group g = lay_out(a, i, n, table.bytes);
+        write_table(table.bytes, g.table_bytes, ws + g.table, stream);
         if (dtype == kFp32) iterate<float, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else if (dtype == kBf16) iterate<__bf16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else iterate<_Float16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);

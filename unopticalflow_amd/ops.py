@@ -1821,6 +1821,28 @@ def _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, n
     return loss, (hidden, weight, kept), (ldh, ldw, dtype, sizes[2])
 
 
+def _linear_ce_backward(ctx, g):
+    hidden, weight, target, kept = ctx.saved_tensors
+    (ignore_index, scale, reduction), (ldh, ldw, dtype, need) = ctx.options, ctx.how
+    need_h, need_w = ctx.needs_input_grad[:2]
+    (N, D), V, dev = hidden.shape, weight.shape[0], hidden.device
+    dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if need_h else None
+    dw = torch.empty((V, D), dtype=weight.dtype, device=dev) if need_w else None
+    if N == 0:
+        return dh, dw.zero_() if need_w else None, None, None, None, None
+    with _on(dev):
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        g = g.contiguous()
+        _call('unflow_linear_ce_bwd', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), g.data_ptr(), N, V, D,
+              dtype, scale, ignore_index, reduction, dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None,
+              kept.data_ptr(), ws.data_ptr(), need, _stream_of(dev),
+              nbytes=2 * (N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+    return dh, dw, None, None, None, None
+
+
+_linear_ce_backward_once = torch.autograd.function.once_differentiable(_linear_ce_backward)
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, scale, reduction):
@@ -1830,24 +1852,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        hidden, weight, target, kept = ctx.saved_tensors
-        (ignore_index, scale, reduction), (ldh, ldw, dtype, need) = ctx.options, ctx.how
-        need_h, need_w = ctx.needs_input_grad[:2]
-        (N, D), V, dev = hidden.shape, weight.shape[0], hidden.device
-        dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if need_h else None
-        dw = torch.empty((V, D), dtype=weight.dtype, device=dev) if need_w else None
-        if N == 0:
-            return dh, dw.zero_() if need_w else None, None, None, None, None
-        with _on(dev):
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            g = g.contiguous()
-            _call('unflow_linear_ce_bwd', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), g.data_ptr(), N, V, D,
-                  dtype, scale, ignore_index, reduction, dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None,
-                  kept.data_ptr(), ws.data_ptr(), need, _stream_of(dev),
-                  nbytes=2 * (N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
-        return dh, dw, None, None, None, None
+        # (the gradients have none of their own: with create_graph they say so when asked)
+        return (_linear_ce_backward_once if torch.is_grad_enabled() else _linear_ce_backward)(ctx, g)
 
 
 def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, reduction='mean'):
