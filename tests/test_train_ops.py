@@ -462,6 +462,40 @@ def test_few_rows(device, shape, rank):
     assert bool(((got - exact).abs() <= bound).all()), float(((got - exact).abs() / bound).max())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_captured_orthogonalize(dtype):
+    """A graph of the tiles, one of the kernels for few rows and one of a Muon step, replayed in turn with eager calls between them."""
+    wide, few = ([_matrix(*s, dtype=dtype, device='cuda', seed=i) for i, s in enumerate(shapes)] for shapes in (((40, 300), (130, 70), (20, 9)), ((31, 700), (5, 5))))
+    weights, grads = ([_matrix(*s, dtype=dtype, device='cuda', seed=9 + i) for s in ((60, 90), (33, 8))] for i in range(2))
+    momenta = [torch.zeros_like(w, dtype=torch.float32) for w in weights]
+
+    def step():
+        optim.muon_step_(weights, grads, momenta, lr=0.1)
+        return weights + momenta
+    graphs = []
+    for call in (lambda: ops.orthogonalize(wide), lambda: ops.orthogonalize(few), step):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, call, call()))
+    for k in range(3):
+        for x in wide + few + grads:
+            x.mul_(0.5).add_(1e-4)
+        for graph, call, out in graphs:
+            before = [t.clone() for t in weights + momenta]
+            graph.replay()
+            kept = [t.clone() for t in out]
+            torch.cuda.synchronize()
+            for t, old in zip(weights + momenta, before):
+                t.copy_(old)
+            assert all(torch.equal(a, b) for a, b in zip(kept, call())), k
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_orthogonalize_low_rank(device, dtype):
     """Rank 3 of 60: the directions that only rounding fills are multiplied by 485 and must be the input's, not the kernel's."""
