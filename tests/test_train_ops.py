@@ -7,7 +7,7 @@ Tolerances.  u(t) = finfo(t).eps / 2 is a rounding to type t.
            dz <= scale (D 2^-24 + 2^-20) max sum_d |h||w|
   loss     two exponents / logarithms of arguments up to Z = max |z| and sums of up to 128 terms in a row: 2 dz + (2 Z + 128) 2^-23
   dh, dw   an element is a sum over K of G times a number.  G = p - [v = t] is off by dp = p (2 dz + (2 Z + 128) 2^-23) + 2^-23, then rounded to
-           u(type) of itself (2^-21 for two planes) or to 2^-39; the sum adds K 2^-24, the result is rounded to its type.
+           u(fp16) of itself (2^-21 for two planes) or to 2^-39; the sum adds K 2^-24, the result is rounded to its type.
   orthogonalize   three matrices a step are rounded to 22 bits where fp32 rounds to 24: four times the error of the same iteration in fp32, plus
            the 16 roundings 2^-22 themselves, plus the output's own rounding; in the Frobenius norm."""
 import contextlib
@@ -81,7 +81,7 @@ def _check_lce(h, w, t, dtype, reduction='mean', scale=1.0, ignore=-100, upstrea
     onehot = torch.zeros_like(p).scatter_(1, at[:, None], 1.0)
     weight = (up if reduction == 'none' else up / count if reduction == 'mean' else up).expand(n) * used * scale
     g = (p - onehot) * weight[:, None]
-    rounding = 2**-21 if dtype == torch.float32 else _u(dtype)
+    rounding = 2**-21 if dtype == torch.float32 else _u(torch.float16)
     off = ((p * loose + 2**-23) + (p - onehot).abs() * rounding + 2**-39) * weight.abs()[:, None]
     if reduction == 'none':                              # (rows are packed relative to the largest upstream gradient)
         off = off + 2**-38 * float(weight.abs().max())
