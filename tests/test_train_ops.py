@@ -109,6 +109,22 @@ def test_loss_and_gradients(device, dtype, rows, vocab, dim, reduction, scale):
     _check_lce(h, w, t, dtype, reduction, scale)
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('rows,dim', [(1, 3), (1, 4), (2, 7), (3, 8), (16, 9), (5, 31), (17, 65), (1, 250), (32, 257), (33, 515), (64, 130), (65, 37), (7, 1023)])
+def test_rows_that_start_and_end_anywhere(device, dtype, rows, dim):
+    """Rows cut out of wider ones, off 16 bytes and with NaN on both sides of them."""
+    h, w, t = _inputs(rows, 100, dim, dtype, device, ignored=0.2 if rows > 4 else 0.0)
+    for before, behind in ((1, 0), (0, 1), (3, 5)):
+        cut = []
+        for x in (h, w):
+            wide = torch.full((len(x), before + dim + behind), float('nan'), dtype=dtype, device=device)
+            wide[:, before:before + dim] = x
+            cut.append(wide[:, before:before + dim])
+        _check_lce(*cut, t, dtype, 'none')
+        with torch.no_grad():
+            assert torch.equal(ops.linear_cross_entropy(*cut, t, reduction='none').isnan(), torch.zeros(rows, dtype=torch.bool, device=device))
+
+
 @pytest.mark.parametrize('rows,vocab,dim,scale', [(60, 90, 16, 14.0), (33, 200, 100, 1.0), (3, 40, 8, 2.0), (20, 50, 33, -3.0)])
 @pytest.mark.parametrize('spread', [1.0, 2.0**-60, 2.0**60])
 def test_gradients_of_bf16_inputs_are_rounded_to_bf16_once(device, rows, vocab, dim, scale, spread):

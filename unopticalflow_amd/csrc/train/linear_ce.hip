@@ -176,15 +176,34 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand 
     }
 }
 
-// ---- forward of few rows (at most 16 NF): reading W is all there is to it.  16-bit inputs of more than 16 rows are better served by the tiles
-// above, where the four waves share the rows of H (61 rows against 50257 classes of 1024 fp16: 20 us against 36); fp32 inputs stay here up to 64
-// rows, for packing W would read and write all of it once more (50257 classes of 1024 dimensions, whole calls: 16 rows 58 us against 200 through
-// the tiles, 33 rows 112 against 204, 64 rows 126 against 212; 5000 of 256: 15 against 18).  One row, 32000 classes of 2048 bf16: 23 us =
-// 5.7 TB/s.  A workgroup takes 16 CF classes, its four waves a quarter of D each, AHEAD
-// steps of loads in flight; the rows of W go from memory to the matrix instruction as they lie there.  16-bit numbers: 32 k a step, lane l holds
-// k = 8 (l >> 4) .. of row l & 15.  fp32: 16 k a step as four v_mfma_f32_16x16x4_f32, the e-th taking k = 4 (l >> 4) + e -- fp32 arithmetic
+// ---- forward of few rows (at most 16 NF): reading W is all there is to it (one row, 32000 classes of 2048 bf16: 23 us = 5.7 TB/s).  Where the tiles
+// above could take W as it is, 16 rows go here: beyond, the four waves of a tile share the rows of H (61 rows against 50257 classes of 1024 fp16: 20
+// us there, 36 here).  Where W would have to be packed first, written and read once more, 64 rows of fp32 (50257 classes of 1023, whole calls: 1 row
+// 52 us, 64 rows 125, 65 rows by the tiles 214) and 32 of 16-bit numbers, which loads off 4 bytes slow down (the same in fp16: 1 row 55 us, 32 rows
+// 94, by the tiles 89; 59332 of 755: 40, 72, 78; 14068 of 1235: 20, 32, 42).  A workgroup takes 16 CF classes, its four waves a quarter of D each,
+// AHEAD steps of loads in flight; the rows of W go from memory to the matrix instruction as they lie there.  16-bit numbers: 32 k a step, lane l
+// holds k = 8 (l >> 4) .. of row l & 15.  fp32: 16 k a step as four v_mfma_f32_16x16x4_f32, the e-th taking k = 4 (l >> 4) + e -- fp32 arithmetic
 // throughout, and no packing.
-template <class T> struct Few { static constexpr int EACH = 16 / sizeof(T), STEP = 4 * EACH; };
+// Rows need no alignment: a lane's 16 bytes are loaded from where they lie, and the last ones of a row as its last 16 bytes, of which both operands
+// drop what the lane before has taken already (the order of k does not matter as long as both agree).
+template <class T> struct Few {
+    static constexpr int EACH = 16 / sizeof(T), STEP = 4 * EACH;
+    struct Piece { unsigned v[4]; } __attribute__((packed, aligned(sizeof(T))));
+    __device__ __forceinline__ static uint4 load(const T* p) {
+        const Piece q = *reinterpret_cast<const Piece*>(p);
+        return uint4{q.v[0], q.v[1], q.v[2], q.v[3]};
+    }
+    // without the first `skip` numbers
+    __device__ __forceinline__ static uint4 behind(uint4 q, int skip) {
+        unsigned v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = i < skip ? 0u : v[i];
+            else v[i] = 2 * i + 1 < skip ? 0u : 2 * i < skip ? v[i] & 0xffff0000u : v[i];
+        }
+        return uint4{v[0], v[1], v[2], v[3]};
+    }
+};
 template <class T> __device__ __forceinline__ f32x4 few_product(uint4 a, uint4 b, f32x4 c) {
     if constexpr (sizeof(T) == 4) {
         const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
@@ -195,16 +214,15 @@ template <class T> __device__ __forceinline__ f32x4 few_product(uint4 a, uint4 b
 }
 template <class T, int NF, int CF, int AHEAD>
 __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, long long ldh, const T* __restrict__ W, long long ldw, int N, int V,
-        int D, float scale, const long long* __restrict__ target,
-        float2* __restrict__ partial, float* __restrict__ ztarget) {
+        int D, float scale, const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
     constexpr int ROWS = 16 * NF, PER = 256 / ROWS, CLASSES = 16 * CF / PER, PITCH = 16 * CF + 2;
     __shared__ float sums[4][ROWS][PITCH];
     const int lane = (int)threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int v0 = (int)blockIdx.x * 16 * CF, k_lane = (lane >> 4) * Few<T>::EACH, r_lane = lane & 15;
     const T* wrow[CF];
     const T* hrow[NF];
-#pragma unroll
     // (classes behind the last repeat it, unused)
+#pragma unroll
     for (int c = 0; c < CF; ++c) wrow[c] = W + (long long)(v0 + 16 * c + r_lane < V ? v0 + 16 * c + r_lane : V - 1) * ldw;
 #pragma unroll
     for (int i = 0; i < NF; ++i) hrow[i] = H + (long long)(16 * i + r_lane < N ? 16 * i + r_lane : N - 1) * ldh;
@@ -216,16 +234,25 @@ __global__ __launch_bounds__(256) void lce_few_kernel(const T* __restrict__ H, l
     const int steps = ceil_div(D, Few<T>::STEP);
     for (int first = 0; first < steps; first += 4 * AHEAD) {
         uint4 a[AHEAD][CF], b[AHEAD][NF];
+        int skip[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             // (a wave takes two steps in a row: whole lines of W)
-            const int k = (first + (u / 2) * 8 + w * 2 + u % 2) * Few<T>::STEP + k_lane;
-            const bool in = k < D;                                                         // (D is a multiple of what a lane loads)
+            const int k = (first + (u / 2) * 8 + w * 2 + u % 2) * Few<T>::STEP + k_lane, from = k < D - Few<T>::EACH ? k : D - Few<T>::EACH;
+            skip[u] = k - from;
 #pragma unroll
-            for (int c = 0; c < CF; ++c) a[u][c] = in ? *reinterpret_cast<const uint4*>(wrow[c] + k) : uint4{0, 0, 0, 0};
+            for (int c = 0; c < CF; ++c) a[u][c] = Few<T>::load(wrow[c] + from);
 #pragma unroll
-            for (int i = 0; i < NF; ++i) b[u][i] = in ? *reinterpret_cast<const uint4*>(hrow[i] + k) : uint4{0, 0, 0, 0};
+            for (int i = 0; i < NF; ++i) b[u][i] = Few<T>::load(hrow[i] + from);
         }
+        if ((first + 4 * AHEAD) * Few<T>::STEP > D)                      // (a row's end is in reach)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+                for (int c = 0; c < CF; ++c) a[u][c] = Few<T>::behind(a[u][c], skip[u]);
+#pragma unroll
+                for (int i = 0; i < NF; ++i) b[u][i] = Few<T>::behind(b[u][i], skip[u]);
+            }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
@@ -625,9 +652,9 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
         bool need_w) {
     Plan p{};
     p.planes = dtype == kFp32 ? TWO : ONE;
-    p.few = N <= (dtype == kFp32 ? 64 : 16) && aligned(h, ldh, D, dtype) && aligned(w, ldw, D, dtype);
     p.pack_h = dtype == kFp32 || !aligned(h, ldh, D, dtype);
     p.pack_w = dtype == kFp32 || !aligned(w, ldw, D, dtype);
+    p.few = N <= (dtype == kFp32 ? 64 : p.pack_w ? 32 : 16) && D >= (dtype == kFp32 ? 4 : 8);
     p.keeps = (p.pack_h || p.pack_w) && !p.few;
     p.wd = packed_width(p.planes, D);
     p.wn = packed_width(p.planes, N);
@@ -729,11 +756,9 @@ static void forward(const Plan& p, const Inputs& in, int reduction, float* loss,
                 in.scale * kLog2E, in.target, partial, zt);
         };
         if (in.N <= 16) launch(lce_few_kernel<T, 1, 4, 4>);
-        else if constexpr (PL == TWO) {
-            // (beyond 16 rows a wave holds fewer classes and steps, so that more waves fit a CU)
-            if (in.N <= 32) launch(lce_few_kernel<T, 2, 2, 4>);
-            else launch(lce_few_kernel<T, 4, 2, 2>);
-        }
+        // (beyond 16 rows a wave holds fewer classes and steps, so that more waves fit a CU)
+        else if (in.N <= 32) launch(lce_few_kernel<T, 2, 2, 4>);
+        else if constexpr (PL == TWO) launch(lce_few_kernel<T, 4, 2, 2>);
     } else {
         Operand H, W;
         const Logits how = operands<T, PL, EL>(p, in, kept, true, stream, H, W);
