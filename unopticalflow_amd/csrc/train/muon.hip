@@ -11,8 +11,8 @@
 //
 // Numbers of the tiles (mfma16.h): every type is iterated on as two fp16 planes (22 bits, products and sums as in fp32).  One plane would
 // take a third of the products, and its 2^-12 looks small beside the 2^-9 of a bf16 result, but the iteration multiplies small singular values by
-// a^5 = 485 and what rounding spreads over their directions with them: a bf16 matrix of low rank comes out several percent off that way.  The Frobenius norm
-// is summed in 64 bits.  |X|, |S|, |Q| are bounded by the polynomial over [0, 1], which gives the powers of two that
+// a^5 = 485 and what rounding spreads over their directions with them: a bf16 matrix of low rank comes out several percent off that way.  The
+// Frobenius norm is summed in 64 bits.  |X|, |S|, |Q| are bounded by the polynomial over [0, 1], which gives the powers of two that
 // the planes are scaled by.  A matrix whose norm is far below eps comes out as nearly zero, as the definition has it, but without relative
 // accuracy.
 #include "pack.h"
