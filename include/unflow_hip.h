@@ -36,7 +36,7 @@ extern "C" {
 /* ABI version of this header (bumped on any signature change).  The library returns the value it was BUILT with; a C user
  * compares `unflow_abi_version() == UNFLOW_ABI_VERSION` (tools/capi_bench.cpp), the Python binding reads this very line
  * (unopticalflow_amd/_lib.py). */
-#define UNFLOW_ABI_VERSION 13
+#define UNFLOW_ABI_VERSION 14
 int unflow_abi_version(void);
 
 /* ---- kernel-exact timing (bench.py's roofline legs; nothing in the reference corresponds) ----
@@ -415,7 +415,7 @@ int unflow_prepare_triplets(const uint8_t* src, const long long* offsets, const 
                             const uint8_t* flip, float* dst, int B, int H, int W, int swap_rb,
                             void* stream);
 
-/* ---- training operators (ABI 13): a classification loss over many classes and an orthogonalising optimiser step.  Nothing in the reference
+/* ---- training operators (ABI 13; ABI 14: the _ex forms and unflow_linear_ce_bwd_workspace): a classification loss over many classes and an orthogonalising optimiser step.  Nothing in the reference
  * corresponds.  They take fp32, bf16 and fp16 tensors, 2-byte types aligned to 2 bytes, row-major. */
 #define UNFLOW_DTYPE_FP32 0
 #define UNFLOW_DTYPE_BF16 1
@@ -430,7 +430,10 @@ int unflow_prepare_triplets(const uint8_t* src, const long long* offsets, const 
  * The backward pass takes the upstream gradient gout ([N] for reduction 0, else [1]) and writes dhidden [N, D] and / or dweight [V, D] (dense,
  * in the inputs' type; NULL: not wanted), working through the classes in pieces.  Sums are fp32, in fixed order (bitwise reproducible).
  * unflow_linear_ce_workspace() says how many bytes are kept and how many each pass needs as workspace (256-byte aligned; its contents mean nothing
- * between calls).  The alignment of hidden and weight is part of the question: ask with the pointers of the call. */
+ * between calls).  The alignment of hidden and weight is part of the question: ask with the pointers of the call.  kept_bytes says with its last two
+ * bits which inputs the buffer holds packed (1 hidden, 2 weight); the _ex forms take it with the buffer and refuse any other size.
+ * unflow_linear_ce_bwd_ex() takes the same inputs in any layout, not only the forward pass's: what is neither held nor fit to be read in place it
+ * packs; unflow_linear_ce_bwd_workspace() says what it needs then.  unflow_linear_ce_bwd() takes the forward pass's own pointers and distances only. */
 #define UNFLOW_LCE_MAX_ROWS (1 << 20)      /* N; split longer batches */
 #define UNFLOW_LCE_MAX_CLASSES (1 << 30)   /* V */
 #define UNFLOW_LCE_MAX_DIM (1 << 20)       /* D, ldh, ldw */
@@ -440,6 +443,13 @@ int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, 
                          long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes, void* stream);
 int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* gout, int N, int V, int D, int dtype,
                          float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept, void* workspace, long long workspace_bytes, void* stream);
+int unflow_linear_ce_fwd_ex(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V, int D, int dtype, float scale,
+                            long long ignore_index, int reduction, float* loss, void* kept, long long kept_bytes, void* workspace, long long workspace_bytes, void* stream);
+int unflow_linear_ce_bwd_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype, int need_dhidden, int need_dweight,
+                                   long long kept_bytes, long long* backward_bytes);
+int unflow_linear_ce_bwd_ex(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* gout, int N, int V, int D, int dtype,
+                            float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept, long long kept_bytes, void* workspace,
+                            long long workspace_bytes, void* stream);
 
 /* Newton-Schulz orthogonalisation of `count` matrices of any shapes (HOST array of descriptors; everything is enqueued, nothing of it is kept):
  *   X = x / (|x|_F + eps);  `steps` times  X <- a X + (b S + c S S) X,  S = X X^T  (on the transpose of a matrix with more rows than columns)

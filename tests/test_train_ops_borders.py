@@ -1,0 +1,104 @@
+"""The training operators at the borders of what a caller may do: saved tensors that come back in another layout, other kinds of derivatives, many steps,
+optimiser groups and checkpoints.  References in 64 bits; the bounds are those of test_train_ops.py unless a test derives its own."""
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, 'tests'))
+
+from unopticalflow_amd import ops, optim  # noqa: E402
+from test_train_ops import DTYPES, _check_lce, _inputs, device  # noqa: E402,F401
+
+
+# ------------------------------------------------------------------------------------------ linear_cross_entropy under saved-tensor hooks
+def _cut(x, before, behind):
+    """x as columns of a wider matrix, NaN around it."""
+    wide = torch.full((len(x), before + x.shape[1] + behind), float('nan'), dtype=x.dtype, device=x.device)
+    wide[:, before:before + x.shape[1]] = x
+    return wide[:, before:before + x.shape[1]]
+
+
+def _shifted(t):
+    """A copy that starts one element behind an aligned address."""
+    room = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return room[1:].view(t.shape).copy_(t)
+
+
+RETURNS = {
+    'dense': lambda t: t.contiguous().clone(),
+    'shifted': _shifted,
+    'columns': lambda t: _cut(t, 3, 5) if t.is_floating_point() and t.dim() == 2 else _shifted(t),
+    'transposed': lambda t: t.mT.clone().mT if t.dim() == 2 else t.clone(),
+}
+
+
+@pytest.mark.parametrize('back', list(RETURNS))
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('rows,dim', [(9, 40), (20, 40), (33, 40), (70, 40), (70, 37)])
+def test_saved_tensors_in_another_layout(device, dtype, rows, dim, back):
+    """Offloading hands back what was saved in a layout of its own.  Every layout of the forward pass (aligned, wider rows, rows that start
+    anywhere, one of the two operands only) with every layout of the backward pass gives the bits of the call without hooks."""
+    h, w, t = _inputs(rows, 50, dim, dtype, device)
+    layouts = (lambda x: x, lambda x: _cut(x, 0, 24), lambda x: _cut(x, 1, 0), _shifted)
+    for lay_h, lay_w in [(a, a) for a in layouts] + [(layouts[0], layouts[2]), (layouts[2], layouts[0])]:
+        a, b = lay_h(h).requires_grad_(), lay_w(w).requires_grad_()
+        want = torch.autograd.grad(ops.linear_cross_entropy(a, b, t), (a, b))
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, RETURNS[back]):
+            got = torch.autograd.grad(ops.linear_cross_entropy(a, b, t), (a, b))
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_offloading_to_the_host(device):
+    h, w, t = _inputs(70, 50, 40, torch.float32, device)
+    a, b = _cut(h, 0, 24).requires_grad_(), _cut(w, 3, 5).requires_grad_()
+    want = torch.autograd.grad(ops.linear_cross_entropy(a, b, t), (a, b))
+    with torch.autograd.graph.save_on_cpu():
+        got = torch.autograd.grad(ops.linear_cross_entropy(a, b, t), (a, b))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_saved_tensors_of_another_kind_are_refused():
+    """What a hook hands back has to be what was saved: another type, shape or size is an error before anything is launched."""
+    import train_on_host
+    with train_on_host.patched():
+        h, w, t = _inputs(70, 50, 40, torch.float32, 'cpu')
+        h.requires_grad_()
+        for wrong in (lambda x: x.to(torch.bfloat16) if x.is_floating_point() else x, lambda x: x[:-1] if x.dim() == 2 else x,
+                      lambda x: x[:, :-1] if x.dim() == 2 else x, lambda x: x[:-1] if x.dtype == torch.int64 else x,
+                      lambda x: x[:-256] if x.dtype == torch.uint8 else x, lambda x: x.int() if x.dtype == torch.int64 else x):
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: x, wrong):
+                loss = ops.linear_cross_entropy(h, w, t)
+                with pytest.raises(RuntimeError):
+                    torch.autograd.grad(loss, h)
+
+
+def test_entry_points_check_what_was_kept():
+    """The C entries take the size of what the forward pass kept, whose last bits say which inputs it holds packed."""
+    import ctypes
+    import __graft_entry__ as ge
+    ge.build()
+    from unopticalflow_amd import _lib
+    lib = _lib.load()
+    k, a, b = ctypes.c_longlong(), ctypes.c_longlong(), ctypes.c_longlong()
+
+    def kept(hidden, weight, n=100, dtype=1):
+        assert lib.unflow_linear_ce_workspace(hidden, 40, weight, 40, n, 50, 40, dtype, 1, 1, ctypes.byref(k), ctypes.byref(a), ctypes.byref(b)) == 0
+        return k.value
+    base, off = 4096, 4098
+    sizes = [kept(base, base), kept(off, base), kept(base, off), kept(off, off)]
+    assert [s % 256 for s in sizes] == [0, 1, 2, 3] and kept(base, base, dtype=0) % 256 == 3
+    assert kept(off, off, 16) % 256 == 0 and kept(base, off, 20) % 256 == 0          # few rows: nothing but statistics
+    fwd = lambda size: lib.unflow_linear_ce_fwd_ex(off, 40, off, 40, base, 100, 50, 40, 1, 1.0, -100, 1, base, base, size, base, 16, None)  # noqa: E731
+    assert all(fwd(s) == -22 for s in sizes + [0, -1])                               # (a workspace of 16 bytes, or a wrong size)
+    need = lambda size, dtype=1, n=100: lib.unflow_linear_ce_bwd_workspace(off, 40, off, 40, n, 50, 40, dtype, 1, 1, size, ctypes.byref(b))  # noqa: E731
+    assert all(need(s) == 0 and b.value > 0 for s in sizes)
+    assert all(need(s) == -22 for s in [x + 256 for x in sizes] + [sizes[0] + 1, sizes[3] - 1, 0, -1]) and need(sizes[3], n=130) == -22
+    # (100 rows and 101 need as many lines of 256 bytes, 1604 or 1620 bytes of statistics and 8000 or 8080 of packed rows, so one's buffer is large enough for the other)
+    assert need(sizes[3], n=101) == 0
+    whole = kept(base, base, dtype=0)
+    assert need(whole, 0) == 0 and need(whole - 1, 0) == -22 and need(whole - 2, 0) == -22
+    bwd = lambda size, at=base: lib.unflow_linear_ce_bwd_ex(off, 40, off, 40, base, base, 100, 50, 40, 1, 1.0, -100, 1, base, None, at, size, base, 1 << 40, None)  # noqa: E731
+    assert bwd(sizes[3] + 256) == -22 and bwd(0) == -22 and bwd(sizes[3], None) == -22 and bwd(sizes[3], base + 2) == -22

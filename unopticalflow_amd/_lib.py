@@ -105,6 +105,9 @@ SIGNATURES = {
     'unflow_linear_ce_workspace': [_P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P],
     'unflow_linear_ce_fwd': [_P, _L, _P, _L, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P],
     'unflow_linear_ce_bwd': [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _P, _L, _P],
+    'unflow_linear_ce_fwd_ex': [_P, _L, _P, _L, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _L, _P, _L, _P],
+    'unflow_linear_ce_bwd_workspace': [_P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _L, _P],
+    'unflow_linear_ce_bwd_ex': [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P, _L, _P],
     'unflow_orthogonalize_workspace': [_P, _I, _I, _P],
     'unflow_orthogonalize': [_P, _I, _I, _I, _F, _F, _F, _F, _P, _L, _P],
     'unflow_muon_step': [_P, _I, _I, _F, _F, _F, _I, _I, _F, _F, _F, _F, _P, _L, _P],
@@ -132,7 +135,7 @@ class UnflowLibraryError(RuntimeError):
 # The ABI this file's SIGNATURES table was written for.  Bump it together with UNFLOW_ABI_VERSION of include/unflow_hip.h whenever an
 # entry point changes: load() wants library == header == this number, so a header bump + rebuild with a stale ctypes table is caught
 # (reading the number from the header alone only detects a stale .so).
-BINDING_ABI = 13
+BINDING_ABI = 14
 
 
 def _abi_version():

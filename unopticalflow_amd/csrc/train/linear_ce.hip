@@ -626,17 +626,25 @@ template <int PL, int EL, class F> static void with_tile(int size, F&& f) {
     else f(Tile<64, 64, 2, 2, 4, PL, EL>{});
 }
 
-// What a call needs of its buffers, and where.  `kept`: what the forward pass leaves for the backward pass.
+// the packed inputs of a call, as bits
+enum { kPackedH = 1, kPackedW = 2, kPackedBoth = 3 };
+
+// What a call needs of its buffers, and where.  `kept` is what the forward pass leaves for the backward pass: statistics of the rows, and those of the
+// inputs that it has packed (`held`).  Where the backward pass finds an input neither held nor fit to be read in place, it packs it into its
+// workspace: the two passes may see the same inputs in different layouts.
+struct Layout { long long maxima, eh, ew, hp, wp; };     // of packed inputs (offsets; those of what is not there are not used)
 struct Plan {
     int planes;
-    bool few, pack_h, pack_w, keeps;
+    bool few;
+    int packed, held;
     long long wd, wn;                    // packed widths of D and N
-    long long stats, maxima, eh, ew, hp, wp, kept_bytes;
+    long long stats, kept_bytes;
+    Layout in_kept, in_workspace;
     int size_z;
     long long partial, ztarget, losses, forward_bytes;
     int vp, size_g, size_p, limit;
     long long wvp, ldc;
-    long long repacked, magnitudes, exponents, largest, g, gt, ht, wt, sum_h, sum_w, backward_bytes;
+    long long magnitudes, exponents, largest, g, gt, ht, wt, sum_h, sum_w, backward_bytes;
 };
 
 // classes a workgroup of lce_few_kernel takes
@@ -648,30 +656,43 @@ static bool aligned(const void* p, long long ld, int D, int dtype) {
     return D % each == 0 && ld % each == 0 && ((size_t)p & 15) == 0;
 }
 
-static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, bool train, bool need_h,
+struct Taken {
+    long long bytes = 0;
+    long long operator()(long long n) { const long long at = bytes; bytes += round_up(n, 256); return at; }
+};
+static Layout layout_of(Taken& take, int packed, int planes, int N, int V, long long wd) {
+    Layout l{};
+    if (packed && planes == TWO) {
+        l.maxima = take(2 * kMaxima * 4);
+        l.eh = take(4ll * N);
+        l.ew = take(4ll * V);
+    }
+    if (packed & kPackedH) l.hp = take(2 * wd * N);
+    if (packed & kPackedW) l.wp = take(2 * wd * V);
+    return l;
+}
+// The size of what is kept also says what it holds: whole lines of 256 bytes, and the bits of the packed inputs.  Two layouts never have one size.
+static long long kept_of(Plan& p, int N, int V) {
+    Taken take;
+    p.stats = take(4ll * (4 * (long long)N + 1));
+    p.in_kept = layout_of(take, p.held, p.planes, N, V, p.wd);
+    return take.bytes + p.held;
+}
+
+// held: the inputs that `kept` holds packed, of a backward pass; -1: a forward pass decides that
+static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, int N, int V, int D, int dtype, int held, bool train, bool need_h,
         bool need_w) {
     Plan p{};
     p.planes = dtype == kFp32 ? TWO : ONE;
-    p.pack_h = dtype == kFp32 || !aligned(h, ldh, D, dtype);
-    p.pack_w = dtype == kFp32 || !aligned(w, ldw, D, dtype);
-    p.few = N <= (dtype == kFp32 ? 64 : p.pack_w ? 32 : 16) && D >= (dtype == kFp32 ? 4 : 8);
-    p.keeps = (p.pack_h || p.pack_w) && !p.few;
     p.wd = packed_width(p.planes, D);
     p.wn = packed_width(p.planes, N);
+    p.packed = dtype == kFp32 ? kPackedBoth : (aligned(h, ldh, D, dtype) ? 0 : kPackedH) | (aligned(w, ldw, D, dtype) ? 0 : kPackedW);
+    p.few = N <= (dtype == kFp32 ? 64 : p.packed & kPackedW ? 32 : 16) && D >= (dtype == kFp32 ? 4 : 8);
+    p.held = held >= 0 ? held : p.few ? 0 : p.packed;
+    p.packed |= p.held;
+    p.kept_bytes = kept_of(p, N, V);
     long long at = 0;
     auto take = [&](long long bytes) { const long long a = at; at += round_up(bytes, 256); return a; };
-    p.stats = take(4ll * (4 * (long long)N + 1));
-    const long long bare = at;
-    if (p.planes == TWO) {
-        p.maxima = take(2 * kMaxima * 4);
-        p.eh = take(4ll * N);
-        p.ew = take(4ll * V);
-    }
-    if (p.pack_h) p.hp = take(2 * p.wd * N);
-    if (p.pack_w) p.wp = take(2 * p.wd * V);
-    const long long packed = at;
-    p.kept_bytes = p.keeps ? packed : bare;
-    at = 0;
     const Job z{N, V, stages_of(p.wd), false, false, 0.};
     p.size_z = choose(p.planes, &z, 1).size;
     p.partial = take(8ll * ceil_div(V, p.few ? few_classes(N) : kSizes[p.size_z]) * N);
@@ -679,8 +700,9 @@ static Plan plan_of(const void* h, long long ldh, const void* w, long long ldw, 
     p.losses = take(4ll * N);
     p.forward_bytes = at;
     if (!train) return p;
-    at = 0;
-    if (p.few && (p.pack_h || p.pack_w)) p.repacked = take(packed);
+    Taken repacked;
+    p.in_workspace = layout_of(repacked, p.packed & ~p.held, p.planes, N, V, p.wd);
+    at = repacked.bytes;
     // A piece of G and its transpose take 256 MB at most (and hold 1024 classes at least): as long as a piece's two products fill the chip and
     // sum over thousands of classes, larger pieces gain nothing.
     const long long per_class = 2ll * p.planes * 2 * round_up(N, 32);
@@ -727,14 +749,22 @@ struct Inputs { const void* h; long long ldh; const void* w; long long ldw; cons
 
 static int pack_blocks(int rows) { return rows > 4 * kMaxima ? kMaxima : ceil_div(rows, 4); }
 
-// H and W as operands: as they are, or packed at `to`
+// H and W as operands: as they are, packed in `kept` or packed in `ws`; those of `pack` are packed now (where they go: all of them in one buffer).
+// The largest magnitudes of packed fp32 inputs are left in `maxima`.
 template <class T, int PL, int EL>
-static Logits operands(const Plan& p, const Inputs& in, char* to, bool pack, hipStream_t stream, Operand& H, Operand& W) {
-    H = p.pack_h ? Operand{(const u16*)(to + p.hp), p.wd, in.N} : Operand{(const u16*)in.h, in.ldh, in.N};
-    W = p.pack_w ? Operand{(const u16*)(to + p.wp), p.wd, in.V} : Operand{(const u16*)in.w, in.ldw, in.V};
-    const Packed at{(u16*)(to + p.hp), (u16*)(to + p.wp), (int*)(to + p.eh), (int*)(to + p.ew), (float*)(to + p.maxima)};
-    if (pack && (p.pack_h || p.pack_w)) {
-        const int blocks_h = p.pack_h ? pack_blocks(in.N) : 0, blocks_w = p.pack_w ? pack_blocks(in.V) : 0;
+static Logits operands(const Plan& p, const Inputs& in, int pack, char* kept, char* ws, hipStream_t stream, Operand& H, Operand& W,
+        float*& maxima) {
+    u16 *hp = (u16*)(p.held & kPackedH ? kept + p.in_kept.hp : ws + p.in_workspace.hp),
+        *wp = (u16*)(p.held & kPackedW ? kept + p.in_kept.wp : ws + p.in_workspace.wp);
+    // (fp32 inputs are packed both or not at all, into one buffer)
+    const Layout& l = p.held ? p.in_kept : p.in_workspace;
+    char* of_both = p.held ? kept : ws;
+    H = p.packed & kPackedH ? Operand{hp, p.wd, in.N} : Operand{(const u16*)in.h, in.ldh, in.N};
+    W = p.packed & kPackedW ? Operand{wp, p.wd, in.V} : Operand{(const u16*)in.w, in.ldw, in.V};
+    maxima = (float*)(of_both + l.maxima);
+    const Packed at{hp, wp, (int*)(of_both + l.eh), (int*)(of_both + l.ew), maxima};
+    if (pack) {
+        const int blocks_h = pack & kPackedH ? pack_blocks(in.N) : 0, blocks_w = pack & kPackedW ? pack_blocks(in.V) : 0;
         UNFLOW_LAUNCH((pack_inputs_kernel<T, PL, EL>), dim3(blocks_h + blocks_w), dim3(256), 0, stream,
             Source{in.h, in.ldh, in.N, in.D, in.target, in.ignore}, Source{in.w, in.ldw, in.V, in.D}, blocks_h, at, p.wd,
             (int)(PL == TWO ? p.wd / 2 : p.wd));
@@ -761,7 +791,8 @@ static void forward(const Plan& p, const Inputs& in, int reduction, float* loss,
         else if constexpr (PL == TWO) launch(lce_few_kernel<T, 4, 2, 2>);
     } else {
         Operand H, W;
-        const Logits how = operands<T, PL, EL>(p, in, kept, true, stream, H, W);
+        float* maxima;
+        const Logits how = operands<T, PL, EL>(p, in, p.packed, kept, ws, stream, H, W, maxima);
         columns = ceil_div(in.V, kSizes[p.size_z]);
         with_tile<PL, EL>(p.size_z, [&](auto tile) {
             using TileT = decltype(tile);
@@ -791,11 +822,11 @@ template <class T, int PL, int EL>
 static void backward(const Plan& p, const Inputs& in, int reduction, const float* gout, void* dh, void* dw, char* kept, char* ws,
         hipStream_t stream) {
     const float* stats = (const float*)(kept + p.stats);
-    char* to = p.keeps ? kept : ws + p.repacked;
     Operand H, W;
-    const Logits how = operands<T, PL, EL>(p, in, to, !p.keeps, stream, H, W);
+    float* maxima;
+    const Logits how = operands<T, PL, EL>(p, in, p.packed & ~p.held, kept, ws, stream, H, W, maxima);
     Exponents* ex = (Exponents*)(ws + p.exponents);
-    float* maxima = (float*)(PL == TWO ? to + p.maxima : ws + p.magnitudes);
+    if (PL == ONE) maxima = (float*)(ws + p.magnitudes);
     if constexpr (kScaled<T> && PL == ONE) {
         const int blocks_h = dw ? pack_blocks(in.N) : 0, blocks_w = dh ? pack_blocks(in.V) : 0;
         UNFLOW_LAUNCH(lce_magnitudes_kernel, dim3(blocks_h + blocks_w), dim3(256), 0, stream, H, W, (int)(p.wd / 8), blocks_h, in.target, in.ignore,
@@ -866,19 +897,41 @@ static bool sizes_ok(long long ldh, long long ldw, int N, int V, int D, int dtyp
 extern "C" int unflow_linear_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype,
         int need_dhidden, int need_dweight, long long* kept_bytes, long long* forward_bytes, long long* backward_bytes) {
     UNFLOW_REQUIRE(kept_bytes && forward_bytes && backward_bytes && sizes_ok(ldh, ldw, N, V, D, dtype, 0));
-    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, need_dhidden || need_dweight, need_dhidden != 0, need_dweight != 0);
+    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, -1, need_dhidden || need_dweight, need_dhidden != 0, need_dweight != 0);
     *kept_bytes = p.kept_bytes;
     *forward_bytes = p.forward_bytes;
     *backward_bytes = p.backward_bytes;
     return 0;
 }
 
-extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V,
-        int D, int dtype, float scale, long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes,
-        void* stream) {
+// what a buffer of this size holds, or -1 where no forward pass of these sizes keeps as much
+static int held_in(long long kept_bytes, int N, int V, int D, int dtype) {
+    if (kept_bytes < 0) return -1;
+    Plan p{};
+    p.planes = dtype == kFp32 ? TWO : ONE;
+    p.wd = packed_width(p.planes, D);
+    p.held = (int)(kept_bytes % 256);
+    if (p.held > kPackedBoth || (dtype == kFp32 && p.held != 0 && p.held != kPackedBoth) || kept_of(p, N, V) != kept_bytes) return -1;
+    return p.held;
+}
+
+extern "C" int unflow_linear_ce_bwd_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int N, int V, int D, int dtype,
+        int need_dhidden, int need_dweight, long long kept_bytes, long long* backward_bytes) {
+    UNFLOW_REQUIRE(backward_bytes && (need_dhidden || need_dweight) && sizes_ok(ldh, ldw, N, V, D, dtype, 0));
+    const int held = held_in(kept_bytes, N, V, D, dtype);
+    UNFLOW_REQUIRE(held >= 0);
+    *backward_bytes = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, held, true, need_dhidden != 0, need_dweight != 0).backward_bytes;
+    return 0;
+}
+
+// kept_bytes -1: as large as unflow_linear_ce_workspace said, by the caller's word
+static int forward_call(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V, int D, int dtype,
+        float scale, long long ignore_index, int reduction, float* loss, void* kept, long long kept_bytes, void* workspace,
+        long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(hidden && weight && target && loss && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
-    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, false, false, false);
-    UNFLOW_REQUIRE(workspace_bytes >= p.forward_bytes);
+    UNFLOW_REQUIRE(((size_t)kept & 15) == 0 && ((size_t)workspace & 15) == 0);
+    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, -1, false, false, false);
+    UNFLOW_REQUIRE(workspace_bytes >= p.forward_bytes && (kept_bytes == -1 || kept_bytes == p.kept_bytes));
     const Inputs in{hidden, ldh, weight, ldw, target, ignore_index, N, V, D, scale};
     char *k = (char*)kept, *ws = (char*)workspace;
     if (dtype == kFp32) forward<float, TWO, FP16>(p, in, reduction, loss, k, ws, (hipStream_t)stream);
@@ -887,11 +940,28 @@ extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const voi
     return unflow_launch_status();
 }
 
-extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
-        const float* gout, int N, int V, int D, int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight,
-        const void* kept, void* workspace, long long workspace_bytes, void* stream) {
+extern "C" int unflow_linear_ce_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V,
+        int D, int dtype, float scale, long long ignore_index, int reduction, float* loss, void* kept, void* workspace, long long workspace_bytes,
+        void* stream) {
+    return forward_call(hidden, ldh, weight, ldw, target, N, V, D, dtype, scale, ignore_index, reduction, loss, kept, -1, workspace, workspace_bytes,
+        stream);
+}
+
+extern "C" int unflow_linear_ce_fwd_ex(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int N, int V,
+        int D, int dtype, float scale, long long ignore_index, int reduction, float* loss, void* kept, long long kept_bytes, void* workspace,
+        long long workspace_bytes, void* stream) {
+    UNFLOW_REQUIRE(kept_bytes >= 0);
+    return forward_call(hidden, ldh, weight, ldw, target, N, V, D, dtype, scale, ignore_index, reduction, loss, kept, kept_bytes, workspace,
+        workspace_bytes, stream);
+}
+
+// held -1: what a forward pass over these very pointers keeps
+static int backward_call(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, const float* gout, int N, int V,
+        int D, int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight, const void* kept, int held,
+        void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(hidden && weight && target && gout && (dhidden || dweight) && kept && workspace && sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
-    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, true, dhidden != nullptr, dweight != nullptr);
+    UNFLOW_REQUIRE(((size_t)kept & 15) == 0 && ((size_t)workspace & 15) == 0);
+    const Plan p = plan_of(hidden, ldh, weight, ldw, N, V, D, dtype, held, true, dhidden != nullptr, dweight != nullptr);
     UNFLOW_REQUIRE(workspace_bytes >= p.backward_bytes);
     const Inputs in{hidden, ldh, weight, ldw, target, ignore_index, N, V, D, scale};
     char *k = (char*)const_cast<void*>(kept), *ws = (char*)workspace;
@@ -899,4 +969,21 @@ extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const voi
     else if (dtype == kBf16) backward<__bf16, ONE, BF16>(p, in, reduction, gout, dhidden, dweight, k, ws, (hipStream_t)stream);
     else backward<_Float16, ONE, FP16>(p, in, reduction, gout, dhidden, dweight, k, ws, (hipStream_t)stream);
     return unflow_launch_status();
+}
+
+extern "C" int unflow_linear_ce_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
+        const float* gout, int N, int V, int D, int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight,
+        const void* kept, void* workspace, long long workspace_bytes, void* stream) {
+    return backward_call(hidden, ldh, weight, ldw, target, gout, N, V, D, dtype, scale, ignore_index, reduction, dhidden, dweight, kept, -1, workspace,
+        workspace_bytes, stream);
+}
+
+extern "C" int unflow_linear_ce_bwd_ex(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
+        const float* gout, int N, int V, int D, int dtype, float scale, long long ignore_index, int reduction, void* dhidden, void* dweight,
+        const void* kept, long long kept_bytes, void* workspace, long long workspace_bytes, void* stream) {
+    UNFLOW_REQUIRE(sizes_ok(ldh, ldw, N, V, D, dtype, reduction));
+    const int held = held_in(kept_bytes, N, V, D, dtype);
+    UNFLOW_REQUIRE(held >= 0);
+    return backward_call(hidden, ldh, weight, ldw, target, gout, N, V, D, dtype, scale, ignore_index, reduction, dhidden, dweight, kept, held, workspace,
+        workspace_bytes, stream);
 }

@@ -1803,39 +1803,57 @@ def _rows_of(t):
 
 
 def _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, need_h, need_w):
-    """-> loss, and what the backward pass takes: (hidden, weight, kept) and (ldh, ldw, dtype, bytes of its workspace)."""
+    """-> loss, and what the backward pass takes: (hidden, weight, kept) and (where and how far apart their rows lay, dtype, bytes kept, bytes of
+    its workspace for that layout)."""
     dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
     (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
     (N, D), V = hidden.shape, weight.shape[0]
     loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
     if N == 0:
-        return loss.zero_(), (hidden, weight, None), (ldh, ldw, dtype, 0)
+        return loss.zero_(), (hidden, weight, None), None
     with _on(dev):
         sizes = (ctypes.c_longlong * 3)()                # bytes kept for the backward pass, of the forward's workspace, of the backward's
         at, ph, pw = ctypes.addressof(sizes), hidden.data_ptr(), weight.data_ptr()
         _call('unflow_linear_ce_workspace', ph, ldh, pw, ldw, N, V, D, dtype, need_h, need_w, at, at + 8, at + 16)
         kept = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
         ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
-        _call('unflow_linear_ce_fwd', ph, ldh, pw, ldw, target.data_ptr(), N, V, D, dtype, scale, ignore_index, reduction,
-              loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), sizes[1], _stream_of(dev), nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
-    return loss, (hidden, weight, kept), (ldh, ldw, dtype, sizes[2])
+        _call('unflow_linear_ce_fwd_ex', ph, ldh, pw, ldw, target.data_ptr(), N, V, D, dtype, scale, ignore_index, reduction,
+              loss.data_ptr(), kept.data_ptr(), sizes[0], ws.data_ptr(), sizes[1], _stream_of(dev), nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+    return loss, (hidden, weight, kept), ((ph, ldh, pw, ldw), dtype, sizes[0], sizes[2])
 
 
 def _linear_ce_backward(ctx, g):
+    # (what was saved may come back, from hooks that offload it, at another place and in another layout)
     hidden, weight, target, kept = ctx.saved_tensors
-    (ignore_index, scale, reduction), (ldh, ldw, dtype, need) = ctx.options, ctx.how
+    ignore_index, scale, reduction = ctx.options
     need_h, need_w = ctx.needs_input_grad[:2]
-    (N, D), V, dev = hidden.shape, weight.shape[0], hidden.device
+    (N, D), V = ctx.shape, weight.shape[0]
+    dev = g.device
+    if any(x.device != dev for x in (hidden, weight, target) + (() if kept is None else (kept,))):
+        raise RuntimeError('linear_cross_entropy: the saved tensors came back on other devices than the gradient\'s, %s' % dev)
+    if hidden.shape != ctx.shape or weight.shape != (ctx.classes, D) or target.shape != (N,) or target.dtype != torch.int64:
+        raise RuntimeError('linear_cross_entropy: the saved tensors came back as others than they were')
     dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if need_h else None
     dw = torch.empty((V, D), dtype=weight.dtype, device=dev) if need_w else None
     if N == 0:
         return dh, dw.zero_() if need_w else None, None, None, None, None
+    where, dtype, kept_bytes, need = ctx.how
+    if _DTYPES.get(hidden.dtype) != dtype or weight.dtype != hidden.dtype or kept.dtype != torch.uint8 or kept.numel() != kept_bytes:
+        raise RuntimeError('linear_cross_entropy: the saved tensors came back as others than they were')
     with _on(dev):
+        (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
+        target, kept, g = target.contiguous(), kept.contiguous(), g.contiguous()
+        if kept.data_ptr() % 16:
+            kept = kept.clone()
+        ph, pw = hidden.data_ptr(), weight.data_ptr()
+        if (ph, ldh, pw, ldw) != where:
+            size = ctypes.c_longlong()
+            _call('unflow_linear_ce_bwd_workspace', ph, ldh, pw, ldw, N, V, D, dtype, need_h, need_w, kept_bytes, ctypes.addressof(size))
+            need = size.value
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        g = g.contiguous()
-        _call('unflow_linear_ce_bwd', hidden.data_ptr(), ldh, weight.data_ptr(), ldw, target.data_ptr(), g.data_ptr(), N, V, D,
+        _call('unflow_linear_ce_bwd_ex', ph, ldh, pw, ldw, target.data_ptr(), g.data_ptr(), N, V, D,
               dtype, scale, ignore_index, reduction, dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None,
-              kept.data_ptr(), ws.data_ptr(), need, _stream_of(dev),
+              kept.data_ptr(), kept_bytes, ws.data_ptr(), need, _stream_of(dev),
               nbytes=2 * (N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
     return dh, dw, None, None, None, None
 
@@ -1848,6 +1866,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, target, ignore_index, scale, reduction):
         loss, (hidden, weight, kept), ctx.how = _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, *ctx.needs_input_grad[:2])
         ctx.options = (ignore_index, scale, reduction)
+        ctx.shape, ctx.classes = tuple(hidden.shape), weight.shape[0]
         ctx.save_for_backward(hidden, weight, target, kept)
         return loss
 
