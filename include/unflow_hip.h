@@ -456,10 +456,13 @@ int unflow_linear_ce_bwd_ex(const void* hidden, long long ldh, const void* weigh
  * and out = X (unflow_orthogonalize), or with momentum as the optimiser step (unflow_muon_step; x = gradient, out = parameter)
  *   momentum += (1 - mu)(x - momentum);  u = nesterov ? x + mu (momentum - x) : momentum
  *   out = out (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X(u)
- * Matrices are dense row-major [rows, cols]; momentum is fp32 whatever the type.  Coefficients whose polynomial leaves [0, 16] are refused. */
+ * Matrices are dense row-major [rows, cols]; momentum is fp32 whatever the type.  Coefficients whose polynomial leaves [0, 16] are refused.
+ * unflow_orthogonalize_workspace_ex() says what a call with these steps and coefficients needs, unflow_orthogonalize_workspace() what is enough for
+ * any (lists of matrices of up to 32 rows or columns need much less for a few steps than for many). */
 #define UNFLOW_MATRIX_MAX_SIDE (1 << 18)
 typedef struct { const void* x; void* out; float* momentum; int rows, cols; } unflow_matrix;
 int unflow_orthogonalize_workspace(const unflow_matrix* matrices, int count, int dtype, long long* bytes);
+int unflow_orthogonalize_workspace_ex(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, long long* bytes);
 int unflow_orthogonalize(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, float eps, void* workspace, long long workspace_bytes, void* stream);
 int unflow_muon_step(const unflow_matrix* matrices, int count, int dtype, float lr, float momentum, float weight_decay, int nesterov, int steps, float a, float b, float c, float eps,
                      void* workspace, long long workspace_bytes, void* stream);

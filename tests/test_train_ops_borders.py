@@ -10,7 +10,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, 'tests'))
 
 from unopticalflow_amd import ops, optim  # noqa: E402
-from test_train_ops import DTYPES, _check_lce, _inputs, device  # noqa: E402,F401
+from test_train_ops import DTYPES, _check_orthogonal, _inputs, _matrix, device  # noqa: E402,F401
 
 
 # ------------------------------------------------------------------------------------------ linear_cross_entropy under saved-tensor hooks
@@ -102,3 +102,68 @@ def test_entry_points_check_what_was_kept():
     assert need(whole, 0) == 0 and need(whole - 1, 0) == -22 and need(whole - 2, 0) == -22
     bwd = lambda size, at=base: lib.unflow_linear_ce_bwd_ex(off, 40, off, 40, base, base, 100, 50, 40, 1, 1.0, -100, 1, base, None, at, size, base, 1 << 40, None)  # noqa: E731
     assert bwd(sizes[3] + 256) == -22 and bwd(0) == -22 and bwd(sizes[3], None) == -22 and bwd(sizes[3], base + 2) == -22
+
+
+# ------------------------------------------------------------------------------------------ orthogonalize: many steps
+def _deficient(kind, shape):
+    """Matrices of low rank, of numbers of 24 bits: products of thin factors, equal rows, one column alone."""
+    g = torch.Generator().manual_seed(0)
+    m, n = min(shape), max(shape)
+    if kind == 'equal rows':
+        x = torch.randn(1, n, generator=g).expand(m, n).clone()
+    elif kind == 'one column':
+        x = torch.zeros(m, n)
+        x[:, n // 2] = torch.randn(m, generator=g)
+    else:
+        x = torch.randn(m, kind, generator=g) @ torch.randn(kind, n, generator=g)
+    return x if shape[0] < shape[1] else x.T.contiguous()
+
+
+@pytest.mark.parametrize('coefficients,top', [((3.4445, -4.7750, 2.0315), 1.2025), ((2.0, -1.5, 0.5), 1.0018), ((1.5, -0.5, 0.0), 1.0)])
+@pytest.mark.parametrize('kind,shape', [(3, (20, 60)), (1, (8, 500)), ('equal rows', (16, 40)), (5, (300, 32)), ('one column', (32, 33))])
+@pytest.mark.parametrize('steps', [9, 12, 20, 40, 64])
+def test_few_rows_of_low_rank_stay_bounded(device, steps, kind, shape, coefficients, top):
+    """No singular value leaves what the polynomial reaches from [0, 1] (`top`), whatever rounding puts into the directions that the matrix does not
+    have: 22 bits of each of the step's three matrices, 2^-10 of them together, on top of it."""
+    x = _deficient(kind, shape).to(device)
+    got = ops.orthogonalize(x, steps=steps, coefficients=coefficients).double()
+    assert bool(torch.isfinite(got).all())
+    size = torch.linalg.svdvals(got.cpu())
+    assert float(size[0]) <= top * (1 + 2**-10), float(size[0])
+    assert float(size[kind - 1 if isinstance(kind, int) else 0]) >= 0.5
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_many_muon_steps_of_few_rows(device, dtype):
+    """A weight of few rows whose gradient has rank 1 moves by at most lr sqrt(max(1, rows / cols)) 1.2025 and the rounding of its type."""
+    p = torch.zeros(40, 24, dtype=dtype, device=device)
+    g = _deficient(1, (40, 24)).to(dtype).to(device)
+    optim.muon_step_([p], [g], [torch.zeros(40, 24, device=device)], lr=0.5, steps=30)
+    size = torch.linalg.svdvals(p.double().cpu())
+    assert bool(torch.isfinite(size).all())
+    assert float(size[0]) <= 0.5 * (40 / 24) ** 0.5 * 1.2025 * (1 + 2**-10) + torch.finfo(dtype).eps / 2 * float(p.double().norm())
+
+
+@pytest.mark.parametrize('steps', [1, 5, 7, 8, 9, 10, 11])
+def test_steps_on_both_sides_of_the_kernels_for_few_rows(device, steps):
+    x = _matrix(24, 90, dtype=torch.float32, device=device)
+    _check_orthogonal(ops.orthogonalize(x, steps=steps), x, steps=steps)
+
+
+def test_the_workspace_depends_on_the_steps():
+    """The size for given steps and coefficients is what a call checks; the one without them is enough for any."""
+    import ctypes
+    import __graft_entry__ as ge
+    ge.build()
+    from unopticalflow_amd import _lib
+    lib = _lib.load()
+    need, any_steps = ctypes.c_longlong(), ctypes.c_longlong()
+    for rows, cols in ((20, 60), (300, 7), (70, 90)):
+        m = (ops._Matrix * 1)((4096, 4096, None, rows, cols))
+        assert lib.unflow_orthogonalize_workspace(m, 1, 0, ctypes.byref(any_steps)) == 0
+        for steps in (1, 5, 12, 64):
+            assert lib.unflow_orthogonalize_workspace_ex(m, 1, 0, steps, 3.4445, -4.7750, 2.0315, ctypes.byref(need)) == 0
+            assert 0 < need.value <= any_steps.value
+            assert lib.unflow_orthogonalize(m, 1, 0, steps, 3.4445, -4.7750, 2.0315, 1e-7, 4096, need.value - 1, None) == -22
+    for bad in ((0, 3.4445, -4.7750, 2.0315), (65, 3.4445, -4.7750, 2.0315), (5, 9.0, 9.0, 9.0)):
+        assert lib.unflow_orthogonalize_workspace_ex(m, 1, 0, *bad, ctypes.byref(need)) == -22

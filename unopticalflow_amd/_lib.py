@@ -109,6 +109,7 @@ SIGNATURES = {
     'unflow_linear_ce_bwd_workspace': [_P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _L, _P],
     'unflow_linear_ce_bwd_ex': [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _F, _L, _I, _P, _P, _P, _L, _P, _L, _P],
     'unflow_orthogonalize_workspace': [_P, _I, _I, _P],
+    'unflow_orthogonalize_workspace_ex': [_P, _I, _I, _I, _F, _F, _F, _P],
     'unflow_orthogonalize': [_P, _I, _I, _I, _F, _F, _F, _F, _P, _L, _P],
     'unflow_muon_step': [_P, _I, _I, _F, _F, _F, _I, _I, _F, _F, _F, _F, _P, _L, _P],
     'unflow_png_unfilter': [_P, _I, _I, _I],

@@ -366,7 +366,10 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void apply_kernel(const Problem*
 // needs twice the digits (what rounding adds to S_0 is multiplied by a^10), so all sums are 64 bits, and that is what bounds m: the 17 products
 // of one workgroup take 17 m^3 fused operations at 64 a cycle (18 us for m = 32).  8 x 500: 30 us against 50 by the tiles, 8 of 32 x 1152 44 against
 // 98, 32 x 100000 122 against 382; and nearer to the formula than the tiles' planes, whose two roundings a step show where sums are short (4 x 512:
-// 3.5e-6 by the tiles, 1.5e-6 in fp32).  A list that has larger matrices goes by the tiles as a whole, whose launches are there anyhow (the flow
+// 3.5e-6 by the tiles, 1.5e-6 in fp32).  Rounding leaves S_0 directions of slightly negative size where the matrix has none; they grow by |a^2| a step,
+// and nothing holds them once they are no longer small (below zero the polynomial has no bound), so a list goes here only for as many steps as keep
+// them below 2^-10 (narrow_holds; 9 with the default coefficients).  Beyond, and in the tiles' own iteration, S is a product X X^T at every
+// step and cannot leave zero by more than its rounding.  A list that has larger matrices goes by the tiles as a whole, whose launches are there anyhow (the flow
 // network's weights: 252 us, 299 where those of few rows have their own kernels).
 constexpr int kNarrow = 32, kColumns = 128, kGramParts = 64;         // a workgroup takes 128 columns at a time; S_0 is summed in at most 64 parts
 constexpr int kNarrowNumbers = kNarrow * kColumns / 256;             // of a thread
@@ -610,6 +613,24 @@ static bool exponents_of(int steps, float a, float b, float c, Exponents& ex) {
     return true;
 }
 
+// log2 of how much `steps` times S <- Q S Q make of a small error in S at most: the largest |d (s q(s)^2) / ds| over the squares of all singular
+// values, to the power of `steps` (at s = 0, a direction the matrix does not have, it is a^2).  -1: the singular values leave [0, 16].
+static double growth_of(int steps, double a, double b, double c) {
+    double most = 0., top = 1.;
+    for (int k = 0; k <= steps; ++k) {                                   // the singular values after k steps lie in [0, top]
+        double next = 0.;
+        for (int i = 0; i <= 64; ++i) {
+            const double s = top * i / 64., t = s * s, q = a + b * t + c * t * t, slope = fabs(q * q + 2. * t * q * (b + 2. * c * t));
+            most = most > slope ? most : slope;
+            next = next > s * fabs(q) ? next : s * fabs(q);
+        }
+        if (next <= top && k > 0) break;                                 // (nothing new from here on)
+        top = top > next ? top : next;
+        if (!(top <= 16.)) return -1.;
+    }
+    return most > 1. ? steps * log2(most) : 0.;
+}
+
 constexpr long long kGroupBytes = 4ll << 30;                         // matrices are taken together as long as their planes fit in this
 
 struct Group {
@@ -657,15 +678,23 @@ static Problem problem_for(const unflow_matrix& q, int m, int n) {
     return p;
 }
 
+// Whether matrices of up to m <= n numbers a side may take the kernels for few rows, where an error in S grows by 2^growth.  S_0 is off by a rounding
+// for each number that is summed after another (the columns of a part and its chunks, then the parts), a step adds the roundings of three products
+// of m terms; all of it has to stay below 2^-10 of a singular value of 1.
+static bool narrow_holds(int m, int n, double growth) {
+    const int chunks = ceil_div(n, kColumns), parts = chunks < kGramParts ? chunks : kGramParts;
+    return m <= kNarrow && log2((double)ceil_div(chunks, parts) * kColumns + parts + 4. * m) - 53. + growth <= -10.;
+}
+
 // lays out a group: problems and running counts on the host (`table`: what g.table_bytes of the workspace will hold), offsets into the workspace
-static Group lay_out(const unflow_matrix* a, int first, int count, char* table) {
+static Group lay_out(const unflow_matrix* a, int first, int count, double growth, char* table) {
     static thread_local Sorted order;
     static thread_local Job jobs[kMost];
     sort_of(a, first, count, order);
     Group g{};
     g.first = first;
     g.count = count;
-    g.narrow = *std::max_element(order.m, order.m + count) <= kNarrow;
+    g.narrow = narrow_holds(*std::max_element(order.m, order.m + count), order.n[0], growth);
     long long at = 0, chunks = 0;
     auto take = [&](long long bytes) { const long long p = at; at += round_up(bytes, 256); return p; };
     g.ends = (long long)sizeof(Problem) * count;                     // (of the table)
@@ -827,16 +856,15 @@ static void iterate(const Group& g, int steps, float a, float b, float c, float 
     }
 }
 
-static int workspace_of(const unflow_matrix* a, int count, int dtype, long long* bytes) {
+static long long workspace_of(const unflow_matrix* a, int count, double growth) {
     long long most = 0;
     for (int i = 0; i < count;) {
         const int e = group_end(a, count, i);
-        const long long b = lay_out(a, i, e - i, nullptr).bytes;
+        const long long b = lay_out(a, i, e - i, growth, nullptr).bytes;
         most = most > b ? most : b;
         i = e;
     }
-    *bytes = most;
-    return 0;
+    return most;
 }
 
 template <bool STEP>
@@ -844,15 +872,14 @@ static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca
         void* workspace, long long workspace_bytes, void* stream_) {
     Exponents ex;
     UNFLOW_REQUIRE(exponents_of(steps, ca, cb, cc, ex));
-    long long need = 0;
-    workspace_of(a, count, dtype, &need);
-    UNFLOW_REQUIRE(workspace_bytes >= need);
+    const double growth = growth_of(steps, ca, cb, cc);
+    UNFLOW_REQUIRE(growth >= 0. && workspace_bytes >= workspace_of(a, count, growth));
     hipStream_t stream = (hipStream_t)stream_;
     char* ws = (char*)workspace;
     for (int i = 0; i < count;) {
         const int e = group_end(a, count, i), n = e - i;
         static thread_local struct alignas(8) { char bytes[kMost * (sizeof(Problem) + 4 * kTables)]; } table;
-        const Group g = lay_out(a, i, n, table.bytes);
+        const Group g = lay_out(a, i, n, growth, table.bytes);
         write_table(table.bytes, g.table_bytes, ws + g.table, stream);
         if (dtype == kFp32) iterate<float, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
         else if (dtype == kBf16) iterate<__bf16, STEP>(g, steps, ca, cb, cc, eps, mu, nesterov, up, ex, ws, stream);
@@ -866,7 +893,18 @@ static int run(const unflow_matrix* a, int count, int dtype, int steps, float ca
 
 extern "C" int unflow_orthogonalize_workspace(const unflow_matrix* matrices, int count, int dtype, long long* bytes) {
     UNFLOW_REQUIRE(bytes && matrices_ok(matrices, count, dtype));
-    return workspace_of(matrices, count, dtype, bytes);
+    // (without and with so many steps that nothing goes by the kernels for few rows)
+    *bytes = std::max(workspace_of(matrices, count, 0.), workspace_of(matrices, count, 1e3));
+    return 0;
+}
+
+extern "C" int unflow_orthogonalize_workspace_ex(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c,
+        long long* bytes) {
+    UNFLOW_REQUIRE(bytes && matrices_ok(matrices, count, dtype) && steps >= 1 && steps <= 64);
+    const double growth = growth_of(steps, a, b, c);
+    UNFLOW_REQUIRE(growth >= 0.);
+    *bytes = workspace_of(matrices, count, growth);
+    return 0;
 }
 
 extern "C" int unflow_orthogonalize(const unflow_matrix* matrices, int count, int dtype, int steps, float a, float b, float c, float eps,

@@ -1944,13 +1944,13 @@ def _check_newton_schulz(what, steps, coefficients, eps):
     return key
 
 
-def _newton_schulz(entry, dev, dtype, table, count, args):
+def _newton_schulz(entry, dev, dtype, table, count, before, steps, coefficients, eps):
     """One call of an entry point that takes a list of matrices and a workspace."""
     with _on(dev):
         need = ctypes.c_longlong()
-        _call('unflow_orthogonalize_workspace', table, count, dtype, ctypes.addressof(need))
+        _call('unflow_orthogonalize_workspace_ex', table, count, dtype, steps, *coefficients, ctypes.addressof(need))
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        _call(entry, table, count, dtype, *args, ws.data_ptr(), need.value, _stream_of(dev))
+        _call(entry, table, count, dtype, *before, steps, *coefficients, float(eps), ws.data_ptr(), need.value, _stream_of(dev))
 
 
 def orthogonalize(matrices, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
@@ -1977,5 +1977,5 @@ def orthogonalize(matrices, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps
         if each:
             items += [(t.data_ptr() + k * each * size, o.data_ptr() + k * each * size, None, t.shape[-2], t.shape[-1]) for k in range(t.numel() // each)]
     if items:
-        _newton_schulz('unflow_orthogonalize', dev, dtype, (_Matrix * len(items))(*items), len(items), (steps, *coefficients, float(eps)))
+        _newton_schulz('unflow_orthogonalize', dev, dtype, (_Matrix * len(items))(*items), len(items), (), steps, coefficients, eps)
     return outs[0] if single else outs

@@ -206,7 +206,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
     if len({x[1] for x in items} | {x[2] for x in items}) < 2 * len(items):
         raise ValueError('muon_step_: a parameter or momentum appears twice')
     ops._newton_schulz('unflow_muon_step', dev, dtype, (ops._Matrix * len(items))(*items), len(items),
-                       (float(lr), float(momentum), float(weight_decay), int(bool(nesterov)), steps, *coefficients, float(eps)))
+                       (float(lr), float(momentum), float(weight_decay), int(bool(nesterov))), steps, coefficients, eps)
 
 
 class FlowMuon(torch.optim.Optimizer):
