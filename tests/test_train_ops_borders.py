@@ -167,3 +167,50 @@ def test_the_workspace_depends_on_the_steps():
             assert lib.unflow_orthogonalize(m, 1, 0, steps, 3.4445, -4.7750, 2.0315, 1e-7, 4096, need.value - 1, None) == -22
     for bad in ((0, 3.4445, -4.7750, 2.0315), (65, 3.4445, -4.7750, 2.0315), (5, 9.0, 9.0, 9.0)):
         assert lib.unflow_orthogonalize_workspace_ex(m, 1, 0, *bad, ctypes.byref(need)) == -22
+
+
+# ------------------------------------------------------------------------------------------ linear_cross_entropy: derivatives and tracers of other kinds
+@pytest.mark.parametrize('which', ['hidden', 'weight'])
+@pytest.mark.parametrize('no_grad', [False, True])
+def test_no_forward_mode_derivative(device, which, no_grad):
+    """A tangent is refused, as it is where an input asks for a gradient; it does not disappear."""
+    from torch.autograd import forward_ad
+    h, w, t = _inputs(5, 7, 8, torch.float32, device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(h if which == 'hidden' else w, torch.ones_like(h if which == 'hidden' else w))
+        with torch.set_grad_enabled(not no_grad), pytest.raises(NotImplementedError):
+            ops.linear_cross_entropy(*((dual, w) if which == 'hidden' else (h, dual)), t)
+        assert torch.isfinite(ops.linear_cross_entropy(h, w, t))             # (without tangents it is an ordinary call)
+
+
+@pytest.mark.parametrize('gradient', [False, True])
+def test_a_trace_calls_the_operator(device, gradient):
+    """torch.jit.trace records the call, not the values of the traced one."""
+    h, w, t = _inputs(5, 7, 8, torch.float32, device)
+    h.requires_grad_(gradient)
+    with pytest.warns(torch.jit.TracerWarning):
+        traced = torch.jit.trace(lambda a, b: ops.linear_cross_entropy(a, b, t), (h, w), check_trace=False)
+    other = _inputs(5, 7, 8, torch.float32, device, seed=1)[0]
+    assert torch.equal(traced(other, w), ops.linear_cross_entropy(other, w, t))
+
+
+def test_tracers_that_would_record_constants_are_refused(device):
+    """make_fx sees the allocations around a kernel only, and jit.trace those of an operator that is no autograd function."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    h, w, t = _inputs(5, 7, 8, torch.float32, device)
+    for x in (h, h.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match='trace'):
+            make_fx(lambda a: ops.linear_cross_entropy(a, w, t))(x)
+    with pytest.raises(RuntimeError, match='trace'):
+        make_fx(lambda a: ops.orthogonalize(a))(h)
+    with pytest.raises(RuntimeError, match='trace'):
+        torch.jit.trace(lambda a: ops.orthogonalize(a), (h,), check_trace=False)
+    m = torch.zeros_like(h)
+
+    def step(p, g):
+        optim.muon_step_([p], [g], [m], lr=0.1)
+        return p
+    for tracer in (lambda: make_fx(step)(h.clone(), h), lambda: torch.jit.trace(step, (h.clone(), h), check_trace=False)):
+        with pytest.raises(RuntimeError, match='trace'):
+            tracer()
+    assert not m.any()

@@ -7,6 +7,7 @@ PyTorch supplies device memory (caching allocator) and the current stream; the k
 called through the plain-C ABI of ``include/unflow_hip.h`` with raw pointers.
 """
 import ctypes
+import sys
 
 import numpy as np
 import torch
@@ -1775,6 +1776,14 @@ _MATRIX_MAX_SIDE = 1 << 18
 _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
 
 
+def _refuse_tracers(what, jit=True):
+    """Tracers that run the Python code and record what torch does in it (make_fx; ``jit``: torch.jit.trace) would see the allocations around a
+    kernel and not the kernel: what they recorded would return memory that nothing has written."""
+    fx = sys.modules.get('torch.fx.experimental.proxy_tensor')
+    if (jit and torch._C._is_tracing()) or (fx is not None and fx.get_proxy_mode() is not None):
+        raise RuntimeError('%s is a kernel behind raw pointers: a trace would not hold it' % what)
+
+
 def _dev_typed(what, *tensors):
     """All operands on one HIP device and of one of the types the training operators take -> (device, UNFLOW_DTYPE_*)."""
     devices, dtypes = {t.device for t in tensors}, {t.dtype for t in tensors}
@@ -1805,6 +1814,7 @@ def _rows_of(t):
 def _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, need_h, need_w):
     """-> loss, and what the backward pass takes: (hidden, weight, kept) and (where and how far apart their rows lay, dtype, bytes kept, bytes of
     its workspace for that layout)."""
+    _refuse_tracers('linear_cross_entropy', jit=False)
     dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
     (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
     (N, D), V = hidden.shape, weight.shape[0]
@@ -1887,6 +1897,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
     and no part in the gradients, whatever it holds; any other target outside [0, V) makes its row's loss, and
     the gradients it reaches, NaN.  Results are bitwise reproducible.
 
+    Neither forward-mode nor second derivatives exist (both are errors); torch.jit.trace records the call, other tracers are refused.
     Between the passes 16 bytes per row are kept, and for fp32 inputs (or rows that are not multiples of 16 bytes) a packed copy of both."""
     if reduction not in _REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction must be 'mean', 'sum' or 'none', got {!r}".format(reduction))
@@ -1905,7 +1916,9 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
     else:
         flat = target
     args = (hidden, weight, flat.contiguous(), int(ignore_index), float(scale), _REDUCTIONS[reduction])
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    # (where nothing asks for a gradient the autograd function is passed over; forward-mode derivatives, which it refuses, and torch.jit.trace, which
+    # records its call, have to meet it)
+    if (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)) or torch.autograd.forward_ad._current_level >= 0 or torch._C._is_tracing():
         loss = _LinearCrossEntropy.apply(*args)
     else:
         loss = _linear_ce_forward(*args, False, False)[0]
@@ -1959,6 +1972,7 @@ def orthogonalize(matrices, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps
 
     ``matrices``: one tensor [..., rows, cols], or a list of such tensors of any shapes (fp32, bf16 or fp16, one type), all of which are
     worked on together.  Returns the same in the same type; the iteration has the accuracy of fp32 whatever the type.  Not differentiable: it makes updates out of gradients."""
+    _refuse_tracers('orthogonalize')
     single = torch.is_tensor(matrices)
     given = [matrices] if single else list(matrices)
     for t in given:

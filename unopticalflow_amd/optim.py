@@ -176,6 +176,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
 
     ``params`` and ``grads`` are fp32, bf16 or fp16 (one type), ``momenta`` fp32 in their parameters' layout (row-major or channels_last;
     a gradient in another layout is copied).  No weight may appear twice."""
+    ops._refuse_tracers('muon_step_')
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError('muon_step_: %d parameters, %d gradients, %d momenta' % (len(params), len(grads), len(momenta)))
