@@ -214,3 +214,30 @@ def test_tracers_that_would_record_constants_are_refused(device):
         with pytest.raises(RuntimeError, match='trace'):
             tracer()
     assert not m.any()
+
+
+# ------------------------------------------------------------------------------------------ linear_cross_entropy: gradients far from 1
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('dtype,sizes', [
+    (torch.float32, (2.0**-40, 2.0**-66, 1.0)), (torch.float32, (2.0**-46, 2.0**-66, 1.0)), (torch.float32, (2.0**-53, 2.0**-66, 1.0)),
+    (torch.float32, (2.0**-60, 2.0**60, 2.0**-66)), (torch.float32, (2.0**60, 2.0**-100, 1.0)), (torch.float32, (2.0**-60, 2.0**-10, 2.0**-20)),
+    (torch.float32, (2.0**40, 2.0**-90, 2.0**-60)), (torch.bfloat16, (2.0**-53, 2.0**-66, 1.0)), (torch.bfloat16, (2.0**60, 2.0**-100, 1.0)),
+    (torch.bfloat16, (2.0**40, 2.0**-90, 2.0**-60))], ids=str)
+def test_gradients_of_any_magnitude(device, dtype, sizes, reduction):
+    """Hidden rows, the upstream gradient and the scale times powers of two (the weights take the inverse, so that the logits stay): the gradients are
+    those of the plain call times powers of two, bit for bit, as long as all of them are ordinary numbers of the type."""
+    size, up, scale = sizes
+    h, w, t = _inputs(40, 33, 24, dtype, device)
+    base = torch.rand(40, generator=torch.Generator().manual_seed(3)).to(device) if reduction == 'none' else torch.tensor(0.75, device=device)
+
+    def grads(h, w, upstream, scale):
+        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+        return torch.autograd.grad(ops.linear_cross_entropy(h, w, t, scale=scale, reduction=reduction), (h, w), upstream)
+    want = grads(h, w, base, 1.0)
+    got = grads(h * size, w / (size * scale), base * up, scale)
+    for x, y, factor in zip(got, want, (up / size, up * scale * size)):
+        exact = y.double() * factor
+        ordinary = (exact.abs() >= torch.finfo(dtype).smallest_normal) | (exact == 0)
+        assert bool(ordinary.any()) and float(exact.abs().max()) <= torch.finfo(dtype).max
+        assert torch.equal(x.double()[ordinary], exact[ordinary])
+        assert bool(((x.double() - exact).abs() <= torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all())

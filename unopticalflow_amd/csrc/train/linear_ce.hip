@@ -418,8 +418,21 @@ __global__ __launch_bounds__(256) void lce_magnitudes_kernel(Operand h, Operand 
 // The upstream gradient: one number for a reduced loss, one per row for reduction none (these relative to the largest, so that fp16 planes hold
 // them).
 struct Upstream { const float* g; const float* largest; const float* count; const long long* target; long long ignore; int reduction; float scale; };
-__device__ __forceinline__ float uniform_factor(const Upstream& u) {
-    return u.reduction == 0 ? u.scale : u.reduction == 1 ? u.scale * u.g[0] / u.count[0] : u.scale * u.g[0];
+// m 2^e, |m| in [1/2, 1) of a number, and the product of such: factors of a gradient may each be far from 1 (a power of two that an operand was scaled
+// by, a small upstream gradient), and only what they make of the sums has to fit the type
+struct Factor { float m; int e; };
+__device__ __forceinline__ Factor factor_of(float v) {
+    int e = 0;
+    const float m = frexpf(v, &e);
+    return fabsf(v) <= 3.4028235e38f ? Factor{m, e} : Factor{v, 0};
+}
+__device__ __forceinline__ Factor operator*(Factor a, Factor b) { return Factor{a.m * b.m, a.e + b.e}; }
+__device__ __forceinline__ f32x4 operator*(f32x4 v, Factor f) { return scaled(v * f.m, f.e); }
+__device__ __forceinline__ Factor uniform_factor(const Upstream& u) {
+    Factor f = factor_of(u.scale);
+    if (u.reduction != 0) f = f * factor_of(u.g[0]);
+    if (u.reduction == 1) f.m /= u.count[0];
+    return f;
 }
 __device__ __forceinline__ float row_factor(const Upstream& u, int m) { return u.target[m] == u.ignore ? 0.f : u.reduction == 0 ? u.g[m] : 1.f; }
 
@@ -528,10 +541,12 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
 struct Product { Operand A, B; int width, shares, tiles; float* sums; long long ldc; int first; void* out; int by_h; };
 
 // what turns a job's sums into gradients: the uniform factor, and the row's own (dH; for dW it is in GT, relative to the largest)
-template <class T> __device__ __forceinline__ float product_factor(const Exponents* ex, const Upstream& up, int by_h) {
-    float f = uniform_factor(up) * (by_h && up.reduction == 0 ? up.largest[0] : 1.f);
-    if constexpr (kScaled<T>) f = ldexpf(f, -(by_h ? ex->h : ex->w));
-    return ldexpf(f, -kProbabilityExponent);
+template <class T> __device__ __forceinline__ Factor product_factor(const Exponents* ex, const Upstream& up, int by_h) {
+    Factor f = uniform_factor(up);
+    if (by_h && up.reduction == 0) f = f * factor_of(up.largest[0]);
+    if constexpr (kScaled<T>) f.e -= by_h ? ex->h : ex->w;
+    f.e -= kProbabilityExponent;
+    return f;
 }
 
 template <class T_, class TileT>
@@ -575,12 +590,12 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product
         }
         return;
     }
-    const float f = product_factor<T_>(ex, up, p.by_h);
+    const Factor f = product_factor<T_>(ex, up, p.by_h);
 #pragma unroll
     for (int i = 0; i < TileT::MI; ++i) {
         const int m = m0 + TileT::row(i);
         if (m >= p.A.rows) continue;
-        const float fm = p.by_h ? f : f * row_factor(up, m);
+        const Factor fm = p.by_h ? f : f * factor_of(row_factor(up, m));
 #pragma unroll
         for (int j = 0; j < TileT::NI; ++j) {
             const int n = n0 + TileT::col(j), left = p.B.rows - n;
@@ -596,7 +611,7 @@ __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, i
     const bool second = (int)blockIdx.x >= blocks_a;
     const Product p = second ? b : a;
     const int block = (int)blockIdx.x - (second ? blocks_a : 0), blocks = second ? (int)gridDim.x - blocks_a : blocks_a;
-    const float f = product_factor<T_>(ex, up, p.by_h);
+    const Factor f = product_factor<T_>(ex, up, p.by_h);
     const int rows = p.A.rows, cols = p.B.rows;
     const long long per = p.ldc / 4, total = per * rows;
     for (long long g = block * 256ll + threadIdx.x; g < total; g += blocks * 256ll) {
@@ -604,8 +619,7 @@ __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, i
         const int n = (int)(g - r * per) * 4;
         f32x4 v = *reinterpret_cast<const f32x4*>(p.sums + r * p.ldc + n);
         for (int s = 1; s < p.shares; ++s) v += *reinterpret_cast<const f32x4*>(p.sums + ((long long)s * rows + r) * p.ldc + n);
-        v *= p.by_h ? f : f * row_factor(up, (int)r);
-        store4<T_>((T_*)p.out + r * cols + n, v, cols - n < 4 ? cols - n : 4);
+        store4<T_>((T_*)p.out + r * cols + n, v * (p.by_h ? f : f * factor_of(row_factor(up, (int)r))), cols - n < 4 ? cols - n : 4);
     }
 }
 
