@@ -241,3 +241,31 @@ def test_gradients_of_any_magnitude(device, dtype, sizes, reduction):
         assert bool(ordinary.any()) and float(exact.abs().max()) <= torch.finfo(dtype).max
         assert torch.equal(x.double()[ordinary], exact[ordinary])
         assert bool(((x.double() - exact).abs() <= torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all())
+
+
+# ------------------------------------------------------------------------------------------ FlowMuon
+def _parameter(*shape, seed=0, dtype=torch.float32, device='cpu'):
+    p = torch.nn.Parameter(torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(device))
+    p.grad = torch.ones_like(p) * 0.5
+    return p
+
+
+def test_a_group_given_as_a_generator(device):
+    """module.parameters() is a generator: its weights are in the group, and they train."""
+    first, second = _parameter(3, 4, device=device), _parameter(5, 4, seed=1, device=device)
+    opt = optim.FlowMuon([first], lr=0.1)
+    group = {'params': (p for p in [second]), 'lr': 0.2}
+    opt.add_param_group(group)
+    assert [len(g['params']) for g in opt.param_groups] == [1, 1] and 'kind' not in group
+    alone = _parameter(6, 4, seed=2, device=device)
+    opt.add_param_group({'params': alone})
+    before = [p.detach().clone() for p in (first, second, alone)]
+    opt.step()
+    assert not any(torch.equal(p, old) for p, old in zip((first, second, alone), before))
+    with pytest.raises(ValueError):
+        opt.add_param_group({'params': (p for p in [_parameter(4, device=device)])})
+
+
+def test_sets_have_no_order():
+    with pytest.raises(TypeError):
+        optim.FlowMuon([_parameter(3, 4)]).add_param_group({'params': {_parameter(3, 4, seed=1)}})

@@ -230,8 +230,12 @@ class FlowMuon(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         """Further groups hold matrices."""
+        group = dict(group)
+        params = group['params']
+        if not isinstance(params, set):                                  # (which torch refuses: it has no order)
+            group['params'] = [params] if torch.is_tensor(params) else list(params)                          # (it may be a generator)
         group.setdefault('kind', 'matrices')
-        if group['kind'] == 'matrices' and any(p.dim() < 2 for p in ([group['params']] if torch.is_tensor(group['params']) else group['params'])):
+        if group['kind'] == 'matrices' and any(p.dim() < 2 for p in group['params'] if torch.is_tensor(p)):
             raise ValueError('FlowMuon: a further parameter group holds weights of two or more dimensions')
         super().add_param_group(group)
 
