@@ -269,3 +269,13 @@ def test_a_group_given_as_a_generator(device):
 def test_sets_have_no_order():
     with pytest.raises(TypeError):
         optim.FlowMuon([_parameter(3, 4)]).add_param_group({'params': {_parameter(3, 4, seed=1)}})
+
+
+@pytest.mark.parametrize('kind', ['others', 'anything'])
+def test_a_further_group_holds_matrices(kind):
+    """Adam's parameters are those of the constructor: a group that no step would reach is refused, and nothing is added."""
+    opt = optim.FlowMuon([_parameter(3, 4), _parameter(4, seed=1)])
+    for p in (_parameter(4, seed=2), _parameter(4, 4, seed=2)):
+        with pytest.raises(ValueError, match='kind'):
+            opt.add_param_group({'params': [p], 'kind': kind})
+    assert [len(g['params']) for g in opt.param_groups] == [1, 1]

@@ -235,6 +235,8 @@ class FlowMuon(torch.optim.Optimizer):
         if not isinstance(params, set):                                  # (which torch refuses: it has no order)
             group['params'] = [params] if torch.is_tensor(params) else list(params)                          # (it may be a generator)
         group.setdefault('kind', 'matrices')
+        if group['kind'] != 'matrices' and hasattr(self, '_adam'):       # (the constructor's own group of others comes before)
+            raise ValueError("FlowMuon: a further parameter group is of kind 'matrices', got %r" % (group['kind'],))
         if group['kind'] == 'matrices' and any(p.dim() < 2 for p in group['params'] if torch.is_tensor(p)):
             raise ValueError('FlowMuon: a further parameter group holds weights of two or more dimensions')
         super().add_param_group(group)
