@@ -279,3 +279,42 @@ def test_a_further_group_holds_matrices(kind):
         with pytest.raises(ValueError, match='kind'):
             opt.add_param_group({'params': [p], 'kind': kind})
     assert [len(g['params']) for g in opt.param_groups] == [1, 1]
+
+
+def test_checkpoints_of_another_optimiser_are_refused_whole(device):
+    """An Adam state of the same groups, a momentum of another shape, moments that are missing: an error, and the optimiser is as it was."""
+    def fresh(seed=0):
+        ps = [_parameter(3, 4, seed=seed, device=device), _parameter(5, 2, seed=seed + 1, device=device), _parameter(4, seed=seed + 2, device=device)]
+        return ps, optim.FlowMuon(ps, lr=0.1)
+    only, narrow = [_parameter(3, 4, device=device), _parameter(5, 2, seed=1, device=device)], None
+    narrow = optim.FlowMuon(only, lr=0.1)
+    adam = torch.optim.Adam([p for p in only], lr=0.1)
+    adam.step()
+    narrow.step()
+    kept = {k: v.clone() for p in only for k, v in ((p, narrow.state[p]['momentum_buffer']),)}
+    with pytest.raises(ValueError):
+        narrow.load_state_dict(adam.state_dict())
+    assert narrow.param_groups[0]['kind'] == 'matrices' and all(torch.equal(narrow.state[p]['momentum_buffer'], m) for p, m in kept.items())
+    narrow.step()
+    if device == 'cuda':                                 # (the biases' Adam runs on the device only)
+        params, opt = fresh()
+        opt.step()
+        good = opt.state_dict()
+        for where, key, value in ((0, 'momentum_buffer', torch.zeros(4, 3, device=device)), (0, 'momentum_buffer', None), (1, 'momentum_buffer', torch.zeros(1, 1, device=device)),
+                                  (2, 'exp_avg', None), (2, 'exp_avg_sq', None), (2, 'step', None), (2, 'exp_avg', torch.zeros(3, device=device))):
+            state = {i: dict(s) for i, s in good['state'].items()}
+            state[where].pop(key)
+            if value is not None:
+                state[where][key] = value
+            with pytest.raises(ValueError):
+                opt.load_state_dict({'state': state, 'param_groups': good['param_groups']})
+        opt.step()
+        opt.load_state_dict(good)
+        opt.step()
+    state = narrow.state_dict()
+    for wrong in (torch.zeros(4, 3), torch.zeros(1, 4), None, 3.0):
+        with pytest.raises(ValueError):
+            narrow.load_state_dict({'state': {0: {'momentum_buffer': wrong}, 1: state['state'][1]}, 'param_groups': state['param_groups']})
+    narrow.load_state_dict({'state': {}, 'param_groups': state['param_groups']})         # (a run that has not stepped)
+    narrow.step()
+    assert all(bool(torch.isfinite(p).all()) for p in only)

@@ -249,14 +249,29 @@ class FlowMuon(torch.optim.Optimizer):
         if self._adam is not None:
             self._adam.state = self.state
 
+    def _check_state(self, state_dict):
+        """Refuses, before anything is replaced, a state that is not one of these parameters' and groups'."""
+        groups = state_dict['param_groups']
+        if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
+            return                                       # (Optimizer.load_state_dict says so)
+        for given, own in zip(groups, self.param_groups):
+            if given.get('kind') != own['kind']:
+                raise ValueError("FlowMuon: a state whose parameter group is of kind %r, not %r" % (given.get('kind'), own['kind']))
+            for i, p in zip(given['params'], own['params']):
+                st = state_dict['state'].get(i)
+                for key in () if not st else ('momentum_buffer',) if own['kind'] == 'matrices' else ('exp_avg', 'exp_avg_sq', 'step'):
+                    v = st.get(key)
+                    if v is None or (key != 'step' and (not torch.is_tensor(v) or v.shape != p.shape)):
+                        raise ValueError('FlowMuon: a state without a %s for a parameter of shape %s' % (key, tuple(p.shape)))
+
     def load_state_dict(self, state_dict):
+        self._check_state(state_dict)
         super().load_state_dict(state_dict)
         # (Optimizer.load_state_dict has cast the momentum to the parameter's type: taken again from what was given)
-        given = [i for g in state_dict['param_groups'] for i in g['params']]
-        kept = [p for g in self.param_groups for p in g['params']]
-        for i, p in zip(given, kept):
-            if p.dim() >= 2 and p in self.state:
-                self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(state_dict['state'][i]['momentum_buffer'])
+        for given, own in zip(state_dict['param_groups'], self.param_groups):
+            for i, p in zip(given['params'], own['params']):
+                if own['kind'] == 'matrices' and state_dict['state'].get(i):
+                    self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(state_dict['state'][i]['momentum_buffer'])
         self._share()
         if self._adam is not None:
             self._adam._tables = None
