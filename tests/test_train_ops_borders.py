@@ -318,3 +318,30 @@ def test_checkpoints_of_another_optimiser_are_refused_whole(device):
     narrow.load_state_dict({'state': {}, 'param_groups': state['param_groups']})         # (a run that has not stepped)
     narrow.step()
     assert all(bool(torch.isfinite(p).all()) for p in only)
+
+
+def test_matrices_of_several_types_in_one_group(device):
+    """Every type has a call of its own; the weights move as they do alone."""
+    shapes, dtypes = [(12, 20), (40, 8), (9, 70), (33, 34)], [torch.float32, torch.bfloat16, torch.float16, torch.bfloat16]
+    params = [_parameter(*s, seed=i, dtype=t, device=device) for i, (s, t) in enumerate(zip(shapes, dtypes))]
+    for i, p in enumerate(params):
+        p.grad = _matrix(*p.shape, dtype=p.dtype, device=device, seed=10 + i)
+    before = [p.detach().clone() for p in params]
+    optim.FlowMuon(params, lr=0.1).step()
+    for t in set(dtypes):
+        chosen = [i for i, d in enumerate(dtypes) if d == t]
+        want = [before[i].clone() for i in chosen]
+        optim.muon_step_(want, [params[i].grad for i in chosen], [torch.zeros_like(w, dtype=torch.float32) for w in want], lr=0.1)
+        assert all(torch.equal(params[i], w) for i, w in zip(chosen, want))
+
+
+def test_weights_that_no_step_takes_are_refused_at_once():
+    """Types and sides that muon_step_ refuses: the optimiser is not made, and no group is added."""
+    good = _parameter(3, 4)
+    opt = optim.FlowMuon([good])
+    for bad in (_parameter(3, 4, dtype=torch.float64), torch.nn.Parameter(torch.zeros(1, (1 << 18) + 1)), torch.nn.Parameter(torch.zeros(3, 4, dtype=torch.complex64))):
+        with pytest.raises((TypeError, ValueError)):
+            optim.FlowMuon([good, bad])
+        with pytest.raises((TypeError, ValueError)):
+            opt.add_param_group({'params': [bad]})
+    assert len(opt.param_groups) == 1

@@ -214,7 +214,8 @@ class FlowMuon(torch.optim.Optimizer):
     """Muon for the weights of two or more dimensions (``muon_step_``), Adam (``FlowAdam``) for everything else.
 
     ``params`` is a list of parameters; it becomes two groups: 'matrices' (``lr``, ``momentum``, ``nesterov``, ``weight_decay``) and 'others'
-    (``adam_lr`` as their ``lr``; betas and eps are FlowAdam's own).  Momentum is kept in fp32 whatever the parameters' type.  Like FlowAdam it can be captured into a hipGraph once ``prepare()`` has created its state."""
+    (``adam_lr`` as their ``lr``; betas and eps are FlowAdam's own).  Further groups (``add_param_group``) hold matrices.  Weights may be of
+    different types (fp32, bf16, fp16): each type is a call of its own.  Momentum is kept in fp32 whatever the parameters' type.  Like FlowAdam it can be captured into a hipGraph once ``prepare()`` has created its state."""
 
     def __init__(self, params, lr=0.02, adam_lr=1e-4, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
         params = [p for p in params]
@@ -239,6 +240,11 @@ class FlowMuon(torch.optim.Optimizer):
             raise ValueError("FlowMuon: a further parameter group is of kind 'matrices', got %r" % (group['kind'],))
         if group['kind'] == 'matrices' and any(p.dim() < 2 for p in group['params'] if torch.is_tensor(p)):
             raise ValueError('FlowMuon: a further parameter group holds weights of two or more dimensions')
+        for p in [p for p in group['params'] if torch.is_tensor(p) and p.requires_grad and group['kind'] == 'matrices']:
+            if p.dtype not in ops._DTYPES:
+                raise TypeError('FlowMuon takes fp32, bf16 or fp16 weights; got %s' % p.dtype)
+            if p.numel() and max(p.shape[0], p.numel() // p.shape[0]) > ops._MATRIX_MAX_SIDE:
+                raise ValueError('FlowMuon: weights are matrices [shape[0], the rest] of sides up to {}; got shape {}'.format(ops._MATRIX_MAX_SIDE, tuple(p.shape)))
         super().add_param_group(group)
 
     def _matrices(self):
@@ -299,9 +305,13 @@ class FlowMuon(torch.optim.Optimizer):
         for g in self.param_groups:
             if g['kind'] != 'matrices':
                 continue
-            params = [p for p in g['params'] if p.grad is not None]
-            muon_step_(params, [p.grad for p in params], [self._momentum(p) for p in params], lr=g['lr'], momentum=g['momentum'], weight_decay=g['weight_decay'],
-                       nesterov=g['nesterov'], steps=g['steps'], coefficients=g['coefficients'], eps=g['eps'])
+            alike = {}                                   # (a call takes weights of one type, on one device)
+            for p in g['params']:
+                if p.grad is not None:
+                    alike.setdefault((p.dtype, p.device), []).append(p)
+            for params in alike.values():
+                muon_step_(params, [p.grad for p in params], [self._momentum(p) for p in params], lr=g['lr'], momentum=g['momentum'], weight_decay=g['weight_decay'],
+                           nesterov=g['nesterov'], steps=g['steps'], coefficients=g['coefficients'], eps=g['eps'])
         if self._adam is not None:
             self._adam.param_groups[0]['lr'] = next(g['lr'] for g in self.param_groups if g['kind'] == 'others')
             self._adam.step()
