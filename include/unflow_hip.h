@@ -456,7 +456,8 @@ int unflow_linear_ce_bwd_ex(const void* hidden, long long ldh, const void* weigh
  * and out = X (unflow_orthogonalize), or with momentum as the optimiser step (unflow_muon_step; x = gradient, out = parameter)
  *   momentum += (1 - mu)(x - momentum);  u = nesterov ? x + mu (momentum - x) : momentum
  *   out = out (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X(u)
- * Matrices are dense row-major [rows, cols]; momentum is fp32 whatever the type.  Coefficients whose polynomial leaves [0, 16] are refused.
+ * Matrices are dense row-major [rows, cols]; momentum is fp32 whatever the type.  Parameters and momenta that share memory with one another, or with
+ * another weight's gradient, are refused.  Coefficients whose polynomial leaves [0, 16] are refused.
  * unflow_orthogonalize_workspace_ex() says what a call with these steps and coefficients needs, unflow_orthogonalize_workspace() what is enough for
  * any (lists of matrices of up to 32 rows or columns need much less for a few steps than for many). */
 #define UNFLOW_MATRIX_MAX_SIDE (1 << 18)

@@ -345,3 +345,64 @@ def test_weights_that_no_step_takes_are_refused_at_once():
         with pytest.raises((TypeError, ValueError)):
             opt.add_param_group({'params': [bad]})
     assert len(opt.param_groups) == 1
+
+
+# ------------------------------------------------------------------------------------------ muon_step_: what it writes
+def _views(device, offsets, shape=(5, 8), size=200):
+    buffer = torch.randn(size, generator=torch.Generator().manual_seed(4)).to(device)
+    return buffer, [buffer[o:o + shape[0] * shape[1]].view(shape) for o in offsets]
+
+
+def test_weights_that_share_memory_are_refused():
+    """Overlapping views of one buffer as momenta, as parameters, as a parameter and a momentum, and a gradient within what another weight writes."""
+    import train_on_host
+    with train_on_host.patched():
+        new = lambda: torch.ones(5, 8)  # noqa: E731
+        for offsets in ((0, 20), (20, 0), (0, 39), (0, 0)):
+            buffer, (a, b) = _views('cpu', offsets)
+            kept = buffer.clone()
+            ps, gs, ms = [new(), new()], [new(), new()], [new(), new()]
+            for params, grads, momenta in ((ps, gs, [a, b]), ([a, b], gs, ms), ([a, ps[0]], gs, [ms[0], b]), (ps, [a, gs[0]], [ms[0], b]), ([ps[0], b], [a, gs[0]], ms)):
+                with pytest.raises(ValueError):
+                    optim.muon_step_(params, grads, momenta, lr=0.1)
+            assert torch.equal(buffer, kept) and all(torch.equal(x, new()) for x in ps + gs + ms)
+        buffer, (a, b) = _views('cpu', (0, 20))          # (a weight's own gradient is its momentum, and another's lies across it)
+        with pytest.raises(ValueError):
+            optim.muon_step_([new(), new()], [b, a], [b, new()], lr=0.1)
+        half = torch.ones(200, dtype=torch.bfloat16)
+        with pytest.raises(ValueError):                  # (weights of 2 bytes a number: 0 .. 79 and 78 .. 157)
+            optim.muon_step_([half[:40].view(5, 8), half[39:79].view(5, 8)], [new().bfloat16()] * 2, [new(), new()], lr=0.1)
+
+
+def test_neighbours_in_one_buffer_are_fine(device):
+    """Views that touch but do not overlap, one gradient for two weights, a weight's own gradient in its momentum."""
+    buffer, (a, b) = _views(device, (0, 40))
+    other, (ma, mb) = _views(device, (40, 0))
+    g = _matrix(5, 8, dtype=torch.float32, device=device)
+    want = [a.clone(), b.clone()], [ma.clone(), mb.clone()]
+    optim.muon_step_(want[0], [g, g.clone()], want[1], lr=0.1)
+    optim.muon_step_([a, b], [g, g], [ma, mb], lr=0.1)
+    assert all(torch.equal(x, y) for x, y in zip([a, b, ma, mb], want[0] + want[1]))
+    m = g.clone()
+    p, q = torch.ones(5, 8, device=device), torch.ones(5, 8, device=device)
+    optim.muon_step_([p], [m], [m], lr=0.1)
+    optim.muon_step_([q], [g], [g.clone()], lr=0.1)
+    assert torch.equal(p, q) and torch.equal(m, g)
+
+
+def test_the_entry_point_refuses_shared_memory():
+    """The C entry over the host-executed kernels, and the library itself, which returns before any launch."""
+    import __graft_entry__ as ge
+    ge.build()
+    from unopticalflow_amd import _lib
+    import train_on_host
+    with train_on_host.patched() as lib:
+        x = torch.zeros(1000)
+        base, ws = x.data_ptr(), torch.zeros(1 << 20, dtype=torch.uint8)
+        call = lambda *m: lib.unflow_muon_step((ops._Matrix * len(m))(*m), len(m), 0, 0.1, 0.9, 0.0, 1, 5, 3.4445, -4.7750, 2.0315, 1e-7, ws.data_ptr(), ws.numel(), None)  # noqa: E731
+        at = lambda *k: tuple(base + 4 * 40 * i for i in k) + (5, 8)  # noqa: E731
+        assert call(at(0, 1, 2), at(3, 4, 5)) == 0 and call(at(0, 1, 2), at(0, 4, 5)) == 0 and call(at(2, 1, 2)) == 0 and call(at(1, 1, 2)) == 0
+        for bad in ((at(0, 1, 2), at(3, 1, 5)), (at(0, 1, 2), at(3, 2, 5)), (at(0, 1, 1),), (at(0, 1, 2), at(1, 4, 5)), (at(0, 1, 2), at(2, 4, 5)),
+                    (at(0, 1, 2), at(2.5, 4, 5)), (at(2, 1, 2), at(1.5, 4, 5))):
+            assert call(*[tuple(int(v) for v in m) for m in bad]) == -22
+    assert _lib.load().unflow_muon_step((ops._Matrix * 1)((4096, 8192, 8192, 5, 7)), 1, 0, 0.1, 0.9, 0.0, 1, 5, 3.4445, -4.7750, 2.0315, 1e-7, 4096, 1 << 30, None) == -22

@@ -19,6 +19,7 @@
 #include "plan.h"
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 
 namespace {
@@ -804,6 +805,32 @@ static bool matrices_ok(const unflow_matrix* a, int count, int dtype) {
     return true;
 }
 
+// Whether no parameter or momentum shares memory with another one, or with another weight's gradient: the kernels work on all of them at once.  (A
+// weight's own gradient may be its momentum or its parameter: whoever writes a number has read it.)  false, too, without memory for the list.
+static bool apart(const unflow_matrix* a, int count, int dtype) {
+    struct Span { size_t from, to; bool written; };
+    const size_t size = dtype == kFp32 ? 4 : 2;
+    Span* spans = (Span*)malloc(sizeof(Span) * 3 * (size_t)count);
+    if (!spans) return false;
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+        const size_t numbers = (size_t)a[i].rows * (size_t)a[i].cols, g = (size_t)a[i].x, p = (size_t)a[i].out, m = (size_t)a[i].momentum;
+        spans[n++] = Span{p, p + numbers * size, true};
+        spans[n++] = Span{m, m + numbers * 4, true};
+        if (g != p && (g != m || size != 4)) spans[n++] = Span{g, g + numbers * size, false};
+    }
+    std::sort(spans, spans + n, [](const Span& x, const Span& y) { return x.from < y.from; });
+    size_t written = 0, read = 0;                                        // bytes behind what lies before
+    bool good = true;
+    for (int i = 0; i < n && good; ++i) {
+        good = spans[i].from >= written && !(spans[i].written && spans[i].from < read);
+        size_t& reach = spans[i].written ? written : read;
+        reach = reach > spans[i].to ? reach : spans[i].to;
+    }
+    free(spans);
+    return good;
+}
+
 #define LAUNCH_TILES(kernel, count, ...)                                                                                              \
     do {                                                                                                                              \
         if (TileT::LDS > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS); \
@@ -919,6 +946,7 @@ extern "C" int unflow_muon_step(const unflow_matrix* matrices, int count, int dt
         void* workspace, long long workspace_bytes, void* stream) {
     UNFLOW_REQUIRE(matrices_ok(matrices, count, dtype) && workspace && steps >= 1 && steps <= 64 && eps >= 0.f);
     for (int i = 0; i < count; ++i) UNFLOW_REQUIRE(matrices[i].x && matrices[i].out && matrices[i].momentum);
+    UNFLOW_REQUIRE(apart(matrices, count, dtype));
     return run<true>(matrices, count, dtype, steps, a, b, c, eps, momentum, nesterov, Update{1.f - lr * weight_decay, lr}, workspace,
         workspace_bytes, stream);
 }

@@ -166,6 +166,29 @@ def _other_strides(a, b):
     return any(x != y and n > 1 for x, y, n in zip(a.stride(), b.stride(), b.shape))
 
 
+def _check_apart(items, size):
+    """Refuses weights whose parameters or momenta share memory with one another, or with another weight's gradient: the kernels work on all of them
+    at once.  (A weight's own gradient may be its momentum or its parameter: whoever writes a number has read it.)  The library refuses the
+    same, without a reason."""
+    spans = []                                           # (first byte, byte behind the last, is written)
+    for g, p, m, rows, cols in items:
+        n = rows * cols
+        spans += [(p, p + n * size, True), (m, m + 4 * n, True)]
+        if g != p and (g != m or size != 4):
+            spans.append((g, g + n * size, False))
+    spans.sort()
+    written = read = 0                                   # bytes behind what lies before
+    for start, end, writes in spans:
+        if start < written:
+            raise ValueError('muon_step_: a parameter or momentum appears twice, or shares memory with another tensor of the step')
+        if not writes:
+            read = max(read, end)
+        elif start < read:
+            raise ValueError('muon_step_: a gradient shares memory with a parameter or momentum')
+        else:
+            written = end
+
+
 @torch.no_grad()
 def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nesterov=True, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     """One Muon step over a list of weights, in place: every weight is a matrix [shape[0], the rest] (csrc/train/muon.hip, one launch per phase
@@ -175,7 +198,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
         p  = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u)
 
     ``params`` and ``grads`` are fp32, bf16 or fp16 (one type), ``momenta`` fp32 in their parameters' layout (row-major or channels_last;
-    a gradient in another layout is copied).  No weight may appear twice."""
+    a gradient in another layout is copied).  No weight may appear twice, nor share memory with another."""
     ops._refuse_tracers('muon_step_')
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
@@ -204,10 +227,12 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
             g = torch.empty_like(p).copy_(g)
             copied.append(g)
         items.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), rows, cols))
-    if len({x[1] for x in items} | {x[2] for x in items}) < 2 * len(items):
-        raise ValueError('muon_step_: a parameter or momentum appears twice')
-    ops._newton_schulz('unflow_muon_step', dev, dtype, (ops._Matrix * len(items))(*items), len(items),
-                       (float(lr), float(momentum), float(weight_decay), int(bool(nesterov))), steps, coefficients, eps)
+    try:
+        ops._newton_schulz('unflow_muon_step', dev, dtype, (ops._Matrix * len(items))(*items), len(items),
+                           (float(lr), float(momentum), float(weight_decay), int(bool(nesterov))), steps, coefficients, eps)
+    except RuntimeError:
+        _check_apart(items, params[0].element_size())
+        raise
 
 
 class FlowMuon(torch.optim.Optimizer):
