@@ -406,3 +406,23 @@ def test_the_entry_point_refuses_shared_memory():
                     (at(0, 1, 2), at(2.5, 4, 5)), (at(2, 1, 2), at(1.5, 4, 5))):
             assert call(*[tuple(int(v) for v in m) for m in bad]) == -22
     assert _lib.load().unflow_muon_step((ops._Matrix * 1)((4096, 8192, 8192, 5, 7)), 1, 0, 0.1, 0.9, 0.0, 1, 5, 3.4445, -4.7750, 2.0315, 1e-7, 4096, 1 << 30, None) == -22
+
+
+def test_autograd_sees_what_a_step_writes(device):
+    """A graph from before the step needs the old weight: its backward pass is an error, as behind torch's own optimisers."""
+    w, x = _parameter(12, 20, device=device), torch.ones(3, 20, device=device)
+    m = torch.zeros(12, 20, device=device)
+    x.requires_grad_()
+    loss = (x @ w.T).sum()
+    versions = w._version, m._version
+    optim.muon_step_([w], [w.grad], [m], lr=0.1)
+    assert w._version > versions[0] and m._version > versions[1]
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    opt = optim.FlowMuon([w], lr=0.1)
+    opt.step()
+    loss = (x @ w.T).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    (x @ w.T).sum().backward()                           # (a graph from behind the step is fine)

@@ -233,6 +233,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
     except RuntimeError:
         _check_apart(items, params[0].element_size())
         raise
+    torch.autograd.graph.increment_version(params + momenta)             # (written through their addresses, which autograd does not see)
 
 
 class FlowMuon(torch.optim.Optimizer):
