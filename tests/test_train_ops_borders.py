@@ -1,5 +1,6 @@
 """The training operators at the borders of what a caller may do: saved tensors that come back in another layout, other kinds of derivatives, many steps,
 optimiser groups and checkpoints.  References in 64 bits; the bounds are those of test_train_ops.py unless a test derives its own."""
+import contextlib
 import os
 import sys
 
@@ -426,3 +427,31 @@ def test_autograd_sees_what_a_step_writes(device):
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         loss.backward()
     (x @ w.T).sum().backward()                           # (a graph from behind the step is fine)
+
+
+@contextlib.contextmanager
+def _adam_on(where):
+    """FlowAdam's kernel: on the device, or host-executed."""
+    if where == 'cuda':
+        yield
+        return
+    import hostexec
+    with hostexec.patched(ops):
+        yield
+
+
+@pytest.mark.parametrize('where', ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)])
+def test_autograd_sees_what_adam_writes(where):
+    """FlowAdam's one launch counts as a write of the weights and moments, as torch.optim.Adam's does."""
+    with _adam_on(where):
+        w, x = _parameter(12, 20, device=where), torch.ones(3, 20, device=where, requires_grad=True)
+        opt = optim.FlowAdam([w], lr=0.1)
+        opt.step()
+        versions = w._version, opt.state[w]['exp_avg']._version, opt.state[w]['exp_avg_sq']._version
+        loss = (x @ w.T).sum()
+        opt.step()
+        assert opt.native_steps == 2
+        assert all(a < b for a, b in zip(versions, (w._version, opt.state[w]['exp_avg']._version, opt.state[w]['exp_avg_sq']._version)))
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            loss.backward()
+        (x @ w.T).sum().backward()

@@ -152,6 +152,8 @@ class FlowAdam(torch.optim.Adam):
                                        ctypes.c_float(g['lr']), ctypes.c_float(g['betas'][0]), ctypes.c_float(g['betas'][1]),
                                        ctypes.c_float(g['eps']), ops._stream())
         _lib.check(rc, 'unflow_adam_multi')
+        # (written through their addresses, which autograd does not see)
+        torch.autograd.graph.increment_version(params + [self.state[p][k] for p in params for k in ('exp_avg', 'exp_avg_sq')])
         self.native_steps += 1
         return None
 
