@@ -11,7 +11,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, 'tests'))
 
 from unopticalflow_amd import ops, optim  # noqa: E402
-from test_train_ops import DTYPES, _check_orthogonal, _inputs, _matrix, device  # noqa: E402,F401
+from test_train_ops import DTYPES, _check_orthogonal, _inputs, _matrix, _muon, device  # noqa: E402,F401
 
 
 # ------------------------------------------------------------------------------------------ linear_cross_entropy under saved-tensor hooks
@@ -307,6 +307,8 @@ def test_checkpoints_of_another_optimiser_are_refused_whole(device):
             state[where].pop(key)
             if value is not None:
                 state[where][key] = value
+            else:                                        # (nothing at all is the state of a weight that has not stepped)
+                state[where]['other'] = 1.0
             with pytest.raises(ValueError):
                 opt.load_state_dict({'state': state, 'param_groups': good['param_groups']})
         opt.step()
@@ -455,3 +457,180 @@ def test_autograd_sees_what_adam_writes(where):
         with pytest.raises(RuntimeError, match='modified by an inplace operation'):
             loss.backward()
         (x @ w.T).sum().backward()
+
+
+# ------------------------------------------------------------------------------------------ lists, ranks and commands
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_lists_of_more_than_a_wave_of_matrices(device, dtype):
+    """140 matrices of sides 3 to 130, of more than 32 rows among them: past 64 a launch searches its table in several goes."""
+    g = torch.Generator().manual_seed(0)
+    sides = torch.randint(3, 131, (140, 2), generator=g).tolist()
+    assert sum(min(s) > 32 for s in sides) > 64
+    xs = [_matrix(*s, dtype=dtype, device=device, seed=i) for i, s in enumerate(sides)]
+    for x, y in zip(xs, ops.orthogonalize(xs)):
+        _check_orthogonal(y, x)
+
+
+class _Net(torch.nn.Module):
+    """What FlowTrainer takes for a model, with a convolution, a projection and biases."""
+
+    def __init__(self):
+        super().__init__()
+        self.conv = torch.nn.Conv2d(3, 36, 3)
+        self.proj = torch.nn.Linear(36, 5)
+
+    def forward(self, x):
+        y = self.proj(torch.tanh(self.conv(x)).mean((2, 3)))
+        return {'loss_pixel': y[:, 0].square(), 'loss_ssim': y[:, 1].square() + y[:, 4].exp(), 'loss_flow_smooth': y[:, 2].square(), 'loss_flow_consis': y[:, 3].square()}
+
+
+class _Either:
+    """Two libraries that each hold a part of the entry points."""
+
+    def __init__(self, *libs):
+        self.libs = libs
+
+    def __getattr__(self, name):
+        return getattr(next(lib for lib in self.libs if hasattr(lib, name)), name)
+
+
+def _muon_rank(rank, world, port, flat, out_path):
+    """One of two ranks of FlowTrainer(optimizer='muon') over gloo and the host-executed kernels: the eager step with its pieces sent from hooks, or
+    (flat) the exchange of the replayed step without its graphs."""
+    import hostexec
+    import train_on_host
+    import torch.distributed as dist
+    from oracle import ref_cpu as R
+    from unopticalflow_amd import _lib
+    from unopticalflow_amd.parallel import init_distributed, shard_batch
+    from unopticalflow_amd.trainer import FlowTrainer
+    os.environ.update(RANK=str(rank), LOCAL_RANK=str(rank), WORLD_SIZE=str(world), MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port))
+    torch.set_num_threads(2)
+    init_distributed('gloo')
+    with hostexec.patched(ops) as lib, train_on_host.patched() as train:
+        _lib._lib = _Either(lib, train)
+        torch.manual_seed(rank)                          # (rank 0's weights win)
+        model = _Net()
+        trainer = FlowTrainer(R.default_cfg(), model, distributed=True, use_graph=flat, optimizer='muon', muon_lr=0.05, defer_bias_grads=False)
+        assert type(trainer.optimizer) is optim.FlowMuon and trainer.optimizer.prepare()
+        x = torch.randn(2 * world, 3, 8, 8, generator=torch.Generator().manual_seed(7))
+        steps = []
+        for _ in range(2):
+            before = [p.detach().clone() for p in model.parameters()]
+            momenta = [trainer.optimizer.state[p]['momentum_buffer'].clone() if p.dim() > 1 else None for p in model.parameters()]
+            if flat:
+                trainer.grads.zero()
+                trainer._backward(trainer.total_loss(trainer.model(shard_batch(x, rank, world))))
+                trainer.grads.pack_all()
+                trainer.grads.all_reduce_flat()
+                trainer.optimizer.step()
+            else:
+                trainer.step(shard_batch(x, rank, world))
+            steps.append((before, [p.grad.clone() for p in model.parameters()], momenta, [p.detach().clone() for p in model.parameters()]))
+        torch.save(steps, '%s.%d' % (out_path, rank))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize('flat', [False, True])
+def test_two_ranks_step_alike(tmp_path, flat):
+    """Both ranks hold the same weights after every step, the gradients are those of the whole batch, and the weights move as the formula has it."""
+    import socket
+    import torch.multiprocessing as mp
+    import hostexec
+    import train_on_host
+    from oracle import ref_cpu as R
+    from unopticalflow_amd.core.config import generate_loss_weights_dict
+    if hostexec.library() is None or train_on_host.library() is None:
+        pytest.skip('needs the ROCm clang++')
+    with socket.socket() as so:
+        so.bind(('127.0.0.1', 0))
+        port = so.getsockname()[1]
+    out = str(tmp_path / 'rank')
+    mp.spawn(_muon_rank, args=(2, port, flat, out), nprocs=2, join=True)
+    ranks = [torch.load('%s.%d' % (out, r)) for r in range(2)]
+    weights = generate_loss_weights_dict(R.default_cfg())
+    x = torch.randn(4, 3, 8, 8, generator=torch.Generator().manual_seed(7))
+    torch.manual_seed(0)
+    model = _Net().double()
+    for a, b in zip(*ranks):
+        assert all(torch.equal(p, q) for p, q in zip(a[0] + a[1] + a[3], b[0] + b[1] + b[3]))
+        before, grads, momenta, after = a
+        with torch.no_grad():
+            for p, v in zip(model.parameters(), before):
+                p.copy_(v)
+        loss = sum(weights[k] * v.mean() for k, v in model(x.double()).items())
+        for p, old, g, exact, m, new in zip(model.parameters(), before, grads, torch.autograd.grad(loss, list(model.parameters())), momenta, after):
+            # (fp32 sums of at most 4 x 36 x 27 terms of a gradient, and the network around them)
+            assert float((g.double() - exact).norm()) <= 2**-24 * 200 * float(exact.norm())
+            if p.dim() < 2:
+                assert not torch.equal(old, new)
+                continue
+            want, _ = _muon(old, g, m, 0.05, 0.95, 0.0, True)
+            plain, _ = _muon(old, g, m, 0.05, 0.95, 0.0, True, torch.float32)
+            step = 0.05 * max(1.0, len(p) / (p.numel() / len(p))) ** 0.5 * p.numel() ** 0.5 * 1.3
+            assert float((new.double() - want).norm()) <= 4 * float((plain.double() - want).norm()) + 16 * 2**-22 * step + 5 * 2**-24 * float(want.norm())
+
+
+YAML = """cfg_name: 'default'
+dataset: 'kitti_depth'
+img_hw: [64, 128]
+num_scales: 3
+num_iterations: 4
+w_ssim: 0.85
+w_flow_smooth: 10.0
+w_flow_consis: 0.01
+h_flow_consist_alpha: 3.0
+h_flow_consist_beta: 0.05
+prepared_base_dir: './none'
+gt_2012_dir: './none'
+gt_2015_dir: './none'
+"""
+
+
+@pytest.mark.parametrize('given,want', [([], ('adam', 0.002, 1e-4)), (['--optimizer', 'muon'], ('muon', 0.002, 1e-4)),
+                                        (['--optimizer', 'muon', '--muon_lr', '0.01', '--lr', '0.5'], ('muon', 0.01, 0.5))])
+def test_the_train_command_passes_its_optimiser_on(tmp_path, monkeypatch, given, want):
+    """What reaches FlowTrainer from the command line."""
+    from unopticalflow_amd import train as cli, tuning
+    seen = {}
+
+    class Reached(Exception):
+        pass
+
+    def trainer(cfg, model, **kw):
+        seen.update(kw, lr=cfg.lr)
+        raise Reached
+    for name, value in (('is_available', lambda: True), ('device_count', lambda: 1), ('set_device', lambda d: None)):
+        monkeypatch.setattr(torch.cuda, name, value)
+    monkeypatch.setattr(tuning, 'default_channels_last', lambda: 0)
+    monkeypatch.setattr(cli, 'init_distributed', lambda *a, **k: (0, 0, 1))
+    monkeypatch.setattr(cli, 'get_model', lambda mode: lambda cfg: type('Model', (), {'to': lambda self, dev: self})())
+    monkeypatch.setattr(cli, 'FlowTrainer', trainer)
+    monkeypatch.chdir(tmp_path)
+    (tmp_path / 'cfg.yaml').write_text(YAML)
+    with pytest.raises(Reached):
+        cli.main(['-c', 'cfg.yaml', '--synthetic', '--no_test', '--miopen_find', '0'] + given)
+    assert (seen['optimizer'], seen['muon_lr'], seen['lr']) == want
+    with pytest.raises(SystemExit):
+        cli.main(['-c', 'cfg.yaml', '--optimizer', 'sgd'])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('graph', ['0', '1'])
+def test_the_train_command_with_muon(tmp_path, monkeypatch, graph):
+    """Four iterations on synthetic triplets, checkpoints, and the last two again from the one in the middle; an Adam checkpoint is refused."""
+    from unopticalflow_amd import train as cli
+    monkeypatch.chdir(tmp_path)
+    (tmp_path / 'cfg.yaml').write_text(YAML)
+    common = ['-c', 'cfg.yaml', '--synthetic', '--no_test', '--miopen_find', '0', '--batch_size', '2', '--log_interval', '1', '--save_interval', '2', '--graph', graph]
+    muon = common + ['--optimizer', 'muon', '--model_dir', 'muon']
+    trainer = cli.main(muon)
+    assert type(trainer.optimizer) is optim.FlowMuon and trainer.iteration == 3
+    again = cli.main(muon + ['--resume', '--iter_start', '1'])
+    assert all(bool(torch.isfinite(p).all()) for p in again.model.parameters())
+    momenta = [again.optimizer.state[p]['momentum_buffer'] for p in again.model.parameters() if p.dim() > 1]
+    assert len(momenta) == 49 and all(m.dtype == torch.float32 and bool(m.any()) for m in momenta)
+    cli.main(common + ['--model_dir', 'adam', '--num_iterations', '2'])
+    with pytest.raises(ValueError):
+        cli.main(common + ['--optimizer', 'muon', '--model_dir', 'adam', '--resume', '--iter_start', '1'])
