@@ -8,6 +8,7 @@ called through the plain-C ABI of ``include/unflow_hip.h`` with raw pointers.
 """
 import ctypes
 import sys
+import weakref
 
 import numpy as np
 import torch
@@ -1776,11 +1777,17 @@ _MATRIX_MAX_SIDE = 1 << 18
 _REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
 
 
+_dispatch_modes, _included, _PRE_DISPATCH = torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+_jit_tracing, _forward_ad = torch._C._is_tracing, torch.autograd.forward_ad
+
+
 def _refuse_tracers(what, jit=True):
     """Tracers that run the Python code and record what torch does in it (make_fx; ``jit``: torch.jit.trace) would see the allocations around a
     kernel and not the kernel: what they recorded would return memory that nothing has written."""
+    if not (_dispatch_modes() or _included(_PRE_DISPATCH) or _jit_tracing()):
+        return
     fx = sys.modules.get('torch.fx.experimental.proxy_tensor')
-    if (jit and torch._C._is_tracing()) or (fx is not None and fx.get_proxy_mode() is not None):
+    if (jit and _jit_tracing()) or (fx is not None and fx.get_proxy_mode() is not None):
         raise RuntimeError('%s is a kernel behind raw pointers: a trace would not hold it' % what)
 
 
@@ -1803,6 +1810,8 @@ def _stream_of(dev):
 
 def _rows_of(t):
     """A [rows, cols] tensor the kernels can walk (adjacent columns, rows a fixed distance apart) and that distance."""
+    if t.is_contiguous():
+        return t, t.shape[1]
     if t.stride(1) == 1 or t.shape[1] == 1:
         ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
         if t.shape[1] <= ld <= _LCE_MAX_DIM:
@@ -1812,58 +1821,65 @@ def _rows_of(t):
 
 
 def _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, need_h, need_w):
-    """-> loss, and what the backward pass takes: (hidden, weight, kept) and (where and how far apart their rows lay, dtype, bytes kept, bytes of
-    its workspace for that layout)."""
+    """-> loss, and what the backward pass takes: (hidden, weight, kept) and (shapes, type, where all lay and how far apart rows were, bytes kept, bytes
+    of its workspace for that layout)."""
     _refuse_tracers('linear_cross_entropy', jit=False)
     dev, dtype = _dev_typed('linear_cross_entropy', hidden, weight)
     (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
-    (N, D), V = hidden.shape, weight.shape[0]
+    shape, wshape = hidden.shape, weight.shape
+    (N, D), V = shape, wshape[0]
     loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
     if N == 0:
-        return loss.zero_(), (hidden, weight, None), None
+        return loss.zero_(), (hidden, weight, None), (shape, wshape, hidden.dtype, None, 0, 0)
     with _on(dev):
         sizes = (ctypes.c_longlong * 3)()                # bytes kept for the backward pass, of the forward's workspace, of the backward's
-        at, ph, pw = ctypes.addressof(sizes), hidden.data_ptr(), weight.data_ptr()
+        at, ph, pw, pt = ctypes.addressof(sizes), hidden.data_ptr(), weight.data_ptr(), target.data_ptr()
         _call('unflow_linear_ce_workspace', ph, ldh, pw, ldw, N, V, D, dtype, need_h, need_w, at, at + 8, at + 16)
-        kept = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
-        ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
-        _call('unflow_linear_ce_fwd_ex', ph, ldh, pw, ldw, target.data_ptr(), N, V, D, dtype, scale, ignore_index, reduction,
-              loss.data_ptr(), kept.data_ptr(), sizes[0], ws.data_ptr(), sizes[1], _stream_of(dev), nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
-    return loss, (hidden, weight, kept), ((ph, ldh, pw, ldw), dtype, sizes[0], sizes[2])
+        kept_bytes = sizes[0]
+        kept = torch.empty(kept_bytes, dtype=torch.uint8, device=dev)
+        ws, pk = torch.empty(sizes[1], dtype=torch.uint8, device=dev), kept.data_ptr()
+        _call('unflow_linear_ce_fwd_ex', ph, ldh, pw, ldw, pt, N, V, D, dtype, scale, ignore_index, reduction,
+              loss.data_ptr(), pk, kept_bytes, ws.data_ptr(), sizes[1], _stream_of(dev), nbytes=(N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
+    return loss, (hidden, weight, kept), (shape, wshape, hidden.dtype, (ph, ldh, pw, ldw, pt, pk), kept_bytes, sizes[2])
+
+
+def _linear_ce_saved_elsewhere(how, dev, needs, hidden, weight, target, kept):
+    """What was saved came back as other tensors, from hooks that offload it: of the same shapes and types, at any place and in any layout."""
+    (N, D), wshape, kind, _, kept_bytes, _ = how
+    if not (hidden.shape == (N, D) and weight.shape == wshape and target.shape == (N,) and kept.shape == (kept_bytes,) and hidden.dtype == weight.dtype == kind and
+            target.dtype == torch.int64 and kept.dtype == torch.uint8 and dev == hidden.device == weight.device == target.device == kept.device):
+        raise RuntimeError('linear_cross_entropy: the saved tensors came back with another shape or type, or on another device')
+    (hidden, ldh), (weight, ldw), target, kept = _rows_of(hidden), _rows_of(weight), target.contiguous(), kept.contiguous()
+    if kept.data_ptr() % 16:
+        kept = kept.clone()
+    where = hidden.data_ptr(), ldh, weight.data_ptr(), ldw
+    size = ctypes.c_longlong()
+    _call('unflow_linear_ce_bwd_workspace', *where, N, wshape[0], D, _DTYPES[kind], *needs, kept_bytes, ctypes.addressof(size))
+    return (hidden, weight, target, kept), (*where, target.data_ptr(), kept.data_ptr()), size.value
 
 
 def _linear_ce_backward(ctx, g):
-    # (what was saved may come back, from hooks that offload it, at another place and in another layout)
-    hidden, weight, target, kept = ctx.saved_tensors
+    saved = ctx.saved_tensors
+    hidden, weight, target, kept = saved
     ignore_index, scale, reduction = ctx.options
     need_h, need_w = ctx.needs_input_grad[:2]
-    (N, D), V = ctx.shape, weight.shape[0]
-    dev = g.device
-    if any(x.device != dev for x in (hidden, weight, target) + (() if kept is None else (kept,))):
-        raise RuntimeError('linear_cross_entropy: the saved tensors came back on other devices than the gradient\'s, %s' % dev)
-    if hidden.shape != ctx.shape or weight.shape != (ctx.classes, D) or target.shape != (N,) or target.dtype != torch.int64:
-        raise RuntimeError('linear_cross_entropy: the saved tensors came back as others than they were')
-    dh = torch.empty((N, D), dtype=hidden.dtype, device=dev) if need_h else None
-    dw = torch.empty((V, D), dtype=weight.dtype, device=dev) if need_w else None
+    shape, wshape, kind, where, kept_bytes, need = ctx.how
+    (N, D), V, dev = shape, wshape[0], g.device
+    dh = torch.empty(shape, dtype=kind, device=dev) if need_h else None
+    dw = torch.empty(wshape, dtype=kind, device=dev) if need_w else None
     if N == 0:
         return dh, dw.zero_() if need_w else None, None, None, None, None
-    where, dtype, kept_bytes, need = ctx.how
-    if _DTYPES.get(hidden.dtype) != dtype or weight.dtype != hidden.dtype or kept.dtype != torch.uint8 or kept.numel() != kept_bytes:
-        raise RuntimeError('linear_cross_entropy: the saved tensors came back as others than they were')
     with _on(dev):
-        (hidden, ldh), (weight, ldw) = _rows_of(hidden), _rows_of(weight)
-        target, kept, g = target.contiguous(), kept.contiguous(), g.contiguous()
-        if kept.data_ptr() % 16:
-            kept = kept.clone()
-        ph, pw = hidden.data_ptr(), weight.data_ptr()
-        if (ph, ldh, pw, ldw) != where:
-            size = ctypes.c_longlong()
-            _call('unflow_linear_ce_bwd_workspace', ph, ldh, pw, ldw, N, V, D, dtype, need_h, need_w, kept_bytes, ctypes.addressof(size))
-            need = size.value
+        was_h, was_w, was_t, was_k = ctx.same
+        if not (was_h() is hidden and was_w() is weight and was_t() is target and was_k() is kept and
+                (hidden.data_ptr(), weight.data_ptr(), target.data_ptr()) == (where[0], where[2], where[4])):
+            saved, where, need = _linear_ce_saved_elsewhere(ctx.how, dev, (need_h, need_w), *saved)
+        ph, ldh, pw, ldw, pt, pk = where
+        g = g.contiguous()
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call('unflow_linear_ce_bwd_ex', ph, ldh, pw, ldw, target.data_ptr(), g.data_ptr(), N, V, D,
-              dtype, scale, ignore_index, reduction, dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None,
-              kept.data_ptr(), kept_bytes, ws.data_ptr(), need, _stream_of(dev),
+        _call('unflow_linear_ce_bwd_ex', ph, ldh, pw, ldw, pt, g.data_ptr(), N, V, D,
+              _DTYPES[kind], scale, ignore_index, reduction, dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None,
+              pk, kept_bytes, ws.data_ptr(), need, _stream_of(dev),
               nbytes=2 * (N + V) * D * hidden.element_size() + 12 * N, shape=(N, V, D))
     return dh, dw, None, None, None, None
 
@@ -1876,7 +1892,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, target, ignore_index, scale, reduction):
         loss, (hidden, weight, kept), ctx.how = _linear_ce_forward(hidden, weight, target, ignore_index, scale, reduction, *ctx.needs_input_grad[:2])
         ctx.options = (ignore_index, scale, reduction)
-        ctx.shape, ctx.classes = tuple(hidden.shape), weight.shape[0]
+        ctx.same = None if kept is None else (weakref.ref(hidden), weakref.ref(weight), weakref.ref(target), weakref.ref(kept))
         ctx.save_for_backward(hidden, weight, target, kept)
         return loss
 
@@ -1918,7 +1934,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
     args = (hidden, weight, flat.contiguous(), int(ignore_index), float(scale), _REDUCTIONS[reduction])
     # (where nothing asks for a gradient the autograd function is passed over; forward-mode derivatives, which it refuses, and torch.jit.trace, which
     # records its call, have to meet it)
-    if (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)) or torch.autograd.forward_ad._current_level >= 0 or torch._C._is_tracing():
+    if (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)) or _forward_ad._current_level >= 0 or _jit_tracing():
         loss = _LinearCrossEntropy.apply(*args)
     else:
         loss = _linear_ce_forward(*args, False, False)[0]
