@@ -51,7 +51,7 @@ __device__ __forceinline__ int exponent_for(float largest) { return largest > 0.
 
 // H and W into packed rows, one launch: the first `blocks_h` workgroups take H (0: H needs no packing), the rest W; a wave takes a row at a time.
 // fp32: the rows' exponents, and the workgroups' largest finite magnitudes of the rows that count (maxima [2][kMaxima]).  Bound by bytes: 11020 rows
-// of 777 fp32 numbers 24 us (34 MB read, 35 written).
+// of 777 fp32 numbers 25 us (34 MB read, 35 written).
 struct Packed { u16 *h, *w; int *eh, *ew; float* maxima; };
 template <class T, int PL, int EL>
 __global__ __launch_bounds__(256) void pack_inputs_kernel(Source h, Source w, int blocks_h, Packed to, long long ldd, int width) {
@@ -98,7 +98,8 @@ template <int PL> __device__ __forceinline__ f32x4 logits_of(const Logits& l, f3
 
 // ---- forward: of each row of a tile of z the maximum (times log2(e), as all that follows) and the sum of exp(z - maximum) over the classes that
 // are not the row's target, and the target's z.  partial [tile column][N].  Bound by the matrix instructions, and for short rows by what a tile's
-// end costs: 8192 rows, 131072 classes of 4096 bf16 6.70 ms = 1313 TFLOP/s; 4096, 32000 of 2048 518 us = 1036; fp32 1013, 10007 of 777 57 us = 276.
+// end costs: 8192 rows, 131072 classes of 4096 bf16 6.3 ms = 1400 TFLOP/s; 4096, 32000 of 2048 470 to 490 us = 1100 to 1140; fp32 1013, 10007 of 777
+// 56 us = 280.
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_forward_kernel(Operand H, Operand W, int width, Logits how,
         const long long* __restrict__ target, float2* __restrict__ partial, float* __restrict__ ztarget) {
@@ -319,8 +320,8 @@ __device__ __forceinline__ float row_of(float2 pair, long long t, long long igno
     return t == ignore ? 0.f : !known ? NAN : own > 0.01f * others ? log1pf(others / own) : (base - zt) * kLn2 + logf(all);
 }
 
-// the tiles' pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup.  4 to 6 us: the latency of a launch and of
-// its loads
+// the tiles' pairs of a row joined in fixed order: R rows x 256 / R shares of the tiles per workgroup.  4 to 10 us: the latency of a launch and
+// of its loads
 template <int R>
 __global__ __launch_bounds__(256) void lce_join_kernel(const float2* __restrict__ partial, int tiles, int N, int V,
         const long long* __restrict__ target, long long ignore, const float* __restrict__ ztarget, Row* __restrict__ stats,
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(1024) void lce_join_reduce_kernel(const float2* __r
 // ---- backward
 // The largest finite magnitudes that workgroups meet in bf16 inputs as pack_inputs_kernel notes them for fp32 ones (rows of 16-byte pieces, zeros
 // behind the last number).  A wave takes a row at a time, four pieces a lane under way together.  Bound by bytes: 139264 rows of 4096
-// 187 us = 6.1 TB/s.
+// 183 us = 6.2 TB/s.
 __global__ __launch_bounds__(256) void lce_magnitudes_kernel(Operand h, Operand w, int pieces, int blocks_h, const long long* __restrict__ target,
         long long ignore, float* __restrict__ maxima) {
     __shared__ unsigned red[4];
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(1024) void lce_largest_upstream_kernel(Upstream u, 
 
 // Transposes of a piece of W and (with the first piece) of H, one launch: the first `blocks_w` workgroups take W.  All but fp16, which goes as it
 // is: with the exponent of the largest of the `counts` magnitudes that were noted, left in `ex`.  Bound by bytes: 8192 classes of 4096 bf16
-// 31 to 39 us = 3.4 to 4.3 TB/s.
+// 40 us = 3.4 TB/s.
 struct Columns { Source s; u16* dst; long long ldd; int width; const float* maxima; int counts; };
 template <class T> constexpr bool kScaled = !__is_same(T, _Float16);
 template <class T, int PL>
@@ -481,7 +482,7 @@ constexpr int kProbabilityExponent = 14;
 
 // a piece of G and of its transpose: classes [v0, v0 + vp).  G [N][packed vp] holds p - [v = t] (0 where the row is ignored), GT [vp][packed N] the
 // same times the row's upstream gradient relative to the largest; columns behind N and vp up to the packed width are zero.  Bound by the matrix
-// instructions, and then by its stores: 8192 rows, 8192 classes of 4096 bf16 460 us = 1195 TFLOP/s, 268 MB of it written.
+// instructions, and then by its stores: 8192 rows, 8192 classes of 4096 bf16 441 us = 1250 TFLOP/s, 268 MB of it written.
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand H, Operand W, int width, Logits how,
         const Row* __restrict__ stats, Upstream up, int v0, int vp, int V, u16* __restrict__ G, long long ldg,
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_gradient_kernel(Operand
 
 // The two products of a piece, one launch: job 0 is dH += G W, job 1 dW = G^T H.  C = A B^T in `shares` shares of what is summed.  A job without
 // `sums` is one share and goes to the gradient as it is; else the shares' accumulators go to fp32 sums [shares][rows of A][ldc], added to what
-// is there unless it is the first piece.  Bound by the matrix instructions: both products of that piece 875 us = 1257 TFLOP/s.
+// is there unless it is the first piece.  Bound by the matrix instructions: both products of that piece 855 us = 1290 TFLOP/s.
 struct Product { Operand A, B; int width, shares, tiles; float* sums; long long ldc; int first; void* out; int by_h; };
 
 // what turns a job's sums into gradients: the uniform factor, and the row's own (dH; for dW it is in GT, relative to the largest)
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void lce_products_kernel(Product
 }
 
 // gradients = sums over the shares, in order, times the factors; one launch for the jobs that have sums (blocks of the first, then of the second).
-// Bound by bytes: 4096 x 2048 to bf16 10.5 us = 4.8 TB/s.
+// Bound by bytes: 4096 x 2048 to bf16 11 us = 4.5 TB/s.
 template <class T_>
 __global__ __launch_bounds__(256) void lce_finish_kernel(Product a, Product b, int blocks_a, const Exponents* __restrict__ ex, Upstream up) {
     const bool second = (int)blockIdx.x >= blocks_a;

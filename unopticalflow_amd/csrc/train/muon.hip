@@ -6,7 +6,8 @@
 //
 // S and Q are symmetric: their tiles above the diagonal are not computed but written as the mirror of those below, so a step costs
 // m^2 n + m^3 + 2 m^2 n operations instead of 4 m^2 n + 2 m^3.  The products bound large matrices; a list of small ones is bound by launches,
-// so every phase is one launch over the tiles of all matrices (a wave finds its matrix in a table of running tile counts), 3 launches a step.
+// so every phase is one launch over the tiles of all matrices (a wave finds its matrix in a table of running tile counts), 3 launches a step, 4
+// where S is summed in shares.
 // Matrices of up to 32 rows or columns, where nothing larger is in the list, have kernels of their own (in the middle of this file).
 //
 // Numbers of the tiles (mfma16.h): every type is iterated on as two fp16 planes (22 bits, products and sums as in fp32).  One plane would
@@ -214,7 +215,8 @@ __device__ __forceinline__ void symmetric_store(TileT& T, char* lds, u16* __rest
 }
 
 // ---- S = X X^T: lower tiles.  A problem of one share writes S, one of several leaves fp32 tiles for join_kernel.  Bound by the matrix
-// instructions: 4096 x 4096 192 us = 1120 TFLOP/s of fp16 products (three for one of fp32)
+// instructions: 4096 x 4096 175 to 183 us = 1130 to 1180 TFLOP/s of fp16 products (three for one of
+// fp32)
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void square_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
         const int* __restrict__ classes, Exponents ex, char* __restrict__ ws) {
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Problem* __restrict__ t
     }
 }
 
-// ---- Q = a I + b S + c S S: lower tiles.  Bound by the matrix instructions: 4096 x 4096 200 us
+// ---- Q = a I + b S + c S S: lower tiles.  Bound by the matrix instructions: 4096 x 4096 182 to 190 us
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* __restrict__ table, const int* __restrict__ ends, int count,
         const int* __restrict__ classes, float a, float b, float c, Exponents ex,
@@ -311,8 +313,8 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void poly_kernel(const Problem* 
     symmetric_store(T, lds, (u16*)(ws + p.Q), ld, p.m, tm, tn, [&](int i, int j) { return T.acc[i][j]; });
 }
 
-// ---- X <- Q X.  LAST: the output, or the parameter's update.  Bound by the matrix instructions (4096 x 4096 335 us = 1230 TFLOP/s of fp16
-// products), for the weights above as much by writing X both ways (343 us = 900 TFLOP/s, 400 MB written): S sums over the columns of X and the next
+// ---- X <- Q X.  LAST: the output, or the parameter's update.  Bound by the matrix instructions (4096 x 4096 306 to 317 us = 1300 to 1350 TFLOP/s
+// of fp16 products), for the weights above as much by writing X both ways (315 us = 980 TFLOP/s, 400 MB written): S sums over the columns of X and the next
 // X over its rows, and both operands of a product lie along what is summed
 struct Update { float keep, lr; };                                   // 1 - lr wd, lr
 template <class TileT, bool LAST, bool STEP, class T>
