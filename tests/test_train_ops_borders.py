@@ -638,3 +638,22 @@ def test_the_train_command_with_muon(tmp_path, monkeypatch, graph):
     cli.main(common + ['--model_dir', 'adam', '--num_iterations', '2'])
     with pytest.raises(ValueError):
         cli.main(common + ['--optimizer', 'muon', '--model_dir', 'adam', '--resume', '--iter_start', '1'])
+
+
+@pytest.mark.parametrize('rows,dim', [(20, 24), (64, 24), (65, 24), (100, 200), (20, 3)])
+@pytest.mark.parametrize('outlier', [2.0**10, 2.0**23, 2.0**30])
+def test_columns_far_larger_than_the_rest(device, rows, dim, outlier):
+    """fp32 rows with one number `outlier` times the others, whose weight is as much smaller.  Up to 64 rows (of 4 numbers and more) fp32 products;
+    beyond, a number x of a row whose largest is M is held to 2^-22 |x| + 2^-39 M, so that a logit is off by what test_train_ops.py derives and
+    2^-39 (M_h sum |w| + M_w sum |h|) on top."""
+    h, w, t = _inputs(rows, 50, dim, torch.float32, device, ignored=0.0)
+    h[:, 1] *= outlier
+    w[:, 1] /= outlier
+    losses = ops.linear_cross_entropy(h, w, t, reduction='none').double()
+    hd, wd = h.double(), w.double()
+    z = hd @ wd.T
+    exact = z.logsumexp(1) - z.gather(1, t[:, None])[:, 0]
+    dz = (dim * 2**-24 + 2**-20) * float((hd.abs() @ wd.abs().T).max())
+    if rows > 64 or dim < 4:
+        dz += 2**-39 * float((hd.abs().amax(1)[:, None] * wd.abs().sum(1)[None] + hd.abs().sum(1)[:, None] * wd.abs().amax(1)[None]).max())
+    assert bool(((losses - exact).abs() <= 2 * dz + (2 * float(z.abs().max()) + 128) * 2**-23).all())

@@ -1907,8 +1907,10 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, scale=1.0, r
 
     ``hidden`` [..., D] and ``weight`` [V, D] are fp32, bf16 or fp16 (one type; any row stride); ``target`` [...] is int64.  The classes may be
     a vocabulary, or the positions of another feature map that a position is to be matched to (``scale`` = 1 / temperature).  The loss is
-    fp32; both gradients come in the inputs' type, from sums in fp32 (fp32 inputs: products and sums of fp32 accuracy; in the gradients' sums
-    numbers below 2^-17 of the largest of their matrix lose digits, of bf16 matrices below 2^-31).  ``reduction``: 'mean' over the rows that
+    fp32; both gradients come in the inputs' type, from sums in fp32.  fp32 inputs: the loss of up to 64 rows from products in fp32; that of more
+    rows, and the gradients, from numbers of 22 bits, of which those below 2^-17 of the largest of their row (in the gradients' sums: of their
+    matrix) are held to 2^-39 of that, so an outlier of 2^30 in a row leaves 9 bits of the others.  16-bit inputs: products of the numbers as they
+    are; in the gradients' sums probabilities of 11 bits, and bf16 numbers below 2^-31 of the largest of their matrix lose digits.  ``reduction``: 'mean' over the rows that
     are not ignored (0 if there are none), 'sum', or 'none' (the shape of ``target``).  A row whose target is ``ignore_index`` has loss 0
     and no part in the gradients, whatever it holds; any other target outside [0, V) makes its row's loss, and
     the gradients it reaches, NaN.  Results are bitwise reproducible.
