@@ -429,8 +429,8 @@ int unflow_prepare_triplets(const uint8_t* src, const long long* offsets, const 
  *   (fp32, or rows that are not multiples of 16 bytes) as they are packed.
  * The backward pass takes the upstream gradient gout ([N] for reduction 0, else [1]) and writes dhidden [N, D] and / or dweight [V, D] (dense,
  * in the inputs' type; NULL: not wanted), working through the classes in pieces.  Sums are fp32, in fixed order (bitwise reproducible).
- * fp32 inputs are products of fp32 in the loss of up to 64 rows (of 4 numbers or more), else numbers of 22 bits that are held to 2^-39 of the largest
- * of their row (in the gradients' sums of their matrix) at best.
+ * fp32 inputs are multiplied in fp32 in the loss of up to 64 rows (of 4 numbers or more); else they are numbers of 22 bits, none held finer than 2^-39
+ * of the largest of its row (in the gradients' sums: of its matrix).
  * unflow_linear_ce_workspace() says how many bytes are kept and how many each pass needs as workspace (256-byte aligned; its contents mean nothing
  * between calls).  The alignment of hidden and weight is part of the question: ask with the pointers of the call.  kept_bytes says with its last two
  * bits which inputs the buffer holds packed (1 hidden, 2 weight); the _ex forms take it with the buffer and refuse any other size.
